@@ -65,11 +65,28 @@ SIGNATURES: dict[str, list] = {
     "ckv_attention_workspace_size": [_i32, _i32, _i32, _i32, _i32],
     "ckv_attention_launches": [_i32, _i32, _i32, _i32, _i32, _i64],
     "ckv_attention": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _p],
+    "ckv_kv8_write": [_p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                      _i32, _i32, _i32, _i32, _p],
+    "ckv_kv8_read": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p],
+    "ckv_block_digest": [_p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _i32, _i32, _i32, _p],
+    "ckv_attention_kv8_workspace_size": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_kv8_launches": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_kv8": [_p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p, _i64, _p],
+    "ckv_block_select_workspace_size": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_block_select_launches": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_block_select": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p],
+    "ckv_attention_blocks_workspace_size": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_blocks_launches": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_blocks": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _p],
+    "ckv_attention_blocks_kv8": [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p,
+                                 _i64, _p],
     "ckv_gemv": [_p, _p, _p, _i32, _i32, _i32, _p],
     "ckv_log_softmax": [_p, _i32, _p, _p],
     "ckv_greedy_next": [_p, _i32, _p, _p, _p],
 }
-_RESTYPES = {"ckv_version": C.c_char_p, "ckv_last_error": C.c_char_p, "ckv_attention_workspace_size": C.c_int64}
+_RESTYPES = {"ckv_version": C.c_char_p, "ckv_last_error": C.c_char_p, "ckv_attention_workspace_size": C.c_int64,
+             "ckv_attention_kv8_workspace_size": C.c_int64, "ckv_block_select_workspace_size": C.c_int64,
+             "ckv_attention_blocks_workspace_size": C.c_int64}
 
 CKV_OK, CKV_ERR_ARG, CKV_ERR_CUDA, CKV_ERR_DEVICE, CKV_ERR_UNSUPPORTED = range(5)
 DEV_ERR_BITS = {
@@ -77,6 +94,7 @@ DEV_ERR_BITS = {
     0x2: "a page id outside the pool was skipped",
     0x4: "the selection kept a position that was never computed",
     0x8: "a position or index outside its range was skipped",
+    0x10: "a NaN or infinity was stored saturated in an 8-bit cache",
 }
 
 _lock = threading.Lock()

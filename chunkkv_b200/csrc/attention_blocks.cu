@@ -1,0 +1,695 @@
+// Attention of few query rows over 16-key blocks streamed straight from HBM: one or a few
+// tokens over a whole 8-bit cache (decode), and any number of tokens over the blocks listed
+// for each of them (8-bit or bf16 cache).
+//
+// Such calls read every key for at most 16 query rows, so they are bound by the cache's
+// bytes; a 128-row tcgen05 tile would be nearly empty.  The kernel keeps the bytes moving:
+// a warp takes whole blocks, loads the next block's K and V into registers (4 KiB per warp
+// at head_dim 128 in 8 bits) while it works on the current one, and uses mma.sync
+// m16n8k16 with the roles turned round: the 16 keys of a block are the M rows, the up to 8
+// query rows the N columns, so nothing is padded for groups of up to 8 heads.
+//   S^T [16 keys x 8 rows]  = K Q^T        A = K, contraction over head_dim
+//   O^T [dims x 8 rows]    += V^T P^T      A = V^T, contraction over the 16 keys
+// The contraction over head_dim may be permuted if K and Q agree, so quad member c of a
+// lane group holds dims [c * D/4, (c + 1) * D/4) of keys g and g + 8 (g = lane / 4): plain
+// 16-byte loads, each row read whole by four lanes.  For V, lane (g, c) loads dims
+// [g * D/8, (g + 1) * D/8) of keys 2c, 2c+1, 2c+8, 2c+9; pairing two keys' bytes with one
+// byte permutation gives the A operand, so V is transposed without shared memory.  P^T is
+// turned into the B operand by movmatrix.
+// 8-bit codes become fp16 exactly (e4m3 by cvt, int8 by adding 1024), so no value is
+// rounded before the tensor core: scores are q (fp16, scaled by a power of two per row) .
+// code, times the block's fp32 key scale; P is multiplied by the block's value scale
+// relative to a running power-of-two reference and rounded to fp16 (2^-12), accumulators,
+// maxima and sums are fp32.  With a bf16 cache P goes in as two bf16 parts (2^-17).
+// The online maximum is lazy: O is rescaled when a row's maximum grew by more than 2^8.
+#include <algorithm>
+
+#include "ckv_common.cuh"
+
+CKV_DEFINE_ERR_WORD(attention_blocks)
+
+namespace ckv {
+namespace {
+
+constexpr int kBlk = CKV_PAGE_TOKENS;
+constexpr int kWarps = 4;  // per CTA; three CTAs per SM
+constexpr float kLazy = 8.0f;       // log2 units
+constexpr float kPBias = 64.0f;     // P * value scale / reference is at most 2^8 * 2^6 in fp16
+enum { kBf16 = 0, kInt8 = 1, kE4m3 = 2 };
+
+struct Args {
+  const uint16_t* q;  // [m][Hq][D]
+  const uint8_t *k, *v;  // [H][rows][D], 1 or 2 bytes per value
+  const float *ks, *vs;  // [H][n_blocks] (8 bits)
+  const int32_t* positions;
+  const int32_t* blocks;  // [m][H][top] (listed form), ascending, -1 past the end
+  uint16_t* out;          // [m][Hq][D]
+  float* part_o;          // [splits][tiles][H][8 NT][D]
+  float2* part_ml;        // [splits][tiles][H][8 NT]
+  int64_t head_rows;      // cache rows per head
+  int m, Hq, Hk, n_ctx, n_blocks, top, splits, head_tiles;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int CT>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (CT == kBf16) mma_bf16(c, a0, a1, a2, a3, b0, b1);
+  else mma_f16(c, a0, a1, a2, a3, b0, b1);
+}
+// four codes -> two pairs of fp16, exactly: (0, 1) and (2, 3)
+template <int CT>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CT == kE4m3) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  } else {
+    // 0x6400 + u is the fp16 number 1024 + u, u = code + 128: minus 1152 is the code
+    const uint32_t u = w ^ 0x80808080u, magic = 0x64646464u;
+    uint32_t a, b;
+    a = __byte_perm(u, magic, 0x4140);
+    b = __byte_perm(u, magic, 0x4342);
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
+  }
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint2 ld_stream2(const void* p) {
+  uint2 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  return r;
+}
+
+// One block's K and V as a lane holds them.
+template <int HD, int CT>
+struct Block {
+  static constexpr int ES = CT == kBf16 ? 2 : 1;
+  static constexpr int KW = HD / 4 * ES / 4;  // 32-bit words of K per key and lane
+  static constexpr int VW = HD / 8 * ES / 4;  // of V
+  uint32_t k[2][KW];  // keys g, g + 8
+  uint32_t v[4][VW];  // keys 2c, 2c + 1, 2c + 8, 2c + 9
+  float ks, vs;
+
+  __device__ __forceinline__ void load(const Args& a, int hk, int b, int last_key, int lane) {
+    const int g = lane >> 2, c = lane & 3;
+    const int64_t row0 = int64_t(hk) * a.head_rows + int64_t(b) * kBlk;
+    const int vis = last_key - b * kBlk;  // rows past it are not read: zeros
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* p = a.k + ((row0 + g + 8 * i) * HD + c * (HD / 4)) * ES;
+      if (g + 8 * i <= vis) {
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) {
+          const uint4 x = ld_stream(p + 4 * w);
+          k[i][w] = x.x, k[i][w + 1] = x.y, k[i][w + 2] = x.z, k[i][w + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < KW; ++w) k[i][w] = 0u;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 2 * c + (i & 1) + 8 * (i >> 1);
+      const uint8_t* p = a.v + ((row0 + key) * HD + g * (HD / 8)) * ES;
+      if (key <= vis) {
+        if constexpr (VW >= 4) {
+#pragma unroll
+          for (int w = 0; w < VW; w += 4) {
+            const uint4 x = ld_stream(p + 4 * w);
+            v[i][w] = x.x, v[i][w + 1] = x.y, v[i][w + 2] = x.z, v[i][w + 3] = x.w;
+          }
+        } else {
+          const uint2 x = ld_stream2(p);
+          v[i][0] = x.x, v[i][1] = x.y;
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) v[i][w] = 0u;
+      }
+    }
+    if constexpr (CT != kBf16) {
+      ks = __ldg(a.ks + int64_t(hk) * a.n_blocks + b);
+      vs = __ldg(a.vs + int64_t(hk) * a.n_blocks + b);
+    }
+  }
+};
+
+// Running state of a warp: for each of its 8 NT query rows a maximum and a sum, and O.
+template <int HD, int CT, int NT>
+struct State {
+  static constexpr int KSTEPS = HD / 16;
+  uint32_t qf[NT][KSTEPS][2];
+  float f[NT][2];      // per query row 2c, 2c + 1: score factor (log2 domain)
+  int lim[NT][2];      // last visible key
+  float mx[NT][2], l[NT][2];
+  float ref;           // value-scale reference (power of two; 0 before the first block)
+  float o[NT][KSTEPS][4];  // dims g * HD/8 + 2t (+ 1) x rows 2c, 2c + 1
+
+  __device__ __forceinline__ void step(const Block<HD, CT>& x, int b, int lane) {
+    const int g = lane >> 2;
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+    for (int t = 0; t < KSTEPS; ++t) {
+      uint32_t a0, a1, a2, a3;
+      if constexpr (CT == kBf16) {
+        a0 = x.k[0][2 * t], a2 = x.k[0][2 * t + 1], a1 = x.k[1][2 * t], a3 = x.k[1][2 * t + 1];
+      } else {
+        widen<CT>(x.k[0][t], a0, a2);
+        widen<CT>(x.k[1][t], a1, a3);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma<CT>(s[n], a0, a1, a2, a3, qf[n][t][0], qf[n][t][1]);
+    }
+    const int key = b * kBlk + g;
+    bool grow = false;
+    float top[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float fk = CT == kBf16 ? f[n][r] : f[n][r] * x.ks;
+        s[n][r] = key <= lim[n][r] ? s[n][r] * fk : -INFINITY;
+        s[n][2 + r] = key + 8 <= lim[n][r] ? s[n][2 + r] * fk : -INFINITY;
+        float t = fmaxf(s[n][r], s[n][2 + r]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+        top[n][r] = t;
+        grow |= t > mx[n][r] + kLazy || (mx[n][r] == -INFINITY && t > -INFINITY);
+      }
+    if constexpr (CT != kBf16) grow |= x.vs > ref;
+    if (__any_sync(0xffffffffu, grow)) {
+      float rs = 1.0f;
+      if constexpr (CT != kBf16) {
+        if (x.vs > ref) {  // the same for the whole warp
+          // the next power of two at or above vs
+          const uint32_t bits = __float_as_uint(x.vs);
+          const float up = __uint_as_float((bits + 0x007fffffu) & 0x7f800000u);
+          rs = ref / up;
+          ref = up;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float m_new = fmaxf(mx[n][r], top[n][r]);
+          const float corr = mx[n][r] == -INFINITY ? 0.f : ex2_approx(mx[n][r] - m_new);
+          l[n][r] *= corr;
+          mx[n][r] = m_new;
+#pragma unroll
+          for (int t = 0; t < KSTEPS; ++t) {
+            o[n][t][r] *= corr * rs;
+            o[n][t][2 + r] *= corr * rs;
+          }
+        }
+    }
+    const float vn = CT == kBf16 ? 1.0f : (ref > 0.f ? x.vs * (kPBias / ref) : 0.f);
+    uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float base = mx[n][e & 1] == -INFINITY ? 0.f : mx[n][e & 1];  // no visible key yet: P = 0, not NaN
+        p[e] = ex2_approx(s[n][e] - base);
+        l[n][e & 1] += p[e];
+      }
+      if constexpr (CT == kBf16) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t hi = pack_bf2(p[2 * i], p[2 * i + 1]);
+          ph[n][i] = transpose8(hi);
+          pl[n][i] = transpose8(pack_bf2(p[2 * i] - lo_bf(hi), p[2 * i + 1] - hi_bf(hi)));
+        }
+      } else {
+        ph[n][0] = transpose8(pack_h2(p[0] * vn, p[1] * vn));
+        ph[n][1] = transpose8(pack_h2(p[2] * vn, p[3] * vn));
+      }
+    }
+    if constexpr (CT == kBf16) {
+#pragma unroll
+      for (int w = 0; w < KSTEPS; ++w) {
+        const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5410), a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7632);
+        const uint32_t a2 = __byte_perm(x.v[2][w], x.v[3][w], 0x5410), a3 = __byte_perm(x.v[2][w], x.v[3][w], 0x7632);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_bf16(o[n][w], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+          mma_bf16(o[n][w], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int w = 0; w < KSTEPS / 2; ++w) {
+        // keys 2c, 2c+1 (and 2c+8, 2c+9) of dims 4w .. 4w+3, two keys of a dim side by side
+        uint32_t a0, a1, a2, a3;
+        widen<CT>(__byte_perm(x.v[0][w], x.v[1][w], 0x5140), a0, a1);
+        widen<CT>(__byte_perm(x.v[2][w], x.v[3][w], 0x5140), a2, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+        widen<CT>(__byte_perm(x.v[0][w], x.v[1][w], 0x7362), a0, a1);
+        widen<CT>(__byte_perm(x.v[2][w], x.v[3][w], 0x7362), a2, a3);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w + 1], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+      }
+    }
+  }
+};
+
+template <int HD>
+struct Merge {
+  static constexpr int STRIDE = HD + 4;
+};
+
+// grid: (splits, row tiles, KV heads).  Dense (LISTED = false): tile y holds the packed rows
+// (token, head of the group) [8 NT y, 8 NT (y + 1)) of its KV head.  Listed: tile y is head
+// tile y % head_tiles of token y / head_tiles, and the split takes its share of the list.
+template <int HD, int CT, int NT, bool LISTED>
+__global__ void __launch_bounds__(kWarps * 32, (CT == kBf16 || NT == 2) ? 2 : 3)
+    attention_blocks_kernel(const __grid_constant__ Args a) {
+  constexpr int KSTEPS = HD / 16, ROWS = 8 * NT;
+  __shared__ __align__(16) float s_o[kWarps][ROWS][HD + 4];
+  __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int G = a.Hq / a.Hk;
+  const int hk = blockIdx.z, split = blockIdx.x;
+  const int tile = blockIdx.y;
+  const int tok0 = LISTED ? tile / a.head_tiles : 0;
+  const int row0 = LISTED ? tok0 * G + (tile % a.head_tiles) * ROWS : tile * ROWS;  // packed row
+  const int row_end = LISTED ? tok0 * G + G : a.m * G;
+  pdl_wait();
+  pdl_launch_next();
+
+  State<HD, CT, NT> st;
+  int last = -1;  // last key any row of the tile sees
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    // as an operand owner: query row 8n + g, dims [c * HD/4, ..)
+    const int pr = row0 + 8 * n + g;
+    const bool ok = pr < row_end;
+    const int tok = ok ? pr / G : 0;
+    int p = -1;
+    if (ok) {
+      p = a.positions[tok];
+      if (p >= a.n_ctx) {
+        if (split == 0 && hk == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
+        p = a.n_ctx - 1;
+      }
+      p = max(p, -1);
+    }
+    uint32_t w[HD / 8];
+#pragma unroll
+    for (int i = 0; i < HD / 8; i += 4) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (ok)
+        x = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD + c * (HD / 4)) + i / 4);
+      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+    }
+    float factor = a.scale_log2;
+    if constexpr (CT == kBf16) {
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        st.qf[n][t][0] = w[2 * t];
+        st.qf[n][t][1] = w[2 * t + 1];
+      }
+    } else {
+      // to fp16 through a power of two that puts the row's largest value in [2^14, 2^15):
+      // exact down to 2^-38 of it
+      uint32_t mag = 0;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) mag = __vmaxu2(mag, w[i] & 0x7fff7fffu);
+      uint32_t am = max(mag & 0xffffu, mag >> 16);
+      am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      const int e = int(am >> 7);  // biased exponent of the largest value
+      int sh = 14 + 127 - e;       // multiply by 2^sh
+      sh = am == 0 ? 0 : max(-126, min(sh, 126));
+      const float up = __uint_as_float(uint32_t(sh + 127) << 23);
+      factor *= __uint_as_float(uint32_t(127 - sh) << 23);
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        st.qf[n][t][0] = pack_h2(lo_bf(w[2 * t]) * up, hi_bf(w[2 * t]) * up);
+        st.qf[n][t][1] = pack_h2(lo_bf(w[2 * t + 1]) * up, hi_bf(w[2 * t + 1]) * up);
+      }
+    }
+    // as a column owner: rows 8n + 2c and 8n + 2c + 1
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      st.f[n][r] = __shfl_sync(0xffffffffu, factor, 4 * (2 * c + r));
+      st.lim[n][r] = __shfl_sync(0xffffffffu, p, 4 * (2 * c + r));
+      st.mx[n][r] = -INFINITY;
+      st.l[n][r] = 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < KSTEPS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[n][t][e] = 0.f;
+    last = max(last, __reduce_max_sync(0xffffffffu, p));
+  }
+  st.ref = 0.f;
+
+  const int nb = (last + kBlk) / kBlk;  // visible blocks
+  const int n_items = LISTED ? a.top : nb;
+  const int per = (n_items + a.splits - 1) / a.splits;
+  const int i1 = min(n_items, (split + 1) * per);
+  const int32_t* list = LISTED ? a.blocks + (int64_t(tok0) * a.Hk + hk) * a.top : nullptr;
+  // item i's block, or -1 when there is none (past the list's end, out of range, not ascending)
+  auto block_of = [&](int i) -> int {
+    if (i >= i1) return -1;
+    if constexpr (!LISTED) return i;
+    const int b = __ldg(list + i);
+    if (b == -1) return -1;
+    if (b < 0 || b >= a.n_blocks || (i > 0 && __ldg(list + i - 1) >= b)) {
+      if (lane == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
+      return -1;
+    }
+    return b < nb ? b : -1;  // wholly past the row's position: nothing visible
+  };
+  int i = split * per + warp;
+  Block<HD, CT> cur, nxt;
+  int b = block_of(i);
+  if (b >= 0) cur.load(a, hk, b, last, lane);
+  for (; i < i1; i += kWarps) {
+    const int bn = block_of(i + kWarps);
+    if (bn >= 0) nxt.load(a, hk, bn, last, lane);
+    if (b >= 0) st.step(cur, b, lane);
+    cur = nxt;
+    b = bn;
+  }
+
+  // the warps' states meet in shared memory
+  const float oscale = CT == kBf16 ? 1.0f : st.ref / kPBias;
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float l = st.l[n][r];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      const int row = 8 * n + 2 * c + r;
+      if (g == 0) {
+        s_m[warp][row] = st.mx[n][r];
+        s_l[warp][row] = l;
+      }
+#pragma unroll
+      for (int t = 0; t < KSTEPS; t += 2)
+        *reinterpret_cast<float4*>(&s_o[warp][row][g * (HD / 8) + 2 * t]) =
+            make_float4(st.o[n][t][r] * oscale, st.o[n][t][2 + r] * oscale, st.o[n][t + 1][r] * oscale,
+                        st.o[n][t + 1][2 + r] * oscale);
+    }
+  __syncthreads();
+  constexpr int QV = HD / 4;  // float4 columns of a row
+  const int64_t prow0 = ((int64_t(split) * gridDim.y + tile) * a.Hk + hk) * ROWS;
+  for (int j = threadIdx.x; j < ROWS * QV; j += kWarps * 32) {
+    const int row = j / QV, col = (j - row * QV) * 4;
+    const int pr = row0 + row;
+    if (pr >= row_end) continue;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][row]);
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float wt = ex2_approx(s_m[w][row] - m);
+        const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][col]);
+        l = fmaf(wt, s_l[w][row], l);
+        o.x = fmaf(wt, x.x, o.x);
+        o.y = fmaf(wt, x.y, o.y);
+        o.z = fmaf(wt, x.z, o.z);
+        o.w = fmaf(wt, x.w, o.w);
+      }
+    }
+    if (a.splits > 1) {
+      *reinterpret_cast<float4*>(a.part_o + (prow0 + row) * HD + col) = o;
+      if (col == 0) a.part_ml[prow0 + row] = make_float2(m, l);
+    } else {
+      const float inv = l > 0.f ? 1.0f / l : 0.f;
+      const int tok = pr / G;
+      *reinterpret_cast<uint2*>(a.out + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD + col) =
+          make_uint2(pack_bf2(o.x * inv, o.y * inv), pack_bf2(o.z * inv, o.w * inv));
+    }
+  }
+}
+
+// Joins the splits: out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s.  A CTA takes one
+// packed row of one KV head; HD / 4 lanes hold four columns each, the other lane groups take
+// other splits, and the groups meet in shared memory.
+template <int HD>
+__global__ void __launch_bounds__(256) attention_blocks_join_kernel(const __grid_constant__ Args a, int tiles, int rows_per_tile,
+                                                                    int listed) {
+  constexpr int QV = HD / 4, GROUPS = 256 / QV;
+  __shared__ float s_red[8];
+  __shared__ float4 s_acc[GROUPS][QV];
+  __shared__ float s_l[GROUPS];
+  const int hk = blockIdx.y;
+  const int G = a.Hq / a.Hk;
+  int tile, row;
+  const int pr = blockIdx.x;  // packed row: token * G + head of the group
+  const int tok = pr / G;
+  if (listed) {
+    const int gi = pr - tok * G;
+    tile = tok * a.head_tiles + gi / rows_per_tile;
+    row = gi % rows_per_tile;
+  } else {
+    tile = pr / rows_per_tile;
+    row = pr % rows_per_tile;
+  }
+  const int grp = threadIdx.x / QV, col = (threadIdx.x % QV) * 4;
+  pdl_wait();
+  pdl_launch_next();
+  const int64_t stride = int64_t(tiles) * a.Hk * rows_per_tile;
+  const int64_t at = (int64_t(tile) * a.Hk + hk) * rows_per_tile + row;
+  float m = -INFINITY;
+  for (int s = threadIdx.x; s < a.splits; s += 256) m = fmaxf(m, __ldcg(&a.part_ml[s * stride + at].x));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = s_red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) m = fmaxf(m, s_red[i]);
+  float l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (m > -INFINITY) {
+#pragma unroll 4
+    for (int s = grp; s < a.splits; s += GROUPS) {
+      const float2 ml = __ldcg(&a.part_ml[s * stride + at]);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + (s * stride + at) * HD + col));
+      const float wt = ex2_approx(ml.x - m);
+      l = fmaf(wt, ml.y, l);
+      o.x = fmaf(wt, x.x, o.x);
+      o.y = fmaf(wt, x.y, o.y);
+      o.z = fmaf(wt, x.z, o.z);
+      o.w = fmaf(wt, x.w, o.w);
+    }
+  }
+  s_acc[grp][threadIdx.x % QV] = o;
+  if (threadIdx.x % QV == 0) s_l[grp] = l;
+  __syncthreads();
+  if (threadIdx.x < QV) {
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) {
+      const float4 x = s_acc[i][threadIdx.x];
+      o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+      l += s_l[i];
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    *reinterpret_cast<uint2*>(a.out + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD + col) =
+        make_uint2(pack_bf2(o.x * inv, o.y * inv), pack_bf2(o.z * inv, o.w * inv));
+  }
+}
+
+struct Plan {
+  int nt, tiles, head_tiles, splits;
+  int64_t bytes;
+};
+
+// Rows of one KV head in tiles of 8 (or 16), and the blocks split over CTAs until about
+// three CTAs per SM run, but no finer than one block per warp.
+Plan plan(int m, int G, int Hk, int HD, int items, bool listed) {
+  Plan p;
+  p.nt = (listed ? G : int64_t(m) * G) > 8 ? 2 : 1;
+  p.head_tiles = listed ? ceil_div(G, 8 * p.nt) : 1;
+  p.tiles = listed ? m * p.head_tiles : ceil_div(int64_t(m) * G, 8 * p.nt);
+  const int64_t ctas = int64_t(p.tiles) * Hk;
+  const int want = int(std::min<int64_t>(std::max<int64_t>(1, 3 * num_sms() / ctas), ceil_div(items, kWarps)));
+  p.splits = std::max(1, want);
+  p.bytes = p.splits > 1 ? int64_t(p.splits) * ctas * 8 * p.nt * (int64_t(HD) * 4 + 8) : 0;
+  return p;
+}
+
+template <int HD, int CT, int NT, bool LISTED>
+int launch(Args a, const Plan& p, void* workspace, cudaStream_t stream) {
+  if (p.splits > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(p.splits) * p.tiles * a.Hk * 8 * NT * HD);
+  }
+  a.splits = p.splits;
+  a.head_tiles = p.head_tiles;
+  launch_pdl(attention_blocks_kernel<HD, CT, NT, LISTED>, dim3(p.splits, p.tiles, a.Hk), dim3(kWarps * 32), 0, stream, a);
+  CKV_LAUNCH_CHECK("ckv_attention_blocks");
+  if (p.splits > 1) {
+    launch_pdl(attention_blocks_join_kernel<HD>, dim3(a.m * (a.Hq / a.Hk), a.Hk), dim3(256), 0, stream, a, p.tiles, 8 * NT,
+               int(LISTED));
+    CKV_LAUNCH_CHECK("ckv_attention_blocks(join)");
+  }
+  return CKV_OK;
+}
+
+template <int HD, int CT, bool LISTED>
+int launch_nt(const Args& a, const Plan& p, void* workspace, cudaStream_t stream) {
+  return p.nt == 1 ? launch<HD, CT, 1, LISTED>(a, p, workspace, stream) : launch<HD, CT, 2, LISTED>(a, p, workspace, stream);
+}
+
+bool shape_ok(int m, int Hq, int Hk, int HD, int n_ctx) {
+  return m >= 0 && Hk > 0 && Hk <= 65535 && Hq > 0 && Hq % Hk == 0 && (HD == 64 || HD == 128) && n_ctx > 0 && n_ctx <= (1 << 30);
+}
+
+int check(const char* name, const Args& a, int HD, int64_t tiles) {
+  CKV_REQUIRE(a.m >= 0 && a.Hk > 0 && a.Hk <= 65535 && a.Hq > 0 && a.Hq % a.Hk == 0, "%s: %d query heads over %d KV heads", name,
+              a.Hq, a.Hk);
+  CKV_REQUIRE(a.n_ctx > 0 && a.n_ctx <= (1 << 30), "%s: context of %d", name, a.n_ctx);
+  if (HD != 64 && HD != 128) {
+    set_error("%s: head_dim %d (64 or 128)", name, HD);
+    return CKV_ERR_UNSUPPORTED;
+  }
+  if (a.m == 0) return CKV_OK;
+  CKV_REQUIRE(a.q && a.k && a.v && a.positions && a.out, "%s: null pointer", name);
+  CKV_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.out), "%s: tensors must be 16-byte aligned", name);
+  if (tiles > 65535) {
+    set_error("%s: %lld row tiles (at most 65535 in one call)", name, static_cast<long long>(tiles));
+    return CKV_ERR_UNSUPPORTED;
+  }
+  return CKV_OK;
+}
+
+}  // namespace
+
+// Few query rows over a whole 8-bit cache; used by ckv_attention_kv8 (attention_kv8.cu).
+int64_t kv8_stream_workspace(int m, int Hq, int Hk, int HD, int n_ctx) {
+  return plan(m, Hq / Hk, Hk, HD, ceil_div(n_ctx, kBlk), false).bytes;
+}
+int kv8_stream_launches(int m, int Hq, int Hk, int HD, int n_ctx) {
+  return plan(m, Hq / Hk, Hk, HD, ceil_div(n_ctx, kBlk), false).splits > 1 ? 2 : 1;
+}
+int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs,
+                         const int32_t* positions, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, float scale, int type,
+                         void* workspace, cudaStream_t stream) {
+  const int nb = ceil_div(n_ctx, kBlk);
+  Args a{q, k8, v8, ks, vs, positions, nullptr, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, 0, 1, 1,
+         scale * 1.4426950408889634f};
+  const Plan p = plan(m, Hq / Hk, Hk, HD, nb, false);
+  if (int rc = check("ckv_attention_kv8", a, HD, p.tiles)) return rc;
+  if (HD == 128)
+    return type == CKV_KV8_E4M3 ? launch_nt<128, kE4m3, false>(a, p, workspace, stream)
+                                : launch_nt<128, kInt8, false>(a, p, workspace, stream);
+  return type == CKV_KV8_E4M3 ? launch_nt<64, kE4m3, false>(a, p, workspace, stream)
+                              : launch_nt<64, kInt8, false>(a, p, workspace, stream);
+}
+
+}  // namespace ckv
+
+using namespace ckv;
+
+extern "C" int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top) {
+  if (m <= 0 || top <= 0 || !shape_ok(m, n_q_heads, n_kv_heads, head_dim, 1)) return 0;
+  return plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, top, true).bytes;
+}
+
+extern "C" int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top) {
+  if (m <= 0 || top <= 0 || !shape_ok(m, n_q_heads, n_kv_heads, head_dim, 1)) return 0;
+  return plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, top, true).splits > 1 ? 2 : 1;
+}
+
+static int attention_blocks(const char* name, Args a, int HD, int type, void* workspace, int64_t ws_bytes, cudaStream_t s) {
+  CKV_REQUIRE(a.top > 0, "%s: lists of %d blocks", name, a.top);
+  const bool sane = a.Hk > 0 && a.Hq > 0 && a.m >= 0;
+  const Plan p = sane ? plan(a.m, std::max(1, a.Hq / a.Hk), a.Hk, HD, a.top, true) : Plan{};
+  if (int rc = check(name, a, HD, 0)) return rc;
+  if (a.m == 0) return CKV_OK;
+  CKV_REQUIRE(a.blocks != nullptr, "%s: null block list", name);
+  CKV_REQUIRE(ws_bytes >= p.bytes && (p.bytes == 0 || (workspace && aligned16(workspace))),
+              "%s: workspace of %lld bytes, needs %lld (16-byte aligned)", name, static_cast<long long>(ws_bytes),
+              static_cast<long long>(p.bytes));
+  // a grid's second dimension is limited: tokens go in runs of at most 32768 tiles (rows are
+  // independent, and a call this long is never split along its lists)
+  const int run = std::max(1, 32768 / p.head_tiles);
+  for (int t = 0; t < a.m; t += run) {
+    Args b = a;
+    Plan pb = p;
+    b.m = std::min(run, a.m - t);
+    pb.tiles = b.m * p.head_tiles;
+    b.q += int64_t(t) * a.Hq * HD;
+    b.out += int64_t(t) * a.Hq * HD;
+    b.positions += t;
+    b.blocks += int64_t(t) * a.Hk * a.top;
+    int rc;
+    if (HD == 128)
+      rc = type < 0 ? launch_nt<128, kBf16, true>(b, pb, workspace, s)
+           : type == CKV_KV8_E4M3 ? launch_nt<128, kE4m3, true>(b, pb, workspace, s)
+                                  : launch_nt<128, kInt8, true>(b, pb, workspace, s);
+    else
+      rc = type < 0 ? launch_nt<64, kBf16, true>(b, pb, workspace, s)
+           : type == CKV_KV8_E4M3 ? launch_nt<64, kE4m3, true>(b, pb, workspace, s)
+                                  : launch_nt<64, kInt8, true>(b, pb, workspace, s);
+    if (rc) return rc;
+  }
+  return CKV_OK;
+}
+
+extern "C" int ckv_attention_blocks(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                    const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int n_q_heads,
+                                    int n_kv_heads, int head_dim, int n_ctx, int top, float scale, void* workspace,
+                                    int64_t workspace_bytes, ckv_stream_t stream) {
+  const Args a{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr,
+               positions, blocks, out, nullptr, nullptr, int64_t(n_ctx), m, n_q_heads, n_kv_heads, n_ctx, ceil_div(n_ctx, kBlk),
+               top, 1, 1, scale * 1.4426950408889634f};
+  return attention_blocks("ckv_attention_blocks", a, head_dim, -1, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int ckv_attention_blocks_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                                        const float* v_scale, const int32_t* positions, const int32_t* blocks, uint16_t* out,
+                                        int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top, float scale,
+                                        int type, void* workspace, int64_t workspace_bytes, ckv_stream_t stream) {
+  CKV_REQUIRE(type == CKV_KV8_INT8 || type == CKV_KV8_E4M3, "ckv_attention_blocks_kv8: type %d", type);
+  CKV_REQUIRE(m == 0 || (k_scale && v_scale), "ckv_attention_blocks_kv8: null scales");
+  const int nb = ceil_div(n_ctx, kBlk);
+  const Args a{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, n_q_heads,
+               n_kv_heads, n_ctx, nb, top, 1, 1, scale * 1.4426950408889634f};
+  return attention_blocks("ckv_attention_blocks_kv8", a, head_dim, type, workspace, workspace_bytes, as_stream(stream));
+}

@@ -70,6 +70,9 @@ uint32_t read_clear_err_attention_tc();
 uint32_t read_clear_err_elementwise();
 uint32_t read_clear_err_tp_reduce();
 uint32_t read_clear_err_gemv_fused();
+uint32_t read_clear_err_kv8();
+uint32_t read_clear_err_block_select();
+uint32_t read_clear_err_attention_blocks();
 
 }  // namespace ckv
 
@@ -92,7 +95,8 @@ int ckv_get_device_error(uint32_t* code) {
   *code = ckv::read_clear_err_rope() | ckv::read_clear_err_select() | ckv::read_clear_err_gemm() |
           ckv::read_clear_err_attention_tc() |
           ckv::read_clear_err_elementwise() | ckv::read_clear_err_tp_reduce() |
-          ckv::read_clear_err_gemv_fused();
+          ckv::read_clear_err_gemv_fused() | ckv::read_clear_err_kv8() | ckv::read_clear_err_block_select() |
+          ckv::read_clear_err_attention_blocks();
   return CKV_OK;
 }
 

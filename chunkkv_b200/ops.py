@@ -696,3 +696,371 @@ def log_softmax(row: torch.Tensor, out: torch.Tensor | None = None) -> torch.Ten
     out = torch.empty(row.numel(), dtype=torch.float32, device=row.device) if out is None else out
     _run("ckv_log_softmax", _ptr(row), row.numel(), _ptr(out), _stream())
     return out
+
+
+# --------------------------------------------------------- K/V cache in 8 bits
+_KV8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # CKV_KV8_INT8, CKV_KV8_E4M3
+
+
+def _on_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    """Every tensor lies on the current CUDA device, whose current stream the call uses."""
+    if not first.is_cuda:
+        raise ValueError("chunkkv_b200 ops take CUDA tensors (there is no CPU path)")
+    dev = first.get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors lie on different devices ({first.device} and {t.device})")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"tensors lie on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _n_blocks(n_ctx: int) -> int:
+    return (n_ctx + PAGE_TOKENS - 1) // PAGE_TOKENS
+
+
+class BlockDigest:
+    """What the block score of the sparse attention reads of K: for every KV head and block of
+    16 tokens its channel maxima and minima in int8 (`codes` [H, blocks, 2, D]) and one fp32
+    `scale` [H, blocks].  Kept up to date by `block_digest`, or by `kv8_write` for the digest of
+    a KV8Cache."""
+
+    __slots__ = ("codes", "scale", "n_ctx")
+
+    def __init__(self, n_kv_heads: int, n_ctx: int, head_dim: int, device="cuda"):
+        nb = _n_blocks(n_ctx)
+        self._set(torch.zeros((n_kv_heads, nb, 2, head_dim), dtype=torch.int8, device=device),
+                  torch.zeros((n_kv_heads, nb), dtype=torch.float32, device=device), n_ctx)
+
+    @classmethod
+    def wrap(cls, codes: torch.Tensor, scale: torch.Tensor, n_ctx: int) -> "BlockDigest":
+        """A digest over buffers that the caller owns."""
+        d = cls.__new__(cls)
+        d._set(codes, scale, n_ctx)
+        return d
+
+    def _set(self, codes: torch.Tensor, scale: torch.Tensor, n_ctx: int) -> None:
+        nb = _n_blocks(n_ctx)
+        if n_ctx <= 0 or codes.dim() != 4 or codes.shape[1] != nb or codes.shape[2] != 2:
+            raise ValueError(f"codes: expected shape (H, {nb}, 2, D) for {n_ctx} tokens, got {tuple(codes.shape)}")
+        if tuple(scale.shape) != (codes.shape[0], nb):
+            raise ValueError(f"scale: expected shape ({codes.shape[0]}, {nb}), got {tuple(scale.shape)}")
+        _buf("codes", codes, 0, dtype=torch.int8)
+        _buf("scale", scale, 0, dtype=torch.float32)
+        self.codes, self.scale, self.n_ctx = codes, scale, int(n_ctx)
+
+
+class KV8Cache:
+    """One layer's K/V cache in 8 bits: codes `k`, `v` [H, blocks * 16, D] (int8 or float8_e4m3fn),
+    fp32 scales `k_scale`, `v_scale` [H, blocks] per KV head and block of 16 tokens, the bf16 rows
+    of the block in progress (`tail` [2, H, 16, D], `tail_end` [2, H]) and, with `digest=True`, the
+    block digest of K for the sparse attention.  Tokens never written read as zeros."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "tail", "tail_end", "digest", "n_ctx", "n_kv_heads", "head_dim",
+                 "dtype")
+
+    def __init__(self, n_kv_heads: int, n_ctx: int, head_dim: int, dtype: torch.dtype = torch.int8, device="cuda",
+                 digest: bool = False):
+        if dtype not in _KV8_TYPES:
+            raise NotImplementedError(f"KV8Cache: dtype {dtype} is not supported (int8 and float8_e4m3fn are)")
+        if n_ctx <= 0 or n_kv_heads <= 0:
+            raise ValueError(f"KV8Cache: {n_kv_heads} heads, {n_ctx} tokens")
+        nb = _n_blocks(n_ctx)
+        kv = [torch.zeros((n_kv_heads, nb * PAGE_TOKENS, head_dim), dtype=torch.uint8, device=device).view(dtype)
+              for _ in range(2)]
+        sc = torch.zeros((2, n_kv_heads, nb), dtype=torch.float32, device=device)
+        self._set(*kv, sc[0], sc[1], n_ctx, None, 0,
+                  BlockDigest(n_kv_heads, n_ctx, head_dim, device) if digest else None)
+
+    @classmethod
+    def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, n_ctx: int,
+             tail: torch.Tensor | None = None, tail_start: int = 0, digest: BlockDigest | None = None) -> "KV8Cache":
+        """A cache over buffers that the caller owns.  `tail`, where given, holds the bf16 rows
+        of the block in progress when the cache holds `tail_start` tokens."""
+        c = cls.__new__(cls)
+        c._set(k, v, k_scale, v_scale, n_ctx, tail, tail_start, digest)
+        return c
+
+    def _set(self, k, v, k_scale, v_scale, n_ctx, tail, tail_start, digest) -> None:
+        nb = _n_blocks(n_ctx)
+        if k.dtype not in _KV8_TYPES:
+            raise NotImplementedError(f"KV8Cache: dtype {k.dtype} is not supported (int8 and float8_e4m3fn are)")
+        if n_ctx <= 0 or k.dim() != 3 or k.shape[1] != nb * PAGE_TOKENS:
+            raise ValueError(f"k: expected shape (H, {nb * PAGE_TOKENS}, D) for {n_ctx} tokens, got {tuple(k.shape)}")
+        H, _, D = k.shape
+        for name, t in (("k", k), ("v", v)):
+            if t.shape != k.shape:
+                raise ValueError(f"{name}: expected shape {tuple(k.shape)}, got {tuple(t.shape)}")
+            _buf(name, t, 0, dtype=k.dtype)
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if tuple(t.shape) != (H, nb):
+                raise ValueError(f"{name}: expected shape ({H}, {nb}), got {tuple(t.shape)}")
+            _buf(name, t, 0, dtype=torch.float32)
+        if tail is None:
+            tail, tail_start = torch.zeros((2, H, PAGE_TOKENS, D), dtype=BF16, device=k.device), 0
+        if tuple(tail.shape) != (2, H, PAGE_TOKENS, D):
+            raise ValueError(f"tail: expected shape (2, {H}, {PAGE_TOKENS}, {D}), got {tuple(tail.shape)}")
+        _buf("tail", tail, 0)
+        if digest is not None and (tuple(digest.codes.shape) != (H, nb, 2, D) or digest.n_ctx != n_ctx):
+            raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache")
+        self.k, self.v, self.k_scale, self.v_scale, self.tail, self.digest = k, v, k_scale, v_scale, tail, digest
+        end = int(tail_start) if tail_start % PAGE_TOKENS else 0
+        self.tail_end = torch.full((2, H), end, dtype=torch.int32, device=k.device)
+        self.n_ctx, self.n_kv_heads, self.head_dim, self.dtype = int(n_ctx), H, D, k.dtype
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes of the codes and scales."""
+        return self.k.numel() * 2 + self.k_scale.numel() * 8
+
+
+def _rows_view(name: str, t: torch.Tensor, H: int, D: int) -> None:
+    """bf16 rows [H, n, D] with contiguous rows (any 16-byte aligned row and head strides)."""
+    if t.dtype != BF16:
+        raise ValueError(f"{name}: expected {BF16}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[0] != H or t.shape[2] != D:
+        raise ValueError(f"{name}: expected shape ({H}, n, {D}), got {tuple(t.shape)}")
+    if t.stride(2) != 1:
+        raise ValueError(f"{name}: expected rows of contiguous elements, got strides {t.stride()}")
+
+
+def _start(start, m: int, n_ctx: int, rows: int, by_position: bool, name: str):
+    """(host start, device pointer of start) after the checks that the host can make."""
+    if isinstance(start, torch.Tensor):
+        _buf("start", start, 1, dtype=torch.int32)
+        return 0, start.data_ptr()
+    if start < 0 or start + m > n_ctx:
+        raise ValueError(f"{name}: tokens [{start}, {start + m}) outside the context of {n_ctx}")
+    if by_position and start + m > rows:
+        raise ValueError(f"{name}: source holds {rows} rows, position {start + m - 1} asked for")
+    return int(start), None
+
+
+def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start, m: int | None = None,
+              by_position: bool = False) -> KV8Cache:
+    """Quantise bf16 K/V rows [H, rows, D] into the cache as tokens [start, start + m): one fp32
+    scale per KV head and block of 16 tokens.  Token t's row is row t - start of `k` and `v`, or
+    row t with `by_position` (a cache-shaped source).  `start` is an int, or an int32 device
+    tensor (then `m` rows are read from wherever it points at launch: a captured call serves
+    every later position).  `m` defaults to all rows (1 for a device `start`)."""
+    H, D = cache.n_kv_heads, cache.head_dim
+    _rows_view("k", k, H, D)
+    _rows_view("v", v, H, D)
+    rows = min(k.shape[1], v.shape[1])
+    if m is None:
+        m = 1 if isinstance(start, torch.Tensor) else (rows - start if by_position else rows)
+    if m < 0 or (not by_position and m > rows):
+        raise ValueError(f"kv8_write: {m} rows asked for, the source has {rows}")
+    s, s_dev = _start(start, m, cache.n_ctx, rows, by_position, "kv8_write")
+    _on_device(k, v, cache.k, start if s_dev is not None else None)
+    dig = cache.digest
+    _run("ckv_kv8_write", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), rows,
+         int(by_position), m, s, s_dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+         cache.v_scale.data_ptr(), cache.tail.data_ptr(), cache.tail_end.data_ptr(),
+         None if dig is None else dig.codes.data_ptr(), None if dig is None else dig.scale.data_ptr(), H, D,
+         cache.n_ctx, _KV8_TYPES[cache.dtype], _stream(), nbytes=6.0 * H * m * D)
+    return cache
+
+
+def kv8_read(cache: KV8Cache, start: int = 0, m: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values of tokens [start, start + m) as bf16 rows: K and V, each [H, m, D]."""
+    m = cache.n_ctx - start if m is None else m
+    if start < 0 or m < 0 or start + m > cache.n_ctx:
+        raise ValueError(f"kv8_read: tokens [{start}, {start + m}) outside the context of {cache.n_ctx}")
+    _on_device(cache.k)
+    H, D = cache.n_kv_heads, cache.head_dim
+    k = torch.empty((H, m, D), dtype=BF16, device=cache.k.device)
+    v = torch.empty_like(k)
+    _run("ckv_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+         k.data_ptr(), v.data_ptr(), H, D, cache.n_ctx, start, m, _KV8_TYPES[cache.dtype], _stream(),
+         nbytes=6.0 * H * m * D)
+    return k, v
+
+
+def block_digest(k_cache: torch.Tensor, digest: BlockDigest, start=0, m: int | None = None) -> BlockDigest:
+    """Bring `digest` up to date with a bf16 K cache [H, n_ctx, D] whose tokens [start, start + m)
+    are new (`start` an int or an int32 device tensor, m then 1 unless given)."""
+    H, nb, _, D = digest.codes.shape
+    _rows_view("k_cache", k_cache, H, D)
+    if m is None:
+        m = 1 if isinstance(start, torch.Tensor) else min(digest.n_ctx, k_cache.shape[1]) - start
+    if m < 0:
+        raise ValueError(f"block_digest: {m} rows")
+    s, s_dev = _start(start, m, digest.n_ctx, k_cache.shape[1], True, "block_digest")
+    _on_device(k_cache, digest.codes, start if s_dev is not None else None)
+    _run("ckv_block_digest", k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.shape[1], m, s, s_dev,
+         digest.codes.data_ptr(), digest.scale.data_ptr(), H, D, digest.n_ctx, _stream(), nbytes=2.0 * H * m * D)
+    return digest
+
+
+def _query(q: torch.Tensor, H: int, D: int, positions: torch.Tensor, m: int | None) -> tuple[int, int]:
+    """(rows, query heads) of q [m, Hq, D] (or [m, Hq * D]) with one int32 position per row."""
+    if q.dim() == 3:
+        Hq = q.shape[1]
+        ok = q.shape[2] == D
+    else:
+        ok = q.dim() == 2 and q.shape[1] % D == 0
+        Hq = q.shape[-1] // D
+    if not ok or Hq == 0 or Hq % H:
+        raise ValueError(f"q: expected shape (m, Hq, {D}) with Hq a multiple of {H}, got {tuple(q.shape)}")
+    m = q.shape[0] if m is None else m
+    if m < 0:
+        raise ValueError(f"{m} rows")
+    _buf("q", q, m * Hq * D)
+    _buf("positions", positions, m, dtype=torch.int32)
+    return m, Hq
+
+
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _workspace_arg(workspace: torch.Tensor | None, need: int, device) -> tuple[torch.Tensor | None, int]:
+    """The caller's workspace (bytes), or one of this call (allocated in stream order)."""
+    if workspace is None:
+        return _scratch(need, device), need
+    if not workspace.is_contiguous():
+        raise ValueError("workspace: expected a contiguous tensor")
+    nbytes = workspace.numel() * workspace.element_size()
+    if nbytes < need:
+        raise ValueError(f"workspace: has {nbytes} bytes, needs {need}")
+    return workspace, nbytes
+
+
+def attention_kv8_workspace_bytes(m: int, n_q_heads: int, n_kv_heads: int, head_dim: int, n_ctx: int) -> int:
+    return int(_lib.load().ckv_attention_kv8_workspace_size(m, n_q_heads, n_kv_heads, head_dim, n_ctx))
+
+
+def attention_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, out: torch.Tensor | None = None,
+                  m: int | None = None, scale: float | None = None, flops: float = 0.0,
+                  workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """`attention` over an 8-bit cache: q/out [m, Hq, D] bf16; key j visible to row i iff
+    j <= positions[i]; a row with a negative position gives zeros.  `workspace` (uint8, of
+    `attention_kv8_workspace_bytes`, any contents) may be kept by the caller; calls that share
+    one must not overlap."""
+    H, D = cache.n_kv_heads, cache.head_dim
+    m, Hq = _query(q, H, D, positions, m)
+    if out is None:
+        out = torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
+    else:
+        _buf("out", out, m * Hq * D)
+    _on_device(q, positions, out, cache.k, workspace)
+    lib = _lib.load()
+    need = lib.ckv_attention_kv8_workspace_size(m, Hq, H, D, cache.n_ctx)
+    workspace, nbytes = _workspace_arg(workspace, need, q.device)
+    kernels = 1 if _TIMER is None else lib.ckv_attention_kv8_launches(m, Hq, H, D, cache.n_ctx)
+    _run("ckv_attention_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+         cache.v_scale.data_ptr(), positions.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
+         1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(workspace), nbytes,
+         _stream(), flops=flops, kernels=kernels)
+    return out
+
+
+# ------------------------------------------------ attention over selected blocks
+def block_select(q: torch.Tensor, digest: BlockDigest, positions: torch.Tensor, top: int, sink: int = 1,
+                 recent: int = 1, out: torch.Tensor | None = None, m: int | None = None) -> torch.Tensor:
+    """For every row of q [m, Hq, D] and KV head the `top` blocks of 16 keys whose score (an upper
+    bound of q . k, from the digest) is highest, the first `sink` and the last `recent` visible
+    blocks always among them; int32 [m, H, top], ascending, -1 past a row's last visible block."""
+    H, _, _, D = digest.codes.shape
+    m, Hq = _query(q, H, D, positions, m)
+    if out is None:
+        out = torch.empty((m, H, top), dtype=torch.int32, device=q.device)
+    else:
+        _buf("out", out, m * H * top, dtype=torch.int32)
+    _on_device(q, positions, out, digest.codes)
+    lib = _lib.load()
+    ws, nbytes = _workspace_arg(None, lib.ckv_block_select_workspace_size(m, Hq, H, D, digest.n_ctx), q.device)
+    kernels = 1 if _TIMER is None else lib.ckv_block_select_launches(m, Hq, H, D, digest.n_ctx)
+    _run("ckv_block_select", q.data_ptr(), digest.codes.data_ptr(), digest.scale.data_ptr(), positions.data_ptr(),
+         out.data_ptr(), m, Hq, H, D, digest.n_ctx, top, sink, recent, _ptr(ws), nbytes, _stream(), kernels=kernels)
+    return out
+
+
+def _blocks_arg(blocks: torch.Tensor, m: int, H: int) -> int:
+    """The list length of int32 block lists [>= m, H, top]."""
+    if blocks.dim() != 3 or blocks.shape[0] < m or blocks.shape[1] != H:
+        raise ValueError(f"blocks: expected shape (>= {m}, {H}, top), got {tuple(blocks.shape)}")
+    _buf("blocks", blocks, 0, dtype=torch.int32)
+    return blocks.shape[2]
+
+
+def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor,
+                     blocks: torch.Tensor, out: torch.Tensor | None = None, m: int | None = None,
+                     scale: float | None = None) -> torch.Tensor:
+    """`attention` restricted to the 16-key blocks listed for each row and KV head (int32
+    [m, H, top], ascending, -1 past the end, as `block_select` returns them); bf16 caches
+    [H, n_ctx, D].  Rows that see no key give zeros."""
+    if k_cache.dim() != 3:
+        raise ValueError(f"k_cache: expected shape (H, n_ctx, D), got {tuple(k_cache.shape)}")
+    H, n_ctx, D = k_cache.shape
+    _cache("k_cache", k_cache, H, D)
+    _cache("v_cache", v_cache, H, D)
+    if v_cache.shape[1] != n_ctx:
+        raise ValueError("k_cache and v_cache differ in length")
+    m, Hq = _query(q, H, D, positions, m)
+    top = _blocks_arg(blocks, m, H)
+    if out is None:
+        out = torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
+    else:
+        _buf("out", out, m * Hq * D)
+    _on_device(q, k_cache, v_cache, positions, blocks, out)
+    lib = _lib.load()
+    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top), q.device)
+    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top)
+    _run("ckv_attention_blocks", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
+         blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, 1.0 / math.sqrt(D) if scale is None else float(scale),
+         _ptr(ws), nbytes, _stream(), kernels=kernels)
+    return out
+
+
+def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, blocks: torch.Tensor,
+                         out: torch.Tensor | None = None, m: int | None = None,
+                         scale: float | None = None) -> torch.Tensor:
+    """`attention_blocks` over an 8-bit cache."""
+    H, D = cache.n_kv_heads, cache.head_dim
+    m, Hq = _query(q, H, D, positions, m)
+    top = _blocks_arg(blocks, m, H)
+    if out is None:
+        out = torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
+    else:
+        _buf("out", out, m * Hq * D)
+    _on_device(q, positions, blocks, out, cache.k)
+    lib = _lib.load()
+    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top), q.device)
+    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top)
+    _run("ckv_attention_blocks_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+         cache.v_scale.data_ptr(), positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
+         top, 1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), nbytes,
+         _stream(), kernels=kernels)
+    return out
+
+
+def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, top: int,
+                     digest: BlockDigest | None = None, sink: int = 1, recent: int = 1,
+                     out: torch.Tensor | None = None, m: int | None = None,
+                     scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Block-sparse attention over a bf16 cache: `block_select`, then `attention_blocks`; returns
+    (out, blocks).  Without a `digest` that the caller keeps, the whole cache's is built first."""
+    if k_cache.dim() != 3:
+        raise ValueError(f"k_cache: expected shape (H, n_ctx, D), got {tuple(k_cache.shape)}")
+    H, n_ctx, D = k_cache.shape
+    if digest is None:
+        nb = _n_blocks(n_ctx)
+        digest = BlockDigest.wrap(torch.empty((H, nb, 2, D), dtype=torch.int8, device=k_cache.device),
+                                  torch.empty((H, nb), dtype=torch.float32, device=k_cache.device), n_ctx)
+        block_digest(k_cache, digest)
+    elif digest.n_ctx != n_ctx or tuple(digest.codes.shape[::3]) != (H, D):
+        raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache "
+                         f"{tuple(k_cache.shape)}")
+    blocks = block_select(q, digest, positions, top, sink, recent, m=m)
+    return attention_blocks(q, k_cache, v_cache, positions, blocks, out=out, m=m, scale=scale), blocks
+
+
+def attention_sparse_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, top: int, sink: int = 1,
+                         recent: int = 1, out: torch.Tensor | None = None, m: int | None = None,
+                         scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """`attention_sparse` over an 8-bit cache that keeps its digest (``KV8Cache(digest=True)``)."""
+    if cache.digest is None:
+        raise ValueError("attention_sparse_kv8: the cache keeps no digest (KV8Cache(..., digest=True))")
+    blocks = block_select(q, cache.digest, positions, top, sink, recent, m=m)
+    return attention_blocks_kv8(q, cache, positions, blocks, out=out, m=m, scale=scale), blocks

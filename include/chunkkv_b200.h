@@ -52,6 +52,7 @@ typedef enum {
 #define CKV_DEV_ERR_SELECT_UNCOMPUTED 0x4u /* selection kept a position never computed
                                               (torch_engine.py:151 assert) */
 #define CKV_DEV_ERR_POSITION_RANGE 0x8u  /* a position outside [0, n_ctx) was skipped */
+#define CKV_DEV_ERR_NONFINITE 0x10u      /* a NaN or infinity was stored saturated in an 8-bit cache */
 
 /* ---- library -------------------------------------------------------------- */
 CKV_API const char* ckv_version(void);
@@ -361,6 +362,90 @@ CKV_API int ckv_attention(const uint16_t* q, const uint16_t* k_cache, const uint
                           const int32_t* positions, uint16_t* out, int m, int n_q_heads,
                           int n_kv_heads, int head_dim, int n_ctx, float scale, void* workspace,
                           int64_t workspace_bytes, ckv_stream_t stream);
+
+/* ---- K/V cache in 8 bits ---------------------------------------------------
+ * One request's cache of one layer held in 8 bits, with one fp32 scale per KV head and
+ * block of CKV_PAGE_TOKENS tokens, for K and for V:
+ *   k8, v8           [H][n_blocks * 16][D] codes (int8 or e4m3), n_blocks = ceil(n_ctx / 16)
+ *   k_scale, v_scale [H][n_blocks]; a value is code * scale
+ *   tail             [2 (K, V)][H][16][D] bf16: the rows of the block in progress
+ *   tail_end         [2][H] int32: one past the last token whose row the tail holds (zero at first)
+ *   dig_codes        [H][n_blocks][2][D] int8, dig_scale [H][n_blocks] (both optional): the
+ *                    block digest of K, its channel maxima and minima
+ * All of them start as zeros.  For a block's written rows with a = max |x|:
+ * scale = fp32(a / qmax), code = rn(fp32(x * fp32(qmax / a))), qmax 127 (int8) or 448 (e4m3);
+ * a < 2^-100 stores zeros with scale 0.  Digest codes likewise with 127.  A NaN is stored as 0
+ * and an infinity as the block's largest value, and CKV_DEV_ERR_NONFINITE is recorded.  The
+ * codes past a block's last written row are 0.  The reference keeps its cache in the model's
+ * dtype (torch_engine.py:187-195); this form has no counterpart there. */
+typedef enum { CKV_KV8_INT8 = 0, CKV_KV8_E4M3 = 1 } ckv_kv8_type;
+
+/* Rows of m tokens into the cache as tokens [start, start + m).  k, v: bf16 rows of D
+ * contiguous elements at the given element strides (multiples of 8); token t's row is row
+ * t - start, or row t when by_position is set.  The block that holds `start` is requantised from
+ * its rows so far: those in the tail, or, when the write goes back into an earlier block, the
+ * values of its codes.  With start_dev the first token is read from the device (one int32; a
+ * captured launch then serves every later position; out of range is recorded and nothing is
+ * written). */
+CKV_API int ckv_kv8_write(const uint16_t* k, const uint16_t* v, int64_t k_head_stride, int64_t k_row_stride,
+                          int64_t v_head_stride, int64_t v_row_stride, int64_t src_rows, int by_position, int m,
+                          int start, const int32_t* start_dev, uint8_t* k8, uint8_t* v8, float* k_scale,
+                          float* v_scale, uint16_t* tail, int32_t* tail_end, int8_t* dig_codes, float* dig_scale,
+                          int n_kv_heads, int head_dim, int n_ctx, int type, ckv_stream_t stream);
+
+/* Values of tokens [start, start + m) as bf16 rows, k_out / v_out [H][m][D]. */
+CKV_API int ckv_kv8_read(const uint8_t* k8, const uint8_t* v8, const float* k_scale, const float* v_scale,
+                         uint16_t* k_out, uint16_t* v_out, int n_kv_heads, int head_dim, int n_ctx, int start, int m,
+                         int type, ckv_stream_t stream);
+
+/* Block digest of a bf16 K cache (rows by position): the blocks that tokens [start, start + m)
+ * touch, over their rows below start + m. */
+CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row_stride, int64_t src_rows, int m,
+                             int start, const int32_t* start_dev, int8_t* dig_codes, float* dig_scale, int n_kv_heads,
+                             int head_dim, int n_ctx, ckv_stream_t stream);
+
+/* ckv_attention over the 8-bit cache: q/out [m][Hq][D] bf16, key j visible to row i iff
+ * j <= positions[i]; a row whose position is negative sees no key and gives zeros, one at or
+ * past n_ctx sees every key (recorded).  At most 128 query heads per KV head, head_dim 64 or
+ * 128.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
+ * 0) needs no initialisation; calls that share one must not overlap on the GPU. */
+CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
+/* Kernels one ckv_attention_kv8 call launches at this shape (0 for a shape it refuses). */
+CKV_API int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
+CKV_API int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                              const float* v_scale, const int32_t* positions, uint16_t* out, int m, int n_q_heads,
+                              int n_kv_heads, int head_dim, int n_ctx, float scale, int type, void* workspace,
+                              int64_t workspace_bytes, ckv_stream_t stream);
+
+/* ---- attention over selected blocks -----------------------------------------
+ * For every query token and KV head the `top` blocks of 16 keys that a cheap score ranks
+ * best: the first `sink` and the last `recent` visible blocks always, the others by score (an
+ * upper bound of q . k over the block from its digest and the query's 8-bit codes, the best
+ * head of the group), equal scores to the lower block.  blocks [m][H][top] int32, ascending, -1
+ * past a row's last visible block.  At most 16 query heads per KV head, contexts up to 786,432
+ * tokens, sink + recent <= top <= 4096, recent >= 1.  The workspace (16-byte aligned) needs no
+ * initialisation. */
+CKV_API int64_t ckv_block_select_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
+CKV_API int ckv_block_select_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
+CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const float* dig_scale,
+                             const int32_t* positions, int32_t* blocks, int m, int n_q_heads, int n_kv_heads,
+                             int head_dim, int n_ctx, int top, int sink, int recent, void* workspace,
+                             int64_t workspace_bytes, ckv_stream_t stream);
+
+/* Attention of row i over the keys j <= positions[i] of the blocks listed for it (ascending, -1
+ * past the end; an entry out of range or not above the one before it is skipped and recorded as
+ * CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache.  Rows that see no
+ * key give zeros. */
+CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top);
+CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top);
+CKV_API int ckv_attention_blocks(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                 const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int n_q_heads,
+                                 int n_kv_heads, int head_dim, int n_ctx, int top, float scale, void* workspace,
+                                 int64_t workspace_bytes, ckv_stream_t stream);
+CKV_API int ckv_attention_blocks_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                                     const float* v_scale, const int32_t* positions, const int32_t* blocks, uint16_t* out,
+                                     int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top, float scale,
+                                     int type, void* workspace, int64_t workspace_bytes, ckv_stream_t stream);
 
 /* Small-m projection (lm_head on the logit rows, torch_engine.py:75-76,165):
  * out [m][n] = bf16(x [m][k] @ w[n][k]^T), m <= 8. */
