@@ -1,5 +1,33 @@
-// Attention over the 8-bit cache.
+// Attention over the 8-bit K/V cache (one fp32 scale per KV head and block of 16 tokens).
+//
+// Few packed rows (token x head of a group) stream the cache through attention_blocks.cu;
+// from kTileRows rows on, the tcgen05 kernel below takes them in 128-row tiles.
+//
+// It is the bf16 kernel's scheme (attention_tc.cu: two Q tiles per CTA, S and P in TMEM,
+// lazy rescale, persistent items, key splits) with the operands made on the SM: a warpgroup
+// of converters reads the codes from global memory (16 bytes per lane and load, one tile
+// ahead in registers) and writes them as fp16 into the 128B-swizzled operand tiles.  Both
+// code types are exact in fp16, so is q scaled by a power of two per row, and the block
+// scales never touch the tensor core:
+//   S (row, key) = q . code            tcgen05.mma kind::f16
+//   x            = S c_b,  c_b = row factor * K scale of the key's block (8 blocks a tile)
+//   P'           = 2^(x - m + 7) * (V scale of the block / reference), rounded to fp16
+//   O           += P' code             tcgen05.mma, A = P' from TMEM
+// The scale of a whole 16-column group folds into constants the softmax uses anyway: the
+// group's maximum is scaled once, the exponent's multiply-add takes c_b and
+// log2(V scale / reference) - m, and the group's sum of P' is divided by the V scale once.
+// So the softmax, which bounds the kernel (issue slots), costs per score what it costs over
+// a bf16 cache.  The reference is the power of two at or above the item's largest V scale:
+// P' stays below 2^15 (2^8 of lazy growth, 2^7 of bias) and keeps 11 bits down to 2^-21 of
+// a row's largest weight.
+// Warps: 0..3 and 4..7 softmax / epilogue of Q tiles 0 and 1, 8..11 converters, 12 item
+// scheduler, 13 MMA issuer and TMEM owner, 14 and 15 idle.  The 512 threads start with 128
+// registers each; setmaxnreg moves them to the softmax warps (168 + 104 + 72: 65,536 in all).
 #include "ckv_common.cuh"
+
+CKV_DEFINE_ERR_WORD(attention_kv8)
+
+#include "attention_split.cuh"
 
 namespace ckv {
 // attention_blocks.cu
@@ -9,6 +37,705 @@ int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8
                          const int32_t* positions, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, float scale, int type,
                          void* workspace, cudaStream_t stream);
 namespace {
+
+constexpr int kBlk = CKV_PAGE_TOKENS;
+constexpr int KS = 2;  // K stages
+constexpr int VS = 2;  // V stages
+constexpr int GRP = BN / kBlk;  // scale blocks per key tile
+constexpr int kScaleSlots = 4;  // tiles whose block scales are held at once
+constexpr int kThreads = 512;
+constexpr int kWarpConv = 8, kWarpSched = 12, kWarpMma = 13;
+constexpr uint32_t TMEM_COLS = 512;  // S/P of tile w at [128w, 128w+128), O of tile w at 256+128w
+constexpr uint32_t O_COL = 256;
+constexpr float kPBits = 7.0f;  // P' is 2^7 times its weight
+constexpr int kRegsSoftmax = 168, kRegsConv = 104, kRegsRest = 72;
+static_assert(8 * kRegsSoftmax + 4 * kRegsConv + 4 * kRegsRest == 16 * 128, "the split is what the launch holds");
+
+template <int HD>
+struct Cfg {
+  static constexpr uint32_t Q_BYTES = BM * HD * 2;
+  static constexpr uint32_t KV_TILE = BN * HD * 2;
+  static constexpr uint32_t SMEM_NEED = 1024 + NQ * Q_BYTES + (KS + VS) * KV_TILE +
+                                        kItemSlots * (sizeof(Item) + NQ * BM * 4) + kStageBytes +
+                                        kScaleSlots * GRP * 12 + 2 * NQ * BM * 4 + 64 + 40 * 8 + 16;
+  // at least 120 KiB so two CTAs never share an SM: each allocates all 512 TMEM columns
+  static constexpr uint32_t SMEM = SMEM_NEED > 120 * 1024 ? SMEM_NEED : 120 * 1024;
+  static constexpr uint32_t IDESC_S = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(BM >> 4) << 24);  // fp16 operands
+  static constexpr uint32_t IDESC_PV = (1u << 4) | (uint32_t(HD >> 3) << 17) | (uint32_t(BM >> 4) << 24) | (1u << 16);
+};
+
+// four codes -> two pairs of fp16, exactly
+template <bool E4M3>
+__device__ __forceinline__ uint2 widen4(uint32_t w) {
+  uint2 r;
+  if constexpr (E4M3) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(r.x), "=r"(r.y)
+        : "r"(w));
+  } else {
+    // 0x6400 + u is the fp16 number 1024 + u, u = code + 128: minus 1152 is the code
+    const uint32_t u = w ^ 0x80808080u, magic = 0x64646464u;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(__byte_perm(u, magic, 0x4140)), "r"(0x64806480u));
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(__byte_perm(u, magic, 0x4342)), "r"(0x64806480u));
+  }
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+__device__ __forceinline__ void conv_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+struct Args {
+  const uint16_t* q;
+  const uint8_t *k, *v;
+  const float *ks, *vs;
+  const int32_t* positions;
+  uint16_t* out;
+  float* part_o;
+  float2* part_ml;
+  int M, Hq, Hk, n_ctx, n_blocks, tps, max_splits, blocks;
+  float scale_log2;
+};
+
+// Item.pad0: last key that any of its rows sees (-1: none), pad1: Q tiles that hold rows.
+// CTA c takes slots c, c + gridDim.x, ... (longest first).
+template <int HD, bool E4M3>
+__global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid_constant__ Args a) {
+  using C = Cfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                      // [NQ][Q_BYTES]
+  uint8_t* sK = sQ + NQ * C::Q_BYTES;      // [KS][KV_TILE]
+  uint8_t* sV = sK + KS * C::KV_TILE;      // [VS][KV_TILE]
+  Item* items = reinterpret_cast<Item*>(sV + VS * C::KV_TILE);                    // [kItemSlots]
+  int* s_pos = reinterpret_cast<int*>(items + kItemSlots);                        // [kItemSlots][NQ * BM]
+  uint32_t* s_stage = reinterpret_cast<uint32_t*>(s_pos + kItemSlots * NQ * BM);  // [8 warps][32][20]
+  float* s_ks = reinterpret_cast<float*>(s_stage + kStageBytes / 4);              // [kScaleSlots][GRP] K scale
+  float* s_lv = s_ks + kScaleSlots * GRP;                                         // log2(V scale / reference) + 7
+  float* s_iv = s_lv + kScaleSlots * GRP;                                         // reference / V scale
+  float* s_qf = s_iv + kScaleSlots * GRP;                                         // [2][NQ * BM] row factors
+  float* s_ref = s_qf + 2 * NQ * BM;                                              // [4] V scale references, by item
+  float* s_red = s_ref + 4;                                                       // [4]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(s_red + 12);
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* s_full = v_empty + VS;    // [NQ]
+  uint64_t* p_full = s_full + NQ;     // [NQ]
+  uint64_t* o_done = p_full + NQ;     // [NQ]
+  uint64_t* q_ready = o_done + NQ;    // [NQ]: Q tile w of the next item is in place
+  uint64_t* q_free = q_ready + NQ;    // [NQ]: the item's last S MMA of tile w is done
+  uint64_t* o_full = q_free + NQ;     // [NQ]: the item's last P V of tile w is done
+  uint64_t* item_full = o_full + NQ;  // [kItemSlots]
+  uint64_t* item_empty = item_full + kItemSlots;  // [kItemSlots]
+  uint64_t* drain = item_empty + kItemSlots;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.Hq / a.Hk;
+  const int T = BM / G;  // tokens per Q tile
+  const int n_slots = a.blocks * a.Hk * a.max_splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < KS; ++s) {
+      mbar_init(&k_full[s], 128);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < VS; ++s) {
+      mbar_init(&v_full[s], 128);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int w = 0; w < NQ; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_done[w], 1);
+      mbar_init(&q_ready[w], 128);
+      mbar_init(&q_free[w], 1);
+      mbar_init(&o_full[w], 1);
+    }
+    for (int s = 0; s < kItemSlots; ++s) {
+      mbar_init(&item_full[s], 1);
+      mbar_init(&item_empty[s], 1 + NQ * 4 + 4);  // the MMA thread, each softmax and converter warp
+    }
+    mbar_init(drain, 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == kWarpMma) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // set-up done; q, the cache, the positions and the workspace belong to the kernels
+  // before (dependent launch)
+  pdl_wait();
+  pdl_launch_next();
+
+  if (warp >= kWarpSched) {
+    regs_dec<kRegsRest>();
+    if (warp == kWarpSched) {
+      // ---------------------------------------------------------------- item scheduler
+      int it = 0;
+      int cursor = blockIdx.x;
+      while (true) {
+        Item rec{-1, 0, 0, 0, 0, 0, 0, 0};
+        int pv[NQ * BM / 32];  // the item's token positions, lane + 32 j (clamped)
+#pragma unroll
+        for (int j = 0; j < NQ * BM / 32; ++j) pv[j] = -1;
+        for (; cursor < n_slots; cursor += gridDim.x) {
+          const int gi = cursor / (a.Hk * a.blocks);  // slot group
+          const int rem = cursor - gi * (a.Hk * a.blocks);
+          const int hk = rem / a.blocks;
+          const int rb = a.blocks - 1 - (rem - hk * a.blocks);
+          const int t0 = rb * NQ * T;
+          const int n_tok = min(NQ * T, a.M - t0);
+          int mx = -1;
+#pragma unroll
+          for (int j = 0; j < NQ * BM / 32; ++j) {
+            const int i = lane + 32 * j;
+            int p = -1;
+            if (i < n_tok) {
+              p = a.positions[t0 + i];
+              if (p >= a.n_ctx) {
+                if (gi == 0 && hk == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
+                p = a.n_ctx - 1;
+              }
+              p = max(p, -1);
+            }
+            pv[j] = p;
+            mx = max(mx, p);
+          }
+          mx = __reduce_max_sync(0xffffffffu, mx);
+          const int kt_all = max(mx, 0) / BN + 1;  // key tiles 0 .. last visible key (one at least)
+          const int n_split = (kt_all + a.tps - 1) / a.tps;
+          const int z = n_split - a.max_splits + gi;  // see Item
+          if (z >= 0) {
+            rec = Item{rb, hk, z, n_split, z * a.tps, min(a.tps, kt_all - z * a.tps), mx, n_tok > T ? 2 : 1};
+            break;
+          }
+        }
+        cursor += gridDim.x;
+        const int s = it % kItemSlots;
+        bool free_slot = true;
+        if (lane == 0) free_slot = mbar_wait(&item_empty[s], ((it / kItemSlots) & 1) ^ 1, abort, &g_err_word);
+        if (!__shfl_sync(0xffffffffu, free_slot ? 1 : 0, 0)) break;
+#pragma unroll
+        for (int j = 0; j < NQ * BM / 32; ++j) s_pos[s * NQ * BM + lane + 32 * j] = pv[j];
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) {
+          items[s] = rec;
+          mbar_arrive(&item_full[s]);
+        }
+        if (rec.rb < 0) break;
+        ++it;
+      }
+    } else if (warp == kWarpMma && lane == 0) {
+      // ---------------------------------------------------------------- MMA issuer
+      auto issue_s = [&](int w, int gt, bool last) {
+        const uint32_t q0 = smem_u32(sQ + w * C::Q_BYTES);
+        const uint32_t k0 = smem_u32(sK + (gt % KS) * C::KV_TILE);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * ATOM_BYTES + (kk & 3) * 32;
+          tc_mma_f16(tmem + w * BN, umma_desc_sw128(q0 + off), umma_desc_sw128(k0 + off), C::IDESC_S, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&s_full[w]);
+        if (last) tc_commit(&q_free[w]);  // Q tile w may be overwritten for the next item
+      };
+      auto issue_pv = [&](int w, int gt, bool first) {
+        const uint32_t v0 = smem_u32(sV + (gt % VS) * C::KV_TILE);
+        const uint32_t pbuf = tmem + w * BN;
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          tc_mma_f16_ts(tmem + O_COL + w * 128, pbuf + kk * 8, umma_desc_sw128_mn(v0 + kk * 16 * 128, ATOM_BYTES), C::IDESC_PV,
+                        (!first || kk > 0) ? 1u : 0u);
+        tc_commit(&o_done[w]);
+      };
+      bool ok = true;
+      int g = 0;                  // key tiles consumed (all items)
+      int gw[NQ] = {}, qw[NQ] = {};  // per Q tile: key tiles and items
+      for (int it = 0; ok; ++it) {
+        const int s = it % kItemSlots;
+        if (!mbar_wait(&item_full[s], (it / kItemSlots) & 1, abort, &g_err_word)) {
+          ok = false;
+          break;
+        }
+        const int n_kt = items[s].rb < 0 ? -1 : items[s].n_kt, nq = items[s].pad1;
+        mbar_arrive(&item_empty[s]);
+        if (n_kt < 0) break;
+        if (!mbar_wait(&k_full[g % KS], (g / KS) & 1, abort, &g_err_word)) {
+          ok = false;
+          break;
+        }
+        for (int w = 0; w < nq && ok; ++w) {
+          if (!mbar_wait(&q_ready[w], qw[w] & 1, abort, &g_err_word)) {
+            ok = false;
+            break;
+          }
+          ++qw[w];
+          tc_fence_after();
+          issue_s(w, g, n_kt == 1);
+        }
+        if (!ok) break;
+        tc_commit(&k_empty[g % KS]);
+        for (int j = 0; j < n_kt && ok; ++j) {
+          const int gt = g + j, nxt = gt + 1;
+          for (int w = 0; w < nq && ok; ++w) {
+            if (!mbar_wait(&p_full[w], (gw[w] + j) & 1, abort, &g_err_word) ||
+                (w == 0 && !mbar_wait(&v_full[gt % VS], (gt / VS) & 1, abort, &g_err_word))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            issue_pv(w, gt, j == 0);
+            if (j + 1 == n_kt) tc_commit(&o_full[w]);  // O of tile w is final
+            if (w == nq - 1) tc_commit(&v_empty[gt % VS]);
+            if (j + 1 < n_kt) {
+              if (w == 0 && !mbar_wait(&k_full[nxt % KS], (nxt / KS) & 1, abort, &g_err_word)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              issue_s(w, nxt, j + 2 == n_kt);
+              if (w == nq - 1) tc_commit(&k_empty[nxt % KS]);
+            }
+          }
+        }
+        g += n_kt;
+        for (int w = 0; w < nq; ++w) gw[w] += n_kt;
+      }
+      if (!ok) {
+        tc_commit(drain);
+        drain_wait(drain, 0);
+      }
+    }
+  } else if (warp >= kWarpConv) {
+    // ------------------------------------------------------------------- converters
+    regs_dec<kRegsConv>();
+    const int t = threadIdx.x - kWarpConv * 32;  // 0 .. 127
+    constexpr int CPR = HD / 16;                 // 16-code chunks per row
+    constexpr int NCH = BN * CPR / 128;          // chunks per thread and tile (8 or 4)
+    constexpr int RSTEP = 128 / CPR;             // rows per pass
+    const int cr = t / CPR, cc = t % CPR;        // row of the first pass, chunk
+    // operand tile address of chunk cc of row r: 64-column atom cc / 4, 16-byte units
+    // 2 (cc % 4) and + 1, swizzled by r % 8 (r % 8 is the same in every pass)
+    const uint32_t sw = uint32_t(cr & 7);
+    const uint32_t u0 = ((2u * (cc & 3)) ^ sw) * 16u, u1 = ((2u * (cc & 3) + 1u) ^ sw) * 16u;
+    const uint32_t base = uint32_t(cc >> 2) * ATOM_BYTES + uint32_t(cr) * 128u;
+    const bool odd = (cc & 4) != 0;  // the two atoms' lanes write their halves in opposite order: distinct banks
+    const uint32_t first_u = odd ? u1 : u0, second_u = odd ? u0 : u1;
+    auto load = [&](const uint8_t* src, int hk, int kt, int last, uint4(&x)[NCH]) {
+      const int64_t row0 = int64_t(hk) * a.n_blocks * kBlk + int64_t(kt) * BN;
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const int r = i * RSTEP + cr;
+        x[i] = kt * BN + r <= last ? __ldg(reinterpret_cast<const uint4*>(src + (row0 + r) * HD) + cc) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    auto store = [&](uint8_t* tile, const uint4(&x)[NCH]) {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i) {
+        const uint2 p0 = widen4<E4M3>(x[i].x), p1 = widen4<E4M3>(x[i].y), p2 = widen4<E4M3>(x[i].z), p3 = widen4<E4M3>(x[i].w);
+        const uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
+        uint8_t* row = tile + base + i * RSTEP * 128;
+        *reinterpret_cast<uint4*>(row + first_u) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(row + second_u) = odd ? lo : hi;
+      }
+    };
+    bool ok = true;
+    int g = 0;         // key tiles converted (all items)
+    int qn[NQ] = {};   // Q tiles converted
+    for (int it = 0; ok; ++it) {
+      const int s = it % kItemSlots;
+      if (!warp_wait(&item_full[s], (it / kItemSlots) & 1, abort)) break;
+      const Item rec = items[s];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[s]);
+      if (rec.rb < 0) break;
+      const int last = rec.pad0;
+      uint4 x[NCH], y[NCH];
+      load(a.k, rec.hk, rec.kt0, last, x);
+      // the item's V scale reference: the power of two at or above its largest scale
+      {
+        const int b1 = min((rec.kt0 + rec.n_kt) * GRP, (last + kBlk) / kBlk);
+        float mx = 0.f;
+        for (int b = rec.kt0 * GRP + t; b < b1; b += 128) mx = fmaxf(mx, __ldg(a.vs + int64_t(rec.hk) * a.n_blocks + b));
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));
+        if (lane == 0) s_red[warp - kWarpConv] = __uint_as_float((bits + 0x007fffffu) & 0x7f800000u);
+        conv_barrier();
+      }
+      float ref = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+      ref = ref > 0.f ? ref : 1.0f;
+      if (t == 0) s_ref[it & 3] = ref;
+      conv_barrier();  // s_red may be rewritten for the next item
+      for (int j = 0; j < rec.n_kt; ++j) {
+        const int gt = g + j, kt = rec.kt0 + j;
+        load(a.v, rec.hk, kt, last, y);
+        float ks = 0.f, vs = 0.f;
+        if (t < GRP && kt * BN + t * kBlk <= last) {
+          const int64_t b = int64_t(rec.hk) * a.n_blocks + kt * GRP + t;
+          ks = __ldg(a.ks + b);
+          vs = __ldg(a.vs + b);
+        }
+        if (!warp_wait(&k_empty[gt % KS], ((gt / KS) & 1) ^ 1, abort)) {
+          ok = false;
+          break;
+        }
+        store(sK + (gt % KS) * C::KV_TILE, x);
+        if (t < GRP) {
+          // a block of zeros (scale 0) adds nothing whatever its weight: any scale will do
+          const int sl = (gt % kScaleSlots) * GRP + t;
+          s_ks[sl] = ks;
+          s_lv[sl] = (vs > 0.f ? log2f(vs / ref) : 0.f) + kPBits;
+          s_iv[sl] = vs > 0.f ? ref / vs : 1.0f;
+        }
+        fence_async_smem();
+        mbar_arrive(&k_full[gt % KS]);
+        if (j + 1 < rec.n_kt) load(a.k, rec.hk, kt + 1, last, x);
+        if (!warp_wait(&v_empty[gt % VS], ((gt / VS) & 1) ^ 1, abort)) {
+          ok = false;
+          break;
+        }
+        store(sV + (gt % VS) * C::KV_TILE, y);
+        fence_async_smem();
+        mbar_arrive(&v_full[gt % VS]);
+        if (j == 0) {
+          // the item's Q tiles, once the item before has no S MMA left on them
+          constexpr int QPR = HD / 8;          // lanes per row
+          constexpr int QSTEP = 128 / QPR;     // rows per pass
+          constexpr int QB = 4;                // passes whose loads are in flight together
+          const int qr = t / QPR, qc = t % QPR;
+          const int n_tok = min(NQ * T, a.M - rec.rb * NQ * T);
+          for (int w = 0; w < rec.pad1 && ok; ++w) {
+            if (qn[w] > 0 && !warp_wait(&q_free[w], (qn[w] - 1) & 1, abort)) {
+              ok = false;
+              break;
+            }
+            ++qn[w];
+#pragma unroll 1
+            for (int p0 = 0; p0 < BM / QSTEP; p0 += QB) {
+              uint4 z[QB];
+#pragma unroll
+              for (int i = 0; i < QB; ++i) {
+                const int r = (p0 + i) * QSTEP + qr;
+                const int tr = r / G, tok = w * T + tr;
+                z[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (r < T * G && tok < n_tok)
+                  z[i] = __ldg(reinterpret_cast<const uint4*>(
+                                   a.q + (int64_t(rec.rb * NQ * T + tok) * a.Hq + rec.hk * G + (r - tr * G)) * HD) + qc);
+              }
+#pragma unroll
+              for (int i = 0; i < QB; ++i) {
+                const int r = (p0 + i) * QSTEP + qr;
+                // the power of two that puts the row's largest value in [2^14, 2^15)
+                const uint32_t mg = __vmaxu2(__vmaxu2(z[i].x & 0x7fff7fffu, z[i].y & 0x7fff7fffu),
+                                             __vmaxu2(z[i].z & 0x7fff7fffu, z[i].w & 0x7fff7fffu));
+                uint32_t am = max(mg & 0xffffu, mg >> 16);
+#pragma unroll
+                for (int o = 1; o < QPR; o <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
+                const int sh = am == 0 ? 0 : max(-126, min(126, 14 + 127 - int(am >> 7)));
+                const float up = __uint_as_float(uint32_t(sh + 127) << 23);
+                if (qc == 0) s_qf[((it & 1) * NQ + w) * BM + r] = a.scale_log2 * __uint_as_float(uint32_t(127 - sh) << 23);
+                const uint4 h = make_uint4(pack_h2(lo_bf(z[i].x) * up, hi_bf(z[i].x) * up), pack_h2(lo_bf(z[i].y) * up, hi_bf(z[i].y) * up),
+                                           pack_h2(lo_bf(z[i].z) * up, hi_bf(z[i].z) * up), pack_h2(lo_bf(z[i].w) * up, hi_bf(z[i].w) * up));
+                *reinterpret_cast<uint4*>(sQ + w * C::Q_BYTES + (qc >> 3) * ATOM_BYTES + r * 128 + (((qc & 7) ^ (r & 7)) << 4)) = h;
+              }
+            }
+            fence_async_smem();
+            mbar_arrive(&q_ready[w]);
+          }
+          if (!ok) break;
+        }
+      }
+      g += rec.n_kt;
+    }
+  } else {
+    // ------------------------------------------------- softmax / correction / epilogue
+    regs_inc<kRegsSoftmax>();
+    const int w = warp >> 2;         // Q tile of this warpgroup
+    const int sub = warp & 3;        // TMEM sub-partition (lanes 32*sub .. +31)
+    const int r = sub * 32 + lane;   // row in the Q tile == TMEM lane
+    const int tr = r / G;            // token of the row in the Q tile
+    const uint32_t lane_base = tmem + (uint32_t(sub * 32) << 16);
+    const uint32_t sbuf = lane_base + w * BN;
+    const uint32_t obuf = lane_base + O_COL + w * 128;
+
+    bool ok = true;
+    int g = 0;   // key tiles seen (all items): the scale slots
+    int gw = 0;  // of them, by this Q tile
+    int iw = 0;  // items by this Q tile
+    for (int it = 0; ok; ++it) {
+      const int s = it % kItemSlots;
+      if (!warp_wait(&item_full[s], (it / kItemSlots) & 1, abort)) {
+        ok = false;
+        break;
+      }
+      const Item cur = items[s];
+      const int n_tok = min(NQ * T, a.M - cur.rb * NQ * T);
+      const int tt = w * T + tr;  // token index in the item
+      const bool valid = cur.rb >= 0 && r < T * G && tt < n_tok;
+      // padding rows see every key: they never force the masked path on their warp
+      const int pos = valid ? s_pos[s * NQ * BM + tt] : a.n_ctx - 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[s]);
+      if (cur.rb < 0) break;
+      if (w >= cur.pad1) {  // no rows on this tile
+        g += cur.n_kt;
+        continue;
+      }
+      float m = -INFINITY, l = 0.f, factor = 0.f, ref = 1.0f;
+      for (int j = 0; j < cur.n_kt; ++j) {
+        const int gt = g + j;
+        if (!warp_wait(&s_full[w], (gw + j) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (j == 0) {
+          factor = s_qf[((it & 1) * NQ + w) * BM + r];
+          ref = s_ref[it & 3];
+        }
+        const int lim = pos - (cur.kt0 + j) * BN;  // keys at index > lim are masked
+        const bool full = __all_sync(0xffffffffu, lim >= BN - 1);
+        const float* ksl = s_ks + (gt % kScaleSlots) * GRP;
+        const float* lvl = s_lv + (gt % kScaleSlots) * GRP;
+        const float* ivl = s_iv + (gt % kScaleSlots) * GRP;
+        float c8[GRP];
+#pragma unroll
+        for (int b = 0; b < GRP; b += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(ksl + b);
+          c8[b] = x.x * factor, c8[b + 1] = x.y * factor, c8[b + 2] = x.z * factor, c8[b + 3] = x.w * factor;
+        }
+        // pass 1: row max; a 16-column group's raw maximum times its factor (>= 0)
+        float mx = -INFINITY;
+#pragma unroll
+        for (int h = 0; h < BN / 64; ++h) {
+          uint32_t u[64];
+          tmem_ld64w(sbuf + 64 * h, u);
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+              if (64 * h + e > lim) u[e] = __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const uint32_t* x = u + 16 * b;
+            float p = max3f(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+            float q2 = max3f(__uint_as_float(x[3]), __uint_as_float(x[4]), __uint_as_float(x[5]));
+#pragma unroll
+            for (int e = 6; e < 14; e += 4) {
+              p = max3f(p, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+              q2 = max3f(q2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+            }
+            p = max3f(p, __uint_as_float(x[14]), __uint_as_float(x[15]));
+            mx = fmaxf(mx, fmaxf(p, q2) * c8[4 * h + b]);  // -inf * 0 is NaN, which fmaxf drops
+          }
+        }
+        const float m_new = fmaxf(m, mx);
+        const bool need = j > 0 && m_new > m + kRescaleThreshold;
+        if (__any_sync(0xffffffffu, need)) {
+          // O may be touched only after P(j-1) V(j-1) has landed
+          if (!warp_wait(&o_done[w], (gw + j - 1) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const float corr = need ? ex2_approx(m - m_new) : 1.0f;
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            float o[32];
+            tmem_ld32(obuf + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= corr;
+            tmem_st32(obuf + c, o);
+          }
+          l *= corr;
+        }
+        if (j == 0 || need) m = m_new;
+        // pass 2: P' = 2^(s c - m + log2(vs / ref) + 7), one packed multiply-add per pair, back
+        // over S as fp16 pairs; masked keys give exactly 0.  A row that has seen no key yet
+        // keeps m = -inf and takes 0 as its base.
+        const float neg_m = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+        for (int h = 0; h < BN / 64; ++h) {
+          uint32_t u[64];
+          tmem_ld64w(sbuf + 64 * h, u);
+          const float4 lv = *reinterpret_cast<const float4*>(lvl + 4 * h);
+          const float4 iv = *reinterpret_cast<const float4*>(ivl + 4 * h);
+          const float lv4[4] = {lv.x, lv.y, lv.z, lv.w}, iv4[4] = {iv.x, iv.y, iv.z, iv.w};
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float2 sc2 = make_float2(c8[4 * h + b], c8[4 * h + b]);
+            const float add = neg_m + lv4[b];
+            const float2 nm2 = make_float2(add, add);
+            float2 rs0 = make_float2(0.f, 0.f), rs1 = rs0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int pr = 8 * b + e;
+              const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[2 * pr]), __uint_as_float(u[2 * pr + 1])), sc2, nm2);
+              float2 pv = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              if (!full) {
+                pv.x = 64 * h + 2 * pr <= lim ? pv.x : 0.f;
+                pv.y = 64 * h + 2 * pr + 1 <= lim ? pv.y : 0.f;
+              }
+              if (e & 1) rs1 = __fadd2_rn(rs1, pv);
+              else rs0 = __fadd2_rn(rs0, pv);
+              u[pr] = pack_h2(pv.x, pv.y);
+            }
+            const float2 rs = __fadd2_rn(rs0, rs1);
+            l = fmaf(rs.x + rs.y, iv4[b], l);
+          }
+          tmem_st32u(sbuf + 32 * h, *reinterpret_cast<const uint32_t(*)[32]>(u));
+        }
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+      }
+      if (!ok) break;
+      g += cur.n_kt;
+      gw += cur.n_kt;
+      if (!warp_wait(&o_full[w], iw & 1, abort)) {
+        ok = false;
+        break;
+      }
+      ++iw;
+      tc_fence_after();
+      uint32_t* stg = s_stage + warp * (32 * kStageStride);
+      if (cur.n_split > 1) {
+        // one slice of the keys: unnormalised O (times the reference) with its (max, sum), in the
+        // column-chunk-major layout that the combine kernel reads, by 1 KiB bulk stores
+        const int64_t blk = (int64_t((cur.rb * a.Hk + cur.hk) * a.max_splits + cur.split) * NQ + w) * BM * HD;
+        float* gdst = a.part_o + blk + sub * 32 * 8;
+        uint8_t* stg8 = reinterpret_cast<uint8_t*>(stg);
+        const int swz = (lane >> 2) & 1;
+        int chunk = 0;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float o[32];
+          tmem_ld32(obuf + c, o);
+#pragma unroll
+          for (int h = 0; h < 4; ++h, ++chunk) {
+            uint8_t* buf = stg8 + (chunk & 1) * 1024;
+            if (chunk >= 2) {  // the store that last read this buffer has read it
+              if (lane == 0) bulk_wait_read<1>();
+              __syncwarp();
+            }
+            float4* mine = reinterpret_cast<float4*>(buf + lane * 32);
+            mine[swz] = make_float4(o[8 * h] * ref, o[8 * h + 1] * ref, o[8 * h + 2] * ref, o[8 * h + 3] * ref);
+            mine[swz ^ 1] = make_float4(o[8 * h + 4] * ref, o[8 * h + 5] * ref, o[8 * h + 6] * ref, o[8 * h + 7] * ref);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              bulk_store(gdst + (c / 8 + h) * (BM * 8), buf, 1024);
+              bulk_commit();
+            }
+          }
+        }
+        if (lane == 0) bulk_wait_read<0>();  // both buffers free for the next epilogue
+        __syncwarp();
+        if (valid) {
+          const int64_t prow = int64_t((cur.rb * a.Hk + cur.hk) * a.max_splits + cur.split) * (NQ * BM) + w * BM + r;
+          a.part_ml[prow] = make_float2(m, l);
+        }
+      } else {
+        // 16 words of each row at a time through the warp's staging tile: four lanes per row,
+        // eight rows per store instruction
+        int64_t dst[4];
+        {
+          const int t0 = cur.rb * NQ * T;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int rq = sub * 32 + 8 * k + (lane >> 2);
+            const int tq = rq / G, gq = rq - tq * G, ttq = w * T + tq;
+            const bool vq = rq < T * G && ttq < n_tok;
+            dst[k] = !vq ? -1 : (int64_t(t0 + ttq) * a.Hq + cur.hk * G + gq) * HD;
+          }
+        }
+        const float inv = l > 0.f ? ref / l : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float o[32];
+          tmem_ld32(obuf + c, o);
+          uint4* mine = reinterpret_cast<uint4*>(stg + lane * kStageStride);
+#pragma unroll
+          for (int qd = 0; qd < 4; ++qd)
+            mine[qd] = make_uint4(pack_bf2(o[8 * qd] * inv, o[8 * qd + 1] * inv), pack_bf2(o[8 * qd + 2] * inv, o[8 * qd + 3] * inv),
+                                  pack_bf2(o[8 * qd + 4] * inv, o[8 * qd + 5] * inv), pack_bf2(o[8 * qd + 6] * inv, o[8 * qd + 7] * inv));
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint4 x = reinterpret_cast<const uint4*>(stg + (8 * k + (lane >> 2)) * kStageStride)[lane & 3];
+            if (dst[k] >= 0) *reinterpret_cast<uint4*>(a.out + dst[k] + c + (lane & 3) * 8) = x;
+          }
+          __syncwarp();
+        }
+      }
+      // O has been read: the next item's first P V (which overwrites it) is issued only
+      // after this warpgroup's next p_full
+      tc_fence_before();
+    }
+    // the split partials' bulk stores have written global memory before the CTA ends
+    if (lane == 0) bulk_wait_all();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kWarpMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Packed rows per KV head from which the tile kernel takes over.
+constexpr int kTileRows = 33;
+
+bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) >= kTileRows; }
+
+template <int HD, bool E4M3>
+int launch_tiles(Args a, const SplitPlan& p, void* workspace, cudaStream_t stream) {
+  auto kern = attention_kv8_kernel<HD, E4M3>;
+  static int regs = 0;  // the register split needs what the kernel is launched with
+  if (regs == 0) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) {
+      set_error("ckv_attention_kv8: cudaFuncGetAttributes: %s", cudaGetErrorString(cudaGetLastError()));
+      return CKV_ERR_CUDA;
+    }
+    regs = fa.numRegs;
+  }
+  if (regs != 128) {
+    set_error("ckv_attention_kv8: built with %d registers per thread, its register split needs 128", regs);
+    return CKV_ERR_CUDA;
+  }
+  if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), Cfg<HD>::SMEM)) return rc;
+  if (p.max_splits > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(p.blocks) * a.Hk * p.max_splits * NQ * BM * HD);
+  }
+  a.tps = p.tps, a.max_splits = p.max_splits, a.blocks = p.blocks;
+  const int64_t n_slots = int64_t(p.blocks) * a.Hk * p.max_splits;
+  CKV_REQUIRE(n_slots < (int64_t(1) << 31) - 4 * 1024 * 1024, "ckv_attention_kv8: too many work items");
+  launch_pdl(kern, dim3(int(std::min<int64_t>(n_slots, num_sms()))), dim3(kThreads), Cfg<HD>::SMEM, stream, a);
+  CKV_LAUNCH_CHECK("ckv_attention_kv8");
+  if (p.max_splits > 1) {
+    launch_pdl(attention_combine_kernel<HD>, dim3(p.blocks * (NQ * BM / (kCombineWarps * kCombineRows)), a.Hk),
+               dim3(kCombineWarps * 32), 0, stream, a.positions, a.out, a.M, a.Hq, a.Hk, a.n_ctx, p.tps, p.max_splits,
+               static_cast<const float*>(a.part_o), static_cast<const float2*>(a.part_ml));
+    CKV_LAUNCH_CHECK("ckv_attention_kv8(combine)");
+  }
+  return CKV_OK;
+}
 
 bool shape_ok(int m, int Hq, int Hk, int HD, int n_ctx) {
   return m > 0 && Hk > 0 && Hk <= 65535 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 128 && (HD == 64 || HD == 128) && n_ctx > 0 &&
@@ -22,11 +749,14 @@ using namespace ckv;
 
 extern "C" int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
-  return kv8_stream_workspace(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
+  return use_tiles(m, n_q_heads, n_kv_heads) ? plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
+                                             : kv8_stream_workspace(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
 extern "C" int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
+  if (use_tiles(m, n_q_heads, n_kv_heads))
+    return plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx).max_splits > 1 ? 2 : 1;
   return kv8_stream_launches(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
@@ -43,11 +773,21 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
               n_q_heads / n_kv_heads, n_ctx);
     return CKV_ERR_UNSUPPORTED;
   }
-  CKV_REQUIRE(k_scale && v_scale, "ckv_attention_kv8: null scales");
-  const int64_t need = kv8_stream_workspace(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
+  CKV_REQUIRE(q && k8 && v8 && k_scale && v_scale && positions && out, "ckv_attention_kv8: null pointer");
+  CKV_REQUIRE(aligned16(q) && aligned16(k8) && aligned16(v8) && aligned16(out),
+              "ckv_attention_kv8: tensors must be 16-byte aligned");
+  const int64_t need = ckv_attention_kv8_workspace_size(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
   CKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "ckv_attention_kv8: workspace of %lld bytes, needs %lld (16-byte aligned)", static_cast<long long>(workspace_bytes),
               static_cast<long long>(need));
-  return kv8_stream_attention(q, k8, v8, k_scale, v_scale, positions, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, scale, type,
-                              workspace, as_stream(stream));
+  if (!use_tiles(m, n_q_heads, n_kv_heads))
+    return kv8_stream_attention(q, k8, v8, k_scale, v_scale, positions, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, scale, type,
+                                workspace, as_stream(stream));
+  const Args a{q, k8, v8, k_scale, v_scale, positions, out, nullptr, nullptr, m, n_q_heads, n_kv_heads, n_ctx,
+               ceil_div(n_ctx, kBlk), 0, 0, 0, scale * 1.4426950408889634f};
+  const SplitPlan p = plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
+  const cudaStream_t s = as_stream(stream);
+  if (head_dim == 128)
+    return type == CKV_KV8_E4M3 ? launch_tiles<128, true>(a, p, workspace, s) : launch_tiles<128, false>(a, p, workspace, s);
+  return type == CKV_KV8_E4M3 ? launch_tiles<64, true>(a, p, workspace, s) : launch_tiles<64, false>(a, p, workspace, s);
 }

@@ -39,28 +39,21 @@
 // last S MMA on that tile is done, so the next item's first S MMA overlaps this item's
 // last P V and its epilogue.  Each Q tile has its own "O complete" barrier, so one
 // warpgroup's epilogue never waits for the other's last tile.
-#include <algorithm>
-#include <mutex>
-#include <vector>
-
 #include "ckv_common.cuh"
 
 CKV_DEFINE_ERR_WORD(attention_tc)
 
+#include "attention_split.cuh"
+
 namespace ckv {
 namespace {
 
-constexpr int BM = 128;  // rows per Q tile (packed token x head)
-constexpr int NQ = 2;    // Q tiles per CTA
-constexpr int BN = 128;  // keys per tile
 constexpr int KS = 2;    // K stages
 constexpr int VS = 2;    // V stages
 constexpr int kThreads = NQ * 128 + 64;  // two softmax warpgroups + producer + MMA warps
 constexpr int kWarpTma = 8, kWarpMma = 9;
 constexpr uint32_t TMEM_COLS = 512;  // S/P of tile w at [128w, 128w+128), O of tile w at 256+128w
 constexpr uint32_t O_COL = 256;
-constexpr uint32_t ATOM_BYTES = 128 * 128;  // one [128 rows][64 bf16] swizzle-128 atom
-constexpr float kRescaleThreshold = 8.0f;   // log2 units
 
 template <int HD>
 struct Cfg {
@@ -78,38 +71,6 @@ struct Cfg {
   static constexpr uint32_t IDESC_PV = umma_idesc_bf16(BM, HD) | (1u << 16);  // B MN-major
 };
 
-// all lanes wait; the warp agrees on the outcome so collective TMEM ops stay converged
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  const bool ok = mbar_wait(bar, parity, abort, &g_err_word);
-  return __all_sync(0xffffffffu, ok);
-}
-
-__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity) {
-  const uint64_t t0 = global_ns();
-  while (!mbar_try_wait(bar, parity))
-    if (global_ns() - t0 > kWaitLimitNs) break;
-}
-
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-// Work items: (row block rb, KV head hk, key split z).  Slots come in groups of one
-// per (head, row block), row blocks from the last (longest) one down; group gi holds
-// split z = n_split - max_splits + gi of the block, so a block's last split, the only
-// one shorter than tps key tiles, is in the last group, and the longest blocks' full
-// splits come first: roughly longest first over the whole grid.  A slot with z < 0 (a
-// block with fewer splits) is empty and skipped.
-struct Item {
-  int rb, hk, split, n_split, kt0, n_kt, pad0, pad1;  // rb < 0: no more work
-};
-constexpr int kItemSlots = 4;  // ring of items published by the producer warp
-// Epilogue staging: per softmax warp 32 rows x 16 words, rows padded to 20 words (80 B)
-// so that the 16-byte writes of eight consecutive lanes fall in distinct banks
-constexpr int kStageStride = 20;
-constexpr uint32_t kStageBytes = NQ * 4 * 32 * kStageStride * 4;
 static_assert(kItemSlots * (sizeof(Item) + NQ * BM * sizeof(int)) + kStageBytes + 40 * sizeof(uint64_t) + 8 <=
                   4096 + 20480 + 512,
               "item ring, positions, staging and barriers must fit the shared-memory reserve");
@@ -652,168 +613,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
-}
-
-// Merge the key splits of the row blocks that were split: O = sum_s 2^(m_s - M) O_s /
-// sum_s 2^(m_s - M) l_s with M = max_s m_s (all in the log2 domain of the kernel).
-// A warp takes kCombineRows packed rows; for each, lane s reads split s's (m, l), then
-// each lane sums its four columns over the splits, the loads of all its rows in flight
-// together (one wave of CTAs at the 7B shape).  Rows of unsplit blocks were written
-// directly.
-constexpr int kCombineWarps = 8;
-constexpr int kCombineRows = 4;
-template <int HD>
-__global__ void __launch_bounds__(kCombineWarps * 32, 4) attention_combine_kernel(
-    const int32_t* __restrict__ positions, uint16_t* __restrict__ out, int M, int Hq, int Hk, int n_ctx,
-    int tps, int max_splits, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
-  pdl_wait();  // the partials come from the attention kernel just before (dependent launch)
-  pdl_launch_next();
-  constexpr int R = kCombineRows;
-  const int G = Hq / Hk;
-  const int T = BM / G;
-  constexpr int kChunks = NQ * BM / (kCombineWarps * R);  // CTAs per (row block, KV head)
-  const int rb = blockIdx.x / kChunks, chunk = blockIdx.x - rb * kChunks, hk = blockIdx.y;
-  const int t0 = rb * NQ * T;
-  const int n_tok = min(NQ * T, M - t0);
-  __shared__ int s_max;
-  if (threadIdx.x == 0) s_max = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_tok; i += blockDim.x)
-    atomicMax(&s_max, min(max(positions[t0 + i], 0), n_ctx - 1));
-  __syncthreads();
-  const int n_split = ((s_max + BN) / BN + tps - 1) / tps;
-  if (n_split <= 1) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t stride = NQ * BM;
-  const int64_t blk = int64_t((rb * Hk + hk) * max_splits);
-  // lane v < HD / 4 takes columns 4v .. 4v + 3: 16-byte half (v & 1) of 8-column chunk
-  // v >> 1, stored swapped with the other half when bit 2 of the row is set (the
-  // kernel's column-chunk-major partial layout)
-  const bool mine = lane < HD / 4;
-  float wgt[R], inv[R];
-  int off[R];
-  int64_t orow[R];
-  bool ok[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int pr = (chunk * kCombineWarps + warp) * R + i;
-    const int w = pr / BM, r = pr - w * BM;
-    const int tr = r / G, g = r - tr * G, tt = w * T + tr;
-    ok[i] = r < T * G && tt < n_tok;  // the same for the whole warp
-    const float2 ml =
-        ok[i] && lane < n_split ? part_ml[blk * stride + pr + lane * stride] : make_float2(-INFINITY, 0.f);
-    float mmax = ml.x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mmax = fmaxf(mmax, __shfl_xor_sync(0xffffffffu, mmax, o));
-    wgt[i] = ok[i] && lane < n_split ? exp2f(ml.x - mmax) : 0.f;
-    float L = wgt[i] * ml.y;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    inv[i] = L > 0.f ? 1.0f / L : 0.f;
-    off[i] = w * (BM * HD) + (lane >> 1) * (BM * 8) + r * 8 + (((lane & 1) ^ ((r >> 2) & 1)) << 2);
-    orow[i] = (int64_t(t0 + tt) * Hq + hk * G + g) * HD;
-  }
-  const float* po = part_o + blk * NQ * BM * HD;
-  float4 acc[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int sp = 0; sp < n_split; ++sp) {
-    const float* ps = po + int64_t(sp) * NQ * BM * HD;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float ws = __shfl_sync(0xffffffffu, wgt[i], sp);
-      if (mine && ok[i]) {
-        const float4 x = *reinterpret_cast<const float4*>(ps + off[i]);
-        acc[i].x = fmaf(ws, x.x, acc[i].x);
-        acc[i].y = fmaf(ws, x.y, acc[i].y);
-        acc[i].z = fmaf(ws, x.z, acc[i].z);
-        acc[i].w = fmaf(ws, x.w, acc[i].w);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-    if (mine && ok[i])
-      *reinterpret_cast<uint2*>(out + orow[i] + 4 * lane) =
-          make_uint2(pack_bf2(acc[i].x * inv[i], acc[i].y * inv[i]), pack_bf2(acc[i].z * inv[i], acc[i].w * inv[i]));
-}
-
-// Key-split plan: split only when the unsplit grid leaves SMs idle.
-struct SplitPlan {
-  int tps, max_splits, blocks;
-  int64_t bytes;  // partial O and (max, sum) of every split item
-};
-// The workspace starts with the scheduler's two words (next slot, CTAs done), padded to
-// 256 bytes; the split partials follow.
-constexpr int64_t kSchedBytes = 256;
-// Fixed cost of one item, in key-tile times, for the persistent kernel: its first S
-// MMA and the epilogue are only partly hidden behind the neighbouring items; a split
-// item also writes its fp32 partial O.
-constexpr double kItemCost = 0.7;
-constexpr double kSplitItemCost = 1.0;
-// Estimated makespan, in key-tile times, of a split plan: the list-scheduling estimate
-// total work / SMs + half the largest item (items go out roughly largest first), plus,
-// when split, the combine (reading every partial at the HBM rate: one tile time per
-// 14.3 MB).  Row block b is assumed to reach position (b + 1) / blocks * n_ctx (sorted
-// positions spread over the context, as the engine passes them).
-double plan_cost(int blocks, int Hk, int HD, int n_ctx, int tps, int sms) {
-  const bool split = tps < ceil_div(n_ctx, BN);
-  const double cta_cost = kItemCost + (split ? kSplitItemCost : 0.0);
-  double total = 0.0;
-  int64_t items_all = 0;
-  int max_item = 0;
-  for (int b = 0; b < blocks; ++b) {
-    const int kt = std::max(1, ceil_div((int64_t(b) + 1) * n_ctx / blocks, BN));
-    const int items = ceil_div(kt, tps);
-    total += kt + items * cta_cost;
-    items_all += items;
-    max_item = std::max(max_item, std::min(kt, tps));
-  }
-  total *= Hk;
-  const double combine = split ? double(items_all) * Hk * NQ * BM * (HD * 4 + 8) / 14.3e6 : 0.0;
-  return total / sms + 0.5 * (max_item + cta_cost) + combine;
-}
-
-// Key-split plan: the tiles-per-split with the smallest estimated makespan (no split
-// included).  Plans are cached per shape.
-SplitPlan plan_splits(int M, int Hq, int Hk, int HD, int n_ctx) {
-  struct Key {
-    int M, Hq, Hk, HD, n_ctx, sms;
-  };
-  static std::mutex mu;
-  static std::vector<std::pair<Key, SplitPlan>> cache;
-  const int sms = num_sms();
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    for (const auto& e : cache)
-      if (e.first.M == M && e.first.Hq == Hq && e.first.Hk == Hk && e.first.HD == HD &&
-          e.first.n_ctx == n_ctx && e.first.sms == sms)
-        return e.second;
-  }
-  const int T = BM / (Hq / Hk);
-  SplitPlan p;
-  p.blocks = ceil_div(M, NQ * T);
-  const int max_kt = ceil_div(n_ctx, BN);
-  const double unsplit = plan_cost(p.blocks, Hk, HD, n_ctx, max_kt, sms);
-  int best_tps = max_kt;
-  double best = unsplit;
-  // at most 32 splits: the combine gives each split one lane
-  for (int tps = std::max(2, ceil_div(max_kt, 32)); tps < max_kt; tps = tps < 8 ? tps + 1 : tps + tps / 4) {
-    const double c = plan_cost(p.blocks, Hk, HD, n_ctx, tps, sms);
-    if (c < best) {
-      best = c;
-      best_tps = tps;
-    }
-  }
-  // split only when the estimate promises at least 10 %
-  if (best > 0.90 * unsplit) best_tps = max_kt;
-  p.tps = best_tps;
-  p.max_splits = ceil_div(max_kt, p.tps);
-  p.bytes = p.max_splits > 1 ? int64_t(p.blocks) * Hk * p.max_splits * NQ * BM * (int64_t(HD) * 4 + 8) : 0;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cache.size() < 256) cache.push_back({Key{M, Hq, Hk, HD, n_ctx, sms}, p});
-  return p;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,

@@ -73,6 +73,7 @@ uint32_t read_clear_err_gemv_fused();
 uint32_t read_clear_err_kv8();
 uint32_t read_clear_err_block_select();
 uint32_t read_clear_err_attention_blocks();
+uint32_t read_clear_err_attention_kv8();
 
 }  // namespace ckv
 
@@ -96,7 +97,7 @@ int ckv_get_device_error(uint32_t* code) {
           ckv::read_clear_err_attention_tc() |
           ckv::read_clear_err_elementwise() | ckv::read_clear_err_tp_reduce() |
           ckv::read_clear_err_gemv_fused() | ckv::read_clear_err_kv8() | ckv::read_clear_err_block_select() |
-          ckv::read_clear_err_attention_blocks();
+          ckv::read_clear_err_attention_blocks() | ckv::read_clear_err_attention_kv8();
   return CKV_OK;
 }
 
