@@ -23,6 +23,8 @@
 // Warps: 0..3 and 4..7 softmax / epilogue of Q tiles 0 and 1, 8..11 converters, 12 item
 // scheduler, 13 MMA issuer and TMEM owner, 14 and 15 idle.  The 512 threads start with 128
 // registers each; setmaxnreg moves them to the softmax warps (168 + 104 + 72: 65,536 in all).
+#include <type_traits>
+
 #include "ckv_common.cuh"
 
 CKV_DEFINE_ERR_WORD(attention_kv8)
@@ -57,7 +59,7 @@ struct Cfg {
   static constexpr uint32_t KV_TILE = BN * HD * 2;
   static constexpr uint32_t SMEM_NEED = 1024 + NQ * Q_BYTES + (KS + VS) * KV_TILE +
                                         kItemSlots * (sizeof(Item) + NQ * BM * 4) + kStageBytes +
-                                        kScaleSlots * GRP * 12 + 2 * NQ * BM * 4 + 64 + 40 * 8 + 16;
+                                        kScaleSlots * GRP * 12 + 64 + 40 * 8 + 16;
   // at least 120 KiB so two CTAs never share an SM: each allocates all 512 TMEM columns
   static constexpr uint32_t SMEM = SMEM_NEED > 120 * 1024 ? SMEM_NEED : 120 * 1024;
   static constexpr uint32_t IDESC_S = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(BM >> 4) << 24);  // fp16 operands
@@ -85,6 +87,21 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
+// two floats from shared memory, where the code says (a hoisted load would hold registers)
+__device__ __forceinline__ float2 lds2(const float* p) {
+  float2 r;
+  asm volatile("ld.volatile.shared.v2.f32 {%0,%1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(smem_u32(p)));
+  return r;
+}
+// 16 TMEM columns from registers; complete after tmem_st_wait
+__device__ __forceinline__ void tmem_st16_issue(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -92,6 +109,35 @@ __device__ __forceinline__ void regs_inc() {
 template <int N>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// The MMA warp stays converged and its operands warp-uniform, so that descriptors live in
+// uniform registers; `lead` (one lane) predicates the issue alone.  Issued from a one-lane
+// branch instead, each tcgen05.mma waited for its descriptors to be moved there.
+__device__ __forceinline__ uint32_t elect_lead() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p;
+}
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void commit_lead(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
 }
 __device__ __forceinline__ void conv_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
@@ -103,12 +149,13 @@ struct Args {
   uint16_t* out;
   float* part_o;
   float2* part_ml;
+  unsigned* sched;  // next slot, zero at launch (null: CTA c takes slots c, c + gridDim.x, ...)
   int M, Hq, Hk, n_ctx, n_blocks, tps, max_splits, blocks;
   float scale_log2;
 };
 
 // Item.pad0: last key that any of its rows sees (-1: none), pad1: Q tiles that hold rows.
-// CTA c takes slots c, c + gridDim.x, ... (longest first).
+// Slots as for Item, row blocks outermost within a group: longest first over all heads.
 template <int HD, bool E4M3>
 __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid_constant__ Args a) {
   using C = Cfg<HD>;
@@ -123,8 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   float* s_ks = reinterpret_cast<float*>(s_stage + kStageBytes / 4);              // [kScaleSlots][GRP] K scale
   float* s_lv = s_ks + kScaleSlots * GRP;                                         // log2(V scale / reference) + 7
   float* s_iv = s_lv + kScaleSlots * GRP;                                         // reference / V scale
-  float* s_qf = s_iv + kScaleSlots * GRP;                                         // [2][NQ * BM] row factors
-  float* s_ref = s_qf + 2 * NQ * BM;                                              // [4] V scale references, by item
+  float* s_ref = s_iv + kScaleSlots * GRP;                                        // [4] V scale references, by item
   float* s_red = s_ref + 4;                                                       // [4]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(s_red + 12);
   uint64_t* k_empty = k_full + KS;
@@ -134,15 +180,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   uint64_t* p_full = s_full + NQ;     // [NQ]
   uint64_t* o_done = p_full + NQ;     // [NQ]
   uint64_t* q_ready = o_done + NQ;    // [NQ]: Q tile w of the next item is in place
-  uint64_t* q_free = q_ready + NQ;    // [NQ]: the item's last S MMA of tile w is done
-  uint64_t* o_full = q_free + NQ;     // [NQ]: the item's last P V of tile w is done
+  uint64_t* o_full = q_ready + NQ;    // [NQ]: the item's last P V of tile w is done
   uint64_t* item_full = o_full + NQ;  // [kItemSlots]
   uint64_t* item_empty = item_full + kItemSlots;  // [kItemSlots]
   uint64_t* drain = item_empty + kItemSlots;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // from a shuffle, so that the compiler knows it for warp-uniform
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int G = a.Hq / a.Hk;
   const int T = BM / G;  // tokens per Q tile
   const int n_slots = a.blocks * a.Hk * a.max_splits;
@@ -161,7 +207,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
       mbar_init(&p_full[w], 128);
       mbar_init(&o_done[w], 1);
       mbar_init(&q_ready[w], 128);
-      mbar_init(&q_free[w], 1);
       mbar_init(&o_full[w], 1);
     }
     for (int s = 0; s < kItemSlots; ++s) {
@@ -193,11 +238,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         int pv[NQ * BM / 32];  // the item's token positions, lane + 32 j (clamped)
 #pragma unroll
         for (int j = 0; j < NQ * BM / 32; ++j) pv[j] = -1;
-        for (; cursor < n_slots; cursor += gridDim.x) {
-          const int gi = cursor / (a.Hk * a.blocks);  // slot group
-          const int rem = cursor - gi * (a.Hk * a.blocks);
-          const int hk = rem / a.blocks;
-          const int rb = a.blocks - 1 - (rem - hk * a.blocks);
+        while (true) {
+          int slot = cursor;
+          if (a.sched != nullptr) {
+            if (lane == 0) slot = int(atomicAdd(a.sched, 1u));
+            slot = __shfl_sync(0xffffffffu, slot, 0);
+          }
+          cursor += gridDim.x;
+          if (slot >= n_slots) break;
+          const int gi = slot / (a.Hk * a.blocks);  // slot group
+          const int rem = slot - gi * (a.Hk * a.blocks);
+          const int hk = rem % a.Hk;
+          const int rb = a.blocks - 1 - rem / a.Hk;
           const int t0 = rb * NQ * T;
           const int n_tok = min(NQ * T, a.M - t0);
           int mx = -1;
@@ -225,7 +277,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
             break;
           }
         }
-        cursor += gridDim.x;
         const int s = it % kItemSlots;
         bool free_slot = true;
         if (lane == 0) free_slot = mbar_wait(&item_empty[s], ((it / kItemSlots) & 1) ^ 1, abort, &g_err_word);
@@ -241,83 +292,90 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         if (rec.rb < 0) break;
         ++it;
       }
-    } else if (warp == kWarpMma && lane == 0) {
+    } else if (warp == kWarpMma) {
       // ---------------------------------------------------------------- MMA issuer
-      auto issue_s = [&](int w, int gt, bool last) {
+      const uint32_t lead = elect_lead();
+      auto issue_s = [&](int w, int gt) {
         const uint32_t q0 = smem_u32(sQ + w * C::Q_BYTES);
         const uint32_t k0 = smem_u32(sK + (gt % KS) * C::KV_TILE);
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk) {
           const uint32_t off = (kk >> 2) * ATOM_BYTES + (kk & 3) * 32;
-          tc_mma_f16(tmem + w * BN, umma_desc_sw128(q0 + off), umma_desc_sw128(k0 + off), C::IDESC_S, kk > 0 ? 1u : 0u);
+          mma_ss(lead, tmem + w * BN, umma_desc_sw128(q0 + off), umma_desc_sw128(k0 + off), C::IDESC_S, kk > 0 ? 1u : 0u);
         }
-        tc_commit(&s_full[w]);
-        if (last) tc_commit(&q_free[w]);  // Q tile w may be overwritten for the next item
+        commit_lead(lead, &s_full[w]);
       };
       auto issue_pv = [&](int w, int gt, bool first) {
         const uint32_t v0 = smem_u32(sV + (gt % VS) * C::KV_TILE);
         const uint32_t pbuf = tmem + w * BN;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          tc_mma_f16_ts(tmem + O_COL + w * 128, pbuf + kk * 8, umma_desc_sw128_mn(v0 + kk * 16 * 128, ATOM_BYTES), C::IDESC_PV,
+          mma_ts(lead, tmem + O_COL + w * 128, pbuf + kk * 8, umma_desc_sw128_mn(v0 + kk * 16 * 128, ATOM_BYTES), C::IDESC_PV,
                         (!first || kk > 0) ? 1u : 0u);
-        tc_commit(&o_done[w]);
+        commit_lead(lead, &o_done[w]);
       };
+      // Per Q tile (w = 0, 1) the parities of its key tiles and items so far, tile 1 in the high
+      // half of each word.  The loops over w stay rolled: unrolled, their descriptors
+      // do not fit this warpgroup's registers.
       bool ok = true;
-      int g = 0;                  // key tiles consumed (all items)
-      int gw[NQ] = {}, qw[NQ] = {};  // per Q tile: key tiles and items
+      int g = 0;  // key tiles consumed (all items)
+      uint32_t tiles_w = 0, items_w = 0;
       for (int it = 0; ok; ++it) {
         const int s = it % kItemSlots;
-        if (!mbar_wait(&item_full[s], (it / kItemSlots) & 1, abort, &g_err_word)) {
+        if (!warp_wait(&item_full[s], (it / kItemSlots) & 1, abort)) {
           ok = false;
           break;
         }
-        const int n_kt = items[s].rb < 0 ? -1 : items[s].n_kt, nq = items[s].pad1;
-        mbar_arrive(&item_empty[s]);
+        const int n_kt = __shfl_sync(0xffffffffu, items[s].rb < 0 ? -1 : items[s].n_kt, 0);
+        const int nq = __shfl_sync(0xffffffffu, items[s].pad1, 0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[s]);
         if (n_kt < 0) break;
-        if (!mbar_wait(&k_full[g % KS], (g / KS) & 1, abort, &g_err_word)) {
+        if (!warp_wait(&k_full[g % KS], (g / KS) & 1, abort)) {
           ok = false;
           break;
         }
-        for (int w = 0; w < nq && ok; ++w) {
-          if (!mbar_wait(&q_ready[w], qw[w] & 1, abort, &g_err_word)) {
+#pragma unroll 1
+        for (int w = 0; w < nq; ++w) {
+          if (!warp_wait(&q_ready[w], (items_w >> (16 * w)) & 1, abort)) {
             ok = false;
             break;
           }
-          ++qw[w];
           tc_fence_after();
-          issue_s(w, g, n_kt == 1);
+          issue_s(w, g);
         }
         if (!ok) break;
-        tc_commit(&k_empty[g % KS]);
-        for (int j = 0; j < n_kt && ok; ++j) {
+        commit_lead(lead, &k_empty[g % KS]);
+#pragma unroll 1
+        for (int jw = 0; jw < n_kt * nq; ++jw) {
+          const int j = nq == 2 ? jw >> 1 : jw, w = nq == 2 ? jw & 1 : 0;
           const int gt = g + j, nxt = gt + 1;
-          for (int w = 0; w < nq && ok; ++w) {
-            if (!mbar_wait(&p_full[w], (gw[w] + j) & 1, abort, &g_err_word) ||
-                (w == 0 && !mbar_wait(&v_full[gt % VS], (gt / VS) & 1, abort, &g_err_word))) {
+          if (!warp_wait(&p_full[w], ((tiles_w >> (16 * w)) + j) & 1, abort) ||
+              (w == 0 && !warp_wait(&v_full[gt % VS], (gt / VS) & 1, abort))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          issue_pv(w, gt, j == 0);
+          if (j + 1 == n_kt) commit_lead(lead, &o_full[w]);  // O of tile w is final
+          if (w == nq - 1) commit_lead(lead, &v_empty[gt % VS]);
+          if (j + 1 < n_kt) {
+            if (w == 0 && !warp_wait(&k_full[nxt % KS], (nxt / KS) & 1, abort)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            issue_pv(w, gt, j == 0);
-            if (j + 1 == n_kt) tc_commit(&o_full[w]);  // O of tile w is final
-            if (w == nq - 1) tc_commit(&v_empty[gt % VS]);
-            if (j + 1 < n_kt) {
-              if (w == 0 && !mbar_wait(&k_full[nxt % KS], (nxt / KS) & 1, abort, &g_err_word)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              issue_s(w, nxt, j + 2 == n_kt);
-              if (w == nq - 1) tc_commit(&k_empty[nxt % KS]);
-            }
+            issue_s(w, nxt);
+            if (w == nq - 1) commit_lead(lead, &k_empty[nxt % KS]);
           }
         }
         g += n_kt;
-        for (int w = 0; w < nq; ++w) gw[w] += n_kt;
+        const uint32_t both = nq == 2 ? 0x00010001u : 0x00000001u;
+        if (n_kt & 1) tiles_w ^= both;
+        items_w ^= both;
       }
       if (!ok) {
-        tc_commit(drain);
+        commit_lead(lead, drain);
         drain_wait(drain, 0);
       }
     }
@@ -325,38 +383,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
     // ------------------------------------------------------------------- converters
     regs_dec<kRegsConv>();
     const int t = threadIdx.x - kWarpConv * 32;  // 0 .. 127
-    constexpr int CPR = HD / 16;                 // 16-code chunks per row
-    constexpr int NCH = BN * CPR / 128;          // chunks per thread and tile (8 or 4)
-    constexpr int RSTEP = 128 / CPR;             // rows per pass
-    const int cr = t / CPR, cc = t % CPR;        // row of the first pass, chunk
-    // operand tile address of chunk cc of row r: 64-column atom cc / 4, 16-byte units
-    // 2 (cc % 4) and + 1, swizzled by r % 8 (r % 8 is the same in every pass)
-    const uint32_t sw = uint32_t(cr & 7);
-    const uint32_t u0 = ((2u * (cc & 3)) ^ sw) * 16u, u1 = ((2u * (cc & 3) + 1u) ^ sw) * 16u;
-    const uint32_t base = uint32_t(cc >> 2) * ATOM_BYTES + uint32_t(cr) * 128u;
-    const bool odd = (cc & 4) != 0;  // the two atoms' lanes write their halves in opposite order: distinct banks
-    const uint32_t first_u = odd ? u1 : u0, second_u = odd ? u0 : u1;
+    constexpr int ATOMS = HD / 64;               // 64-column atoms of an operand tile
+    constexpr int NCH = BN / 32 * ATOMS;         // 16-code chunks per thread and tile
+    // chunk c4 of a 64-column atom in row r0 + 32 i: four lanes read 64 bytes of a row.  The
+    // widened chunk is the 16-byte units 2 c4 and 2 c4 + 1 of the row, swizzled by row % 8:
+    // the two rows of eight lanes differ in that bit, so a store's lanes hit distinct banks.
+    const int r0 = t >> 2, c4 = t & 3;
+    const uint32_t u0 = ((2u * c4) ^ (r0 & 7)) * 16u, u1 = u0 ^ 16u;
     auto load = [&](const uint8_t* src, int hk, int kt, int last, uint4(&x)[NCH]) {
-      const int64_t row0 = int64_t(hk) * a.n_blocks * kBlk + int64_t(kt) * BN;
+      const uint8_t* p = src + (int64_t(hk) * a.n_blocks * kBlk + int64_t(kt) * BN + r0) * HD + c4 * 16;
+      const int vis = last - kt * BN - r0;  // rows past it stay zero
 #pragma unroll
-      for (int i = 0; i < NCH; ++i) {
-        const int r = i * RSTEP + cr;
-        x[i] = kt * BN + r <= last ? __ldg(reinterpret_cast<const uint4*>(src + (row0 + r) * HD) + cc) : make_uint4(0u, 0u, 0u, 0u);
-      }
+      for (int i = 0; i < NCH; ++i)
+        x[i] = (i / ATOMS) * 32 <= vis ? __ldg(reinterpret_cast<const uint4*>(p + (i / ATOMS) * 32 * HD + (i % ATOMS) * 64))
+                                       : make_uint4(0u, 0u, 0u, 0u);
     };
     auto store = [&](uint8_t* tile, const uint4(&x)[NCH]) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i) {
         const uint2 p0 = widen4<E4M3>(x[i].x), p1 = widen4<E4M3>(x[i].y), p2 = widen4<E4M3>(x[i].z), p3 = widen4<E4M3>(x[i].w);
-        const uint4 lo = make_uint4(p0.x, p0.y, p1.x, p1.y), hi = make_uint4(p2.x, p2.y, p3.x, p3.y);
-        uint8_t* row = tile + base + i * RSTEP * 128;
-        *reinterpret_cast<uint4*>(row + first_u) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(row + second_u) = odd ? lo : hi;
+        uint8_t* row = tile + (i % ATOMS) * ATOM_BYTES + (r0 + (i / ATOMS) * 32) * 128;
+        *reinterpret_cast<uint4*>(row + u0) = make_uint4(p0.x, p0.y, p1.x, p1.y);
+        *reinterpret_cast<uint4*>(row + u1) = make_uint4(p2.x, p2.y, p3.x, p3.y);
       }
     };
     bool ok = true;
-    int g = 0;         // key tiles converted (all items)
-    int qn[NQ] = {};   // Q tiles converted
+    int g = 0;  // key tiles converted (all items)
     for (int it = 0; ok; ++it) {
       const int s = it % kItemSlots;
       if (!warp_wait(&item_full[s], (it / kItemSlots) & 1, abort)) break;
@@ -411,53 +463,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         store(sV + (gt % VS) * C::KV_TILE, y);
         fence_async_smem();
         mbar_arrive(&v_full[gt % VS]);
-        if (j == 0) {
-          // the item's Q tiles, once the item before has no S MMA left on them
-          constexpr int QPR = HD / 8;          // lanes per row
-          constexpr int QSTEP = 128 / QPR;     // rows per pass
-          constexpr int QB = 4;                // passes whose loads are in flight together
-          const int qr = t / QPR, qc = t % QPR;
-          const int n_tok = min(NQ * T, a.M - rec.rb * NQ * T);
-          for (int w = 0; w < rec.pad1 && ok; ++w) {
-            if (qn[w] > 0 && !warp_wait(&q_free[w], (qn[w] - 1) & 1, abort)) {
-              ok = false;
-              break;
-            }
-            ++qn[w];
-#pragma unroll 1
-            for (int p0 = 0; p0 < BM / QSTEP; p0 += QB) {
-              uint4 z[QB];
-#pragma unroll
-              for (int i = 0; i < QB; ++i) {
-                const int r = (p0 + i) * QSTEP + qr;
-                const int tr = r / G, tok = w * T + tr;
-                z[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (r < T * G && tok < n_tok)
-                  z[i] = __ldg(reinterpret_cast<const uint4*>(
-                                   a.q + (int64_t(rec.rb * NQ * T + tok) * a.Hq + rec.hk * G + (r - tr * G)) * HD) + qc);
-              }
-#pragma unroll
-              for (int i = 0; i < QB; ++i) {
-                const int r = (p0 + i) * QSTEP + qr;
-                // the power of two that puts the row's largest value in [2^14, 2^15)
-                const uint32_t mg = __vmaxu2(__vmaxu2(z[i].x & 0x7fff7fffu, z[i].y & 0x7fff7fffu),
-                                             __vmaxu2(z[i].z & 0x7fff7fffu, z[i].w & 0x7fff7fffu));
-                uint32_t am = max(mg & 0xffffu, mg >> 16);
-#pragma unroll
-                for (int o = 1; o < QPR; o <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
-                const int sh = am == 0 ? 0 : max(-126, min(126, 14 + 127 - int(am >> 7)));
-                const float up = __uint_as_float(uint32_t(sh + 127) << 23);
-                if (qc == 0) s_qf[((it & 1) * NQ + w) * BM + r] = a.scale_log2 * __uint_as_float(uint32_t(127 - sh) << 23);
-                const uint4 h = make_uint4(pack_h2(lo_bf(z[i].x) * up, hi_bf(z[i].x) * up), pack_h2(lo_bf(z[i].y) * up, hi_bf(z[i].y) * up),
-                                           pack_h2(lo_bf(z[i].z) * up, hi_bf(z[i].z) * up), pack_h2(lo_bf(z[i].w) * up, hi_bf(z[i].w) * up));
-                *reinterpret_cast<uint4*>(sQ + w * C::Q_BYTES + (qc >> 3) * ATOM_BYTES + r * 128 + (((qc & 7) ^ (r & 7)) << 4)) = h;
-              }
-            }
-            fence_async_smem();
-            mbar_arrive(&q_ready[w]);
-          }
-          if (!ok) break;
-        }
       }
       g += rec.n_kt;
     }
@@ -472,66 +477,94 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
     const uint32_t sbuf = lane_base + w * BN;
     const uint32_t obuf = lane_base + O_COL + w * 128;
 
-    bool ok = true;
+    // this thread's row of an item: whether it is real, and the last key it sees (padding rows
+    // see every key: they never force the masked path on their warp)
+    struct Row {
+      bool valid;
+      int pos;
+    };
+    auto take = [&](int it, Item& rec, Row& x) -> bool {
+      const int s = it % kItemSlots;
+      if (!warp_wait(&item_full[s], (it / kItemSlots) & 1, abort)) return false;
+      rec = items[s];
+      const int tt = w * T + tr;  // token index in the item
+      x.valid = rec.rb >= 0 && r < T * G && tt < min(NQ * T, a.M - rec.rb * NQ * T);
+      x.pos = x.valid ? s_pos[s * NQ * BM + tt] : a.n_ctx - 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[s]);
+      return true;
+    };
+    // This thread's row of Q tile w as fp16 times the power of two that puts its largest value
+    // in [2^14, 2^15): exact down to 2^-38 of it.  Returns what undoes it in a score (log2
+    // domain).  The tile is free: the last S MMA that read it has been waited for.
+    auto place_q = [&](const Item& rec, const Row& x) -> float {
+      uint4 z[HD / 8];
+      const uint4* src = reinterpret_cast<const uint4*>(
+          a.q + (int64_t(rec.rb * NQ * T + w * T + tr) * a.Hq + rec.hk * G + (r - tr * G)) * HD);
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) z[i] = x.valid ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+      uint32_t mg = 0;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+        mg = __vmaxu2(mg, __vmaxu2(__vmaxu2(z[i].x & 0x7fff7fffu, z[i].y & 0x7fff7fffu),
+                                   __vmaxu2(z[i].z & 0x7fff7fffu, z[i].w & 0x7fff7fffu)));
+      const uint32_t am = max(mg & 0xffffu, mg >> 16);
+      const int sh = am == 0 ? 0 : max(-126, min(126, 14 + 127 - int(am >> 7)));
+      const float up = __uint_as_float(uint32_t(sh + 127) << 23);
+      uint8_t* row = sQ + w * C::Q_BYTES + r * 128;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+        *reinterpret_cast<uint4*>(row + (i >> 3) * ATOM_BYTES + (((i & 7) ^ (r & 7)) << 4)) =
+            make_uint4(pack_h2(lo_bf(z[i].x) * up, hi_bf(z[i].x) * up), pack_h2(lo_bf(z[i].y) * up, hi_bf(z[i].y) * up),
+                       pack_h2(lo_bf(z[i].z) * up, hi_bf(z[i].z) * up), pack_h2(lo_bf(z[i].w) * up, hi_bf(z[i].w) * up));
+      fence_async_smem();
+      mbar_arrive(&q_ready[w]);
+      return a.scale_log2 * __uint_as_float(uint32_t(127 - sh) << 23);
+    };
+
     int g = 0;   // key tiles seen (all items): the scale slots
     int gw = 0;  // of them, by this Q tile
     int iw = 0;  // items by this Q tile
-    for (int it = 0; ok; ++it) {
-      const int s = it % kItemSlots;
-      if (!warp_wait(&item_full[s], (it / kItemSlots) & 1, abort)) {
-        ok = false;
-        break;
-      }
-      const Item cur = items[s];
-      const int n_tok = min(NQ * T, a.M - cur.rb * NQ * T);
-      const int tt = w * T + tr;  // token index in the item
-      const bool valid = cur.rb >= 0 && r < T * G && tt < n_tok;
-      // padding rows see every key: they never force the masked path on their warp
-      const int pos = valid ? s_pos[s * NQ * BM + tt] : a.n_ctx - 1;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&item_empty[s]);
-      if (cur.rb < 0) break;
-      if (w >= cur.pad1) {  // no rows on this tile
-        g += cur.n_kt;
-        continue;
-      }
-      float m = -INFINITY, l = 0.f, factor = 0.f, ref = 1.0f;
-      for (int j = 0; j < cur.n_kt; ++j) {
+    Item cur;
+    Row row{false, 0};
+    bool ok = take(0, cur, row);
+    float factor = 0.f;
+    if (ok && cur.rb >= 0 && w < cur.pad1) factor = place_q(cur, row);
+    for (int it = 0; ok && cur.rb >= 0; ++it) {
+      float m = -INFINITY, l = 0.f, ref = 1.0f;
+      const bool mine = w < cur.pad1;  // the item has rows on this tile
+      for (int j = 0; mine && j < cur.n_kt; ++j) {
         const int gt = g + j;
         if (!warp_wait(&s_full[w], (gw + j) & 1, abort)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        if (j == 0) {
-          factor = s_qf[((it & 1) * NQ + w) * BM + r];
-          ref = s_ref[it & 3];
-        }
-        const int lim = pos - (cur.kt0 + j) * BN;  // keys at index > lim are masked
+        if (j == 0) ref = s_ref[it & 3];
+        const int lim = row.pos - (cur.kt0 + j) * BN;  // keys at index > lim are masked
         const bool full = __all_sync(0xffffffffu, lim >= BN - 1);
         const float* ksl = s_ks + (gt % kScaleSlots) * GRP;
         const float* lvl = s_lv + (gt % kScaleSlots) * GRP;
         const float* ivl = s_iv + (gt % kScaleSlots) * GRP;
-        float c8[GRP];
-#pragma unroll
-        for (int b = 0; b < GRP; b += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(ksl + b);
-          c8[b] = x.x * factor, c8[b + 1] = x.y * factor, c8[b + 2] = x.z * factor, c8[b + 3] = x.w * factor;
-        }
-        // pass 1: row max; a 16-column group's raw maximum times its factor (>= 0)
+        // pass 1: row max; a 16-column group's raw maximum times its factor (>= 0).  S comes 32
+        // columns at a time, the next 32 on their way while these are worked on (both passes).
         float mx = -INFINITY;
+        uint32_t u[2][32];
+        tmem_ld32_issue(sbuf, u[0]);
 #pragma unroll
-        for (int h = 0; h < BN / 64; ++h) {
-          uint32_t u[64];
-          tmem_ld64w(sbuf + 64 * h, u);
+        for (int h = 0; h < BN / 32; ++h) {
+          tmem_ld_wait(u[h & 1]);
+          if (h + 1 < BN / 32) tmem_ld32_issue(sbuf + 32 * (h + 1), u[(h + 1) & 1]);
+          uint32_t(&v)[32] = u[h & 1];
           if (!full) {
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-              if (64 * h + e > lim) u[e] = __float_as_uint(-INFINITY);
+            for (int e = 0; e < 32; ++e)
+              if (32 * h + e > lim) v[e] = __float_as_uint(-INFINITY);
           }
+          const float2 kq = lds2(ksl + 2 * h);
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const uint32_t* x = u + 16 * b;
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t* x = v + 16 * b;
             float p = max3f(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
             float q2 = max3f(__uint_as_float(x[3]), __uint_as_float(x[4]), __uint_as_float(x[5]));
 #pragma unroll
@@ -540,9 +573,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
               q2 = max3f(q2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
             }
             p = max3f(p, __uint_as_float(x[14]), __uint_as_float(x[15]));
-            mx = fmaxf(mx, fmaxf(p, q2) * c8[4 * h + b]);  // -inf * 0 is NaN, which fmaxf drops
+            mx = fmaxf(mx, fmaxf(p, q2) * ((b ? kq.y : kq.x) * factor));  // -inf * 0 is NaN, which fmaxf drops
           }
         }
+        tmem_ld32_issue(sbuf, u[0]);  // pass 2's first columns, on their way during the rescale's test
         const float m_new = fmaxf(m, mx);
         const bool need = j > 0 && m_new > m + kRescaleThreshold;
         if (__any_sync(0xffffffffu, need)) {
@@ -553,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
           }
           tc_fence_after();
           const float corr = need ? ex2_approx(m - m_new) : 1.0f;
+          tmem_ld_wait(u[0]);
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             float o[32];
@@ -568,42 +603,61 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         // over S as fp16 pairs; masked keys give exactly 0.  A row that has seen no key yet
         // keeps m = -inf and takes 0 as its base.
         const float neg_m = m == -INFINITY ? 0.f : -m;
+        auto pass2 = [&](auto all_visible) {
+          constexpr bool kAll = decltype(all_visible)::value;
 #pragma unroll
-        for (int h = 0; h < BN / 64; ++h) {
-          uint32_t u[64];
-          tmem_ld64w(sbuf + 64 * h, u);
-          const float4 lv = *reinterpret_cast<const float4*>(lvl + 4 * h);
-          const float4 iv = *reinterpret_cast<const float4*>(ivl + 4 * h);
-          const float lv4[4] = {lv.x, lv.y, lv.z, lv.w}, iv4[4] = {iv.x, iv.y, iv.z, iv.w};
+          for (int h = 0; h < BN / 32; ++h) {
+            tmem_ld_wait(u[h & 1]);
+            if (h + 1 < BN / 32) tmem_ld32_issue(sbuf + 32 * (h + 1), u[(h + 1) & 1]);
+            uint32_t(&v)[32] = u[h & 1];
+            const float2 kq = lds2(ksl + 2 * h), lv = lds2(lvl + 2 * h), iv = lds2(ivl + 2 * h);
+            uint32_t out16[16];
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const float2 sc2 = make_float2(c8[4 * h + b], c8[4 * h + b]);
-            const float add = neg_m + lv4[b];
-            const float2 nm2 = make_float2(add, add);
-            float2 rs0 = make_float2(0.f, 0.f), rs1 = rs0;
+            for (int b = 0; b < 2; ++b) {
+              const float cb = (b ? kq.y : kq.x) * factor, add = neg_m + (b ? lv.y : lv.x);
+              const float2 sc2 = make_float2(cb, cb), nm2 = make_float2(add, add);
+              float2 rs0 = make_float2(0.f, 0.f), rs1 = rs0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int pr = 8 * b + e;
-              const float2 x = __ffma2_rn(make_float2(__uint_as_float(u[2 * pr]), __uint_as_float(u[2 * pr + 1])), sc2, nm2);
-              float2 pv = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-              if (!full) {
-                pv.x = 64 * h + 2 * pr <= lim ? pv.x : 0.f;
-                pv.y = 64 * h + 2 * pr + 1 <= lim ? pv.y : 0.f;
+              for (int e = 0; e < 8; ++e) {
+                const int pr = 8 * b + e;
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[2 * pr]), __uint_as_float(v[2 * pr + 1])), sc2, nm2);
+                float2 pv = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                if constexpr (!kAll) {
+                  pv.x = 32 * h + 2 * pr <= lim ? pv.x : 0.f;
+                  pv.y = 32 * h + 2 * pr + 1 <= lim ? pv.y : 0.f;
+                }
+                if (e & 1) rs1 = __fadd2_rn(rs1, pv);
+                else rs0 = __fadd2_rn(rs0, pv);
+                out16[pr] = pack_h2(pv.x, pv.y);
               }
-              if (e & 1) rs1 = __fadd2_rn(rs1, pv);
-              else rs0 = __fadd2_rn(rs0, pv);
-              u[pr] = pack_h2(pv.x, pv.y);
+              const float2 rs = __fadd2_rn(rs0, rs1);
+              l = fmaf(rs.x + rs.y, b ? iv.y : iv.x, l);
             }
-            const float2 rs = __fadd2_rn(rs0, rs1);
-            l = fmaf(rs.x + rs.y, iv4[b], l);
+            // P of keys 32 h .. goes to columns 16 h .., whose scores were read before
+            tmem_st16_issue(sbuf + 16 * h, out16);
           }
-          tmem_st32u(sbuf + 32 * h, *reinterpret_cast<const uint32_t(*)[32]>(u));
-        }
+        };
+        if (full) pass2(std::true_type{});
+        else pass2(std::false_type{});
+        tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&p_full[w]);
       }
       if (!ok) break;
       g += cur.n_kt;
+      // the next item's Q tile, under this item's last P V
+      Item nxt;
+      Row nrow{false, 0};
+      if (!take(it + 1, nxt, nrow)) {
+        ok = false;
+        break;
+      }
+      float nfactor = 0.f;
+      if (nxt.rb >= 0 && w < nxt.pad1) nfactor = place_q(nxt, nrow);
+      if (!mine) {
+        cur = nxt, row = nrow, factor = nfactor;
+        continue;
+      }
       gw += cur.n_kt;
       if (!warp_wait(&o_full[w], iw & 1, abort)) {
         ok = false;
@@ -644,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         }
         if (lane == 0) bulk_wait_read<0>();  // both buffers free for the next epilogue
         __syncwarp();
-        if (valid) {
+        if (row.valid) {
           const int64_t prow = int64_t((cur.rb * a.Hk + cur.hk) * a.max_splits + cur.split) * (NQ * BM) + w * BM + r;
           a.part_ml[prow] = make_float2(m, l);
         }
@@ -654,6 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         int64_t dst[4];
         {
           const int t0 = cur.rb * NQ * T;
+          const int n_tok = min(NQ * T, a.M - t0);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int rq = sub * 32 + 8 * k + (lane >> 2);
@@ -684,6 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
       // O has been read: the next item's first P V (which overwrites it) is issued only
       // after this warpgroup's next p_full
       tc_fence_before();
+      cur = nxt, row = nrow, factor = nfactor;
     }
     // the split partials' bulk stores have written global memory before the CTA ends
     if (lane == 0) bulk_wait_all();
@@ -719,13 +775,20 @@ int launch_tiles(Args a, const SplitPlan& p, void* workspace, cudaStream_t strea
     return CKV_ERR_CUDA;
   }
   if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), Cfg<HD>::SMEM)) return rc;
+  const int64_t n_slots = int64_t(p.blocks) * a.Hk * p.max_splits;
+  CKV_REQUIRE(n_slots < (int64_t(1) << 31) - 4 * 1024 * 1024, "ckv_attention_kv8: too many work items");
+  if (n_slots > num_sms()) {  // more than one item per CTA: they take them from a counter
+    a.sched = static_cast<unsigned*>(workspace);
+    if (cudaMemsetAsync(a.sched, 0, sizeof(unsigned), stream) != cudaSuccess) {
+      set_error("ckv_attention_kv8: cudaMemsetAsync: %s", cudaGetErrorString(cudaGetLastError()));
+      return CKV_ERR_CUDA;
+    }
+  }
   if (p.max_splits > 1) {
-    a.part_o = static_cast<float*>(workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kSchedBytes);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(p.blocks) * a.Hk * p.max_splits * NQ * BM * HD);
   }
   a.tps = p.tps, a.max_splits = p.max_splits, a.blocks = p.blocks;
-  const int64_t n_slots = int64_t(p.blocks) * a.Hk * p.max_splits;
-  CKV_REQUIRE(n_slots < (int64_t(1) << 31) - 4 * 1024 * 1024, "ckv_attention_kv8: too many work items");
   launch_pdl(kern, dim3(int(std::min<int64_t>(n_slots, num_sms()))), dim3(kThreads), Cfg<HD>::SMEM, stream, a);
   CKV_LAUNCH_CHECK("ckv_attention_kv8");
   if (p.max_splits > 1) {
@@ -749,7 +812,7 @@ using namespace ckv;
 
 extern "C" int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
-  return use_tiles(m, n_q_heads, n_kv_heads) ? plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
+  return use_tiles(m, n_q_heads, n_kv_heads) ? kSchedBytes + plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
                                              : kv8_stream_workspace(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
@@ -783,7 +846,7 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
   if (!use_tiles(m, n_q_heads, n_kv_heads))
     return kv8_stream_attention(q, k8, v8, k_scale, v_scale, positions, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, scale, type,
                                 workspace, as_stream(stream));
-  const Args a{q, k8, v8, k_scale, v_scale, positions, out, nullptr, nullptr, m, n_q_heads, n_kv_heads, n_ctx,
+  const Args a{q, k8, v8, k_scale, v_scale, positions, out, nullptr, nullptr, nullptr, m, n_q_heads, n_kv_heads, n_ctx,
                ceil_div(n_ctx, kBlk), 0, 0, 0, scale * 1.4426950408889634f};
   const SplitPlan p = plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
   const cudaStream_t s = as_stream(stream);
