@@ -111,8 +111,9 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 // The MMA warp stays converged and its operands warp-uniform, so that descriptors live in
-// uniform registers; `lead` (one lane) predicates the issue alone.  Issued from a one-lane
-// branch instead, each tcgen05.mma waited for its descriptors to be moved there.
+// uniform registers (values that vary come from warp reductions); `lead` (one lane)
+// predicates the issue alone.  Issued from a one-lane branch, each tcgen05.mma waited for its
+// operands to be moved there: a 5248-token prompt took 441 us instead of 374.
 __device__ __forceinline__ uint32_t elect_lead() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
@@ -178,7 +179,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   uint64_t* v_empty = v_full + VS;
   uint64_t* s_full = v_empty + VS;    // [NQ]
   uint64_t* p_full = s_full + NQ;     // [NQ]
-  uint64_t* o_done = p_full + NQ;     // [NQ]
+  uint64_t* p_half = p_full + NQ;     // [NQ]: the first 64 keys' P is in place
+  uint64_t* o_done = p_half + NQ;     // [NQ]
   uint64_t* q_ready = o_done + NQ;    // [NQ]: Q tile w of the next item is in place
   uint64_t* o_full = q_ready + NQ;    // [NQ]: the item's last P V of tile w is done
   uint64_t* item_full = o_full + NQ;  // [kItemSlots]
@@ -187,8 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  // from a shuffle, so that the compiler knows it for warp-uniform
-  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  // from a warp reduction, so that the compiler knows it for warp-uniform
+  const int warp = int(__reduce_max_sync(0xffffffffu, threadIdx.x >> 5)), lane = threadIdx.x & 31;
   const int G = a.Hq / a.Hk;
   const int T = BM / G;  // tokens per Q tile
   const int n_slots = a.blocks * a.Hk * a.max_splits;
@@ -205,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
     for (int w = 0; w < NQ; ++w) {
       mbar_init(&s_full[w], 1);
       mbar_init(&p_full[w], 128);
+      mbar_init(&p_half[w], 128);
       mbar_init(&o_done[w], 1);
       mbar_init(&q_ready[w], 128);
       mbar_init(&o_full[w], 1);
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __reduce_max_sync(0xffffffffu, *tmem_slot);
   // set-up done; q, the cache, the positions and the workspace belong to the kernels
   // before (dependent launch)
   pdl_wait();
@@ -305,14 +308,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         }
         commit_lead(lead, &s_full[w]);
       };
-      auto issue_pv = [&](int w, int gt, bool first) {
-        const uint32_t v0 = smem_u32(sV + (gt % VS) * C::KV_TILE);
-        const uint32_t pbuf = tmem + w * BN;
+      // half of P_w V (64 keys): P arrives in two halves, so the first runs under the
+      // exponentials of the second
+      auto issue_pv = [&](int w, int gt, int half, bool first) {
+        const uint32_t v0 = smem_u32(sV + (gt % VS) * C::KV_TILE) + half * (BN / 2 * 128);
+        const uint32_t pbuf = tmem + w * BN + half * (BN / 4);
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
+        for (int kk = 0; kk < BN / 32; ++kk)
           mma_ts(lead, tmem + O_COL + w * 128, pbuf + kk * 8, umma_desc_sw128_mn(v0 + kk * 16 * 128, ATOM_BYTES), C::IDESC_PV,
-                        (!first || kk > 0) ? 1u : 0u);
-        commit_lead(lead, &o_done[w]);
+                 (!first || kk > 0) ? 1u : 0u);
       };
       // Per Q tile (w = 0, 1) the parities of its key tiles and items so far, tile 1 in the high
       // half of each word.  The loops over w stay rolled: unrolled, their descriptors
@@ -326,8 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
           ok = false;
           break;
         }
-        const int n_kt = __shfl_sync(0xffffffffu, items[s].rb < 0 ? -1 : items[s].n_kt, 0);
-        const int nq = __shfl_sync(0xffffffffu, items[s].pad1, 0);
+        const int n_kt = __reduce_max_sync(0xffffffffu, items[s].rb < 0 ? -1 : items[s].n_kt);
+        const int nq = __reduce_max_sync(0xffffffffu, items[s].pad1);
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_empty[s]);
         if (n_kt < 0) break;
@@ -350,13 +354,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         for (int jw = 0; jw < n_kt * nq; ++jw) {
           const int j = nq == 2 ? jw >> 1 : jw, w = nq == 2 ? jw & 1 : 0;
           const int gt = g + j, nxt = gt + 1;
-          if (!warp_wait(&p_full[w], ((tiles_w >> (16 * w)) + j) & 1, abort) ||
+          if (!warp_wait(&p_half[w], ((tiles_w >> (16 * w)) + j) & 1, abort) ||
               (w == 0 && !warp_wait(&v_full[gt % VS], (gt / VS) & 1, abort))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          issue_pv(w, gt, j == 0);
+          issue_pv(w, gt, 0, j == 0);
+          if (!warp_wait(&p_full[w], ((tiles_w >> (16 * w)) + j) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          issue_pv(w, gt, 1, false);
+          commit_lead(lead, &o_done[w]);
           if (j + 1 == n_kt) commit_lead(lead, &o_full[w]);  // O of tile w is final
           if (w == nq - 1) commit_lead(lead, &v_empty[gt % VS]);
           if (j + 1 < n_kt) {
@@ -635,6 +646,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
             }
             // P of keys 32 h .. goes to columns 16 h .., whose scores were read before
             tmem_st16_issue(sbuf + 16 * h, out16);
+            if (h == 1) {
+              tmem_st_wait();
+              tc_fence_before();
+              mbar_arrive(&p_half[w]);
+            }
           }
         };
         if (full) pass2(std::true_type{});
