@@ -75,8 +75,8 @@ SIGNATURES: dict[str, list] = {
     "ckv_block_select_workspace_size": [_i32, _i32, _i32, _i32, _i32],
     "ckv_block_select_launches": [_i32, _i32, _i32, _i32, _i32],
     "ckv_block_select": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p],
-    "ckv_attention_blocks_workspace_size": [_i32, _i32, _i32, _i32, _i32],
-    "ckv_attention_blocks_launches": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_blocks_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_blocks_launches": [_i32, _i32, _i32, _i32, _i32, _i32],
     "ckv_attention_blocks": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _p],
     "ckv_attention_blocks_kv8": [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p,
                                  _i64, _p],

@@ -4,18 +4,19 @@
 //
 // Such calls read every key for at most 16 query rows, so they are bound by the cache's
 // bytes; a 128-row tcgen05 tile would be nearly empty.  The kernel keeps the bytes moving:
-// a warp takes whole blocks, loads the next block's K and V into registers (4 KiB per warp
-// at head_dim 128 in 8 bits) while it works on the current one, and uses mma.sync
-// m16n8k16 with the roles turned round: the 16 keys of a block are the M rows, the up to 8
-// query rows the N columns, so nothing is padded for groups of up to 8 heads.
+// a warp takes whole blocks (contiguous, 2 KiB of K and of V at head_dim 128 in 8 bits)
+// through a ring of TMA bulk copies in shared memory and uses mma.sync m16n8k16 with the
+// roles turned round: the 16 keys of a block are the M rows, the up to 8 query rows the N
+// columns, so nothing is padded for groups of up to 8 heads.
 //   S^T [16 keys x 8 rows]  = K Q^T        A = K, contraction over head_dim
 //   O^T [dims x 8 rows]    += V^T P^T      A = V^T, contraction over the 16 keys
 // The contraction over head_dim may be permuted if K and Q agree, so quad member c of a
-// lane group holds dims [c * D/4, (c + 1) * D/4) of keys g and g + 8 (g = lane / 4): plain
-// 16-byte loads, each row read whole by four lanes.  For V, lane (g, c) loads dims
-// [g * D/8, (g + 1) * D/8) of keys 2c, 2c+1, 2c+8, 2c+9; pairing two keys' bytes with one
-// byte permutation gives the A operand, so V is transposed without shared memory.  P^T is
-// turned into the B operand by movmatrix.
+// lane group holds the 16-byte pieces c, c + 4, .. of the rows of keys g and g + 8 (g = lane /
+// 4): plain 16-byte loads, four lanes to 64 contiguous bytes (whole sectors: with D/4
+// contiguous dims per lane every sector was fetched twice).  For V, lane (g, c) holds the
+// pieces g, g + 8 of keys 2c, 2c+1, 2c+8, 2c+9; pairing two keys' bytes with one byte
+// permutation gives the A operand, so V is transposed without shared memory.  P^T is turned
+// into the B operand by movmatrix.
 // 8-bit codes become fp16 exactly (e4m3 by cvt, int8 by adding 1024), so no value is
 // rounded before the tensor core: scores are q (fp16, scaled by a power of two per row) .
 // code, times the block's fp32 key scale; P is multiplied by the block's value scale
@@ -32,7 +33,7 @@ namespace ckv {
 namespace {
 
 constexpr int kBlk = CKV_PAGE_TOKENS;
-constexpr int kWarps = 4;  // per CTA; three CTAs per SM
+constexpr int kCluster = 8;  // CTAs that share one row tile's blocks and join through shared memory
 constexpr float kLazy = 8.0f;       // log2 units
 constexpr float kPBias = 64.0f;     // P * value scale / reference is at most 2^8 * 2^6 in fp16
 enum { kBf16 = 0, kInt8 = 1, kE4m3 = 2 };
@@ -97,68 +98,84 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float r;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
   return r;
 }
-__device__ __forceinline__ uint2 ld_stream2(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 r;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(addr) : "memory");
   return r;
 }
-
-// One block's K and V as a lane holds them.
+// A stage holds NB blocks: their 16 rows of K each, then their 16 rows of V.  A warp works on
+// the NB blocks together: two independent chains of mma and exponentials, one wait and one
+// request (a warp's latency, not the issue rate, bounds the kernel).  Two where a pair is at
+// most 8 KiB, so that twelve warps keep two stages each.
 template <int HD, int CT>
 struct Block {
   static constexpr int ES = CT == kBf16 ? 2 : 1;
-  static constexpr int KW = HD / 4 * ES / 4;  // 32-bit words of K per key and lane
-  static constexpr int VW = HD / 8 * ES / 4;  // of V
-  uint32_t k[2][KW];  // keys g, g + 8
-  uint32_t v[4][VW];  // keys 2c, 2c + 1, 2c + 8, 2c + 9
-  float ks, vs;
+  static constexpr int ROW = HD * ES;         // bytes of a row
+  static constexpr int KW = HD / 4 * ES / 4;  // 32-bit words of K per key and lane (a multiple of 4)
+  static constexpr int VW = HD / 8 * ES / 4;  // of V (2 or a multiple of 4)
+  static constexpr int HALF = kBlk * ROW;     // bytes of one block's K
+  static constexpr int NB = 4 * HALF <= 8192 ? 2 : 1;
+  static constexpr int STAGE = 2 * NB * HALF;
 
-  __device__ __forceinline__ void load(const Args& a, int hk, int b, int last_key, int lane) {
-    const int g = lane >> 2, c = lane & 3;
-    const int64_t row0 = int64_t(hk) * a.head_rows + int64_t(b) * kBlk;
-    const int vis = last_key - b * kBlk;  // rows past it are not read: zeros
+  // The warp: the rows that exist of blocks ids (a bf16 cache may end inside a block; -1: none).
+  // Lane i < 2 NB copies K or V of one block.
+  static __device__ __forceinline__ void request(const Args& a, uint8_t* stage, uint64_t* bar, int hk, const int (&ids)[NB],
+                                                 int lane) {
+    uint32_t total = 0, bytes = 0;
+    int b = -1;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t* p = a.k + ((row0 + g + 8 * i) * HD + c * (HD / 4)) * ES;
-      if (g + 8 * i <= vis) {
-#pragma unroll
-        for (int w = 0; w < KW; w += 4) {
-          const uint4 x = ld_stream(p + 4 * w);
-          k[i][w] = x.x, k[i][w + 1] = x.y, k[i][w + 2] = x.z, k[i][w + 3] = x.w;
-        }
-      } else {
-#pragma unroll
-        for (int w = 0; w < KW; ++w) k[i][w] = 0u;
-      }
+    for (int e = 0; e < NB; ++e) {
+      const uint32_t n = ids[e] < 0 ? 0u : uint32_t(min(int64_t(kBlk), a.head_rows - int64_t(ids[e]) * kBlk)) * ROW;
+      total += 2 * n;
+      if (lane % NB == e) b = ids[e], bytes = n;
     }
+    if (lane == 0) mbar_expect_tx(bar, total);
+    if (lane < 2 * NB && b >= 0)
+      bulk_load(stage + lane * HALF, (lane < NB ? a.k : a.v) + (int64_t(hk) * a.head_rows + int64_t(b) * kBlk) * ROW, bytes, bar);
+  }
+  // k: the lane's pieces of keys g, g + 8
+  static __device__ __forceinline__ void fetch_k(const uint8_t* stage, int lane, uint32_t (&k)[2][KW]) {
+    const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < KW; w += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(stage + (g + 8 * i) * ROW + 16 * (w + c));
+        k[i][w] = x.x, k[i][w + 1] = x.y, k[i][w + 2] = x.z, k[i][w + 3] = x.w;
+      }
+  }
+  // v: of keys 2c, 2c + 1, 2c + 8, 2c + 9; rows past `vis` as zeros (they may hold anything, and a
+  // weight of 0 does not silence a NaN)
+  static __device__ __forceinline__ void fetch_v(const uint8_t* stage, int lane, int vis, uint32_t (&v)[4][VW]) {
+    const int g = lane >> 2, c = lane & 3;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int key = 2 * c + (i & 1) + 8 * (i >> 1);
-      const uint8_t* p = a.v + ((row0 + key) * HD + g * (HD / 8)) * ES;
-      if (key <= vis) {
-        if constexpr (VW >= 4) {
+      const uint8_t* row = stage + (2 * c + (i & 1) + 8 * (i >> 1)) * ROW;
+      if constexpr (VW >= 4) {
 #pragma unroll
-          for (int w = 0; w < VW; w += 4) {
-            const uint4 x = ld_stream(p + 4 * w);
-            v[i][w] = x.x, v[i][w + 1] = x.y, v[i][w + 2] = x.z, v[i][w + 3] = x.w;
-          }
-        } else {
-          const uint2 x = ld_stream2(p);
-          v[i][0] = x.x, v[i][1] = x.y;
+        for (int w = 0; w < VW; w += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(row + 16 * g + 32 * w);
+          v[i][w] = x.x, v[i][w + 1] = x.y, v[i][w + 2] = x.z, v[i][w + 3] = x.w;
         }
       } else {
-#pragma unroll
-        for (int w = 0; w < VW; ++w) v[i][w] = 0u;
+        const uint2 x = *reinterpret_cast<const uint2*>(row + 8 * g);
+        v[i][0] = x.x, v[i][1] = x.y;
       }
     }
-    if constexpr (CT != kBf16) {
-      ks = __ldg(a.ks + int64_t(hk) * a.n_blocks + b);
-      vs = __ldg(a.vs + int64_t(hk) * a.n_blocks + b);
+    if (vis < kBlk - 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (2 * c + (i & 1) + 8 * (i >> 1) > vis)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) v[i][w] = 0u;
     }
   }
 };
@@ -172,51 +189,67 @@ struct State {
   int lim[NT][2];      // last visible key
   float mx[NT][2], l[NT][2];
   float ref;           // value-scale reference (power of two; 0 before the first block)
-  float o[NT][KSTEPS][4];  // dims g * HD/8 + 2t (+ 1) x rows 2c, 2c + 1
+  float o[NT][KSTEPS][4];  // the lane's V dims 2t, 2t + 1 x rows 2c, 2c + 1
 
-  __device__ __forceinline__ void step(const Block<HD, CT>& x, int b, int lane) {
+  // The blocks ids of a stage (-1: none) with their scales; `last`: the last key any row sees.
+  __device__ __forceinline__ void step(const uint8_t* stage, const int (&ids)[Block<HD, CT>::NB],
+                                       const float (&ks)[Block<HD, CT>::NB], const float (&vs)[Block<HD, CT>::NB], int last,
+                                       int lane) {
+    using B = Block<HD, CT>;
+    constexpr int NB = B::NB;
     const int g = lane >> 2;
-    float s[NT][4];
+    float s[NB][NT][4], s2[NB][NT][4];  // even and odd steps of the contraction: half the length of the chain
+    {
+      uint32_t k[NB][2][B::KW];
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < NB; ++i) {
+        B::fetch_k(stage + i * B::HALF, lane, k[i]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int t = 0; t < KSTEPS; ++t) {
-      uint32_t a0, a1, a2, a3;
-      if constexpr (CT == kBf16) {
-        a0 = x.k[0][2 * t], a2 = x.k[0][2 * t + 1], a1 = x.k[1][2 * t], a3 = x.k[1][2 * t + 1];
-      } else {
-        widen<CT>(x.k[0][t], a0, a2);
-        widen<CT>(x.k[1][t], a1, a3);
+          for (int e = 0; e < 4; ++e) s[i][n][e] = s2[i][n][e] = 0.f;
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma<CT>(s[n], a0, a1, a2, a3, qf[n][t][0], qf[n][t][1]);
+      for (int t = 0; t < KSTEPS; ++t) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (CT == kBf16) {
+            a0 = k[i][0][2 * t], a2 = k[i][0][2 * t + 1], a1 = k[i][1][2 * t], a3 = k[i][1][2 * t + 1];
+          } else {
+            widen<CT>(k[i][0][t], a0, a2);
+            widen<CT>(k[i][1][t], a1, a3);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma<CT>(t & 1 ? s2[i][n] : s[i][n], a0, a1, a2, a3, qf[n][t][0], qf[n][t][1]);
+        }
+      }
     }
-    const int key = b * kBlk + g;
+    // Scores; a row's maximum is renewed (and O rescaled) only when some score exceeds it by
+    // more than 2^kLazy, so the usual step needs no reduction over the lanes.
     bool grow = false;
-    float top[NT][2];
+    float vtop = 0.f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int i = 0; i < NB; ++i) {
+      const int key = ids[i] < 0 ? 0x7fffff00 : ids[i] * kBlk + g;
+      if constexpr (CT != kBf16) vtop = fmaxf(vtop, vs[i]);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float fk = CT == kBf16 ? f[n][r] : f[n][r] * x.ks;
-        s[n][r] = key <= lim[n][r] ? s[n][r] * fk : -INFINITY;
-        s[n][2 + r] = key + 8 <= lim[n][r] ? s[n][2 + r] * fk : -INFINITY;
-        float t = fmaxf(s[n][r], s[n][2 + r]);
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
-        top[n][r] = t;
-        grow |= t > mx[n][r] + kLazy || (mx[n][r] == -INFINITY && t > -INFINITY);
-      }
-    if constexpr (CT != kBf16) grow |= x.vs > ref;
+        for (int r = 0; r < 2; ++r) {
+          const float fk = CT == kBf16 ? f[n][r] : f[n][r] * ks[i];
+          s[i][n][r] = key <= lim[n][r] ? (s[i][n][r] + s2[i][n][r]) * fk : -INFINITY;
+          s[i][n][2 + r] = key + 8 <= lim[n][r] ? (s[i][n][2 + r] + s2[i][n][2 + r]) * fk : -INFINITY;
+          grow |= fmaxf(s[i][n][r], s[i][n][2 + r]) > mx[n][r] + kLazy;  // (mx = -inf: any score)
+        }
+    }
+    if constexpr (CT != kBf16) grow |= vtop > ref;
     if (__any_sync(0xffffffffu, grow)) {
       float rs = 1.0f;
       if constexpr (CT != kBf16) {
-        if (x.vs > ref) {  // the same for the whole warp
-          // the next power of two at or above vs
-          const uint32_t bits = __float_as_uint(x.vs);
-          const float up = __uint_as_float((bits + 0x007fffffu) & 0x7f800000u);
+        if (vtop > ref) {  // the same for the whole warp
+          // the next power of two at or above it
+          const float up = __uint_as_float((__float_as_uint(vtop) + 0x007fffffu) & 0x7f800000u);
           rs = ref / up;
           ref = up;
         }
@@ -225,10 +258,14 @@ struct State {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float m_new = fmaxf(mx[n][r], top[n][r]);
-          const float corr = mx[n][r] == -INFINITY ? 0.f : ex2_approx(mx[n][r] - m_new);
+          float top = mx[n][r];
+#pragma unroll
+          for (int i = 0; i < NB; ++i) top = fmaxf(top, fmaxf(s[i][n][r], s[i][n][2 + r]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+          const float corr = mx[n][r] == -INFINITY ? 0.f : ex2_approx(mx[n][r] - top);
           l[n][r] *= corr;
-          mx[n][r] = m_new;
+          mx[n][r] = top;
 #pragma unroll
           for (int t = 0; t < KSTEPS; ++t) {
             o[n][t][r] *= corr * rs;
@@ -236,72 +273,93 @@ struct State {
           }
         }
     }
-    const float vn = CT == kBf16 ? 1.0f : (ref > 0.f ? x.vs * (kPBias / ref) : 0.f);
-    uint32_t ph[NT][2], pl[NT][2];
+    uint32_t ph[NB][NT][2];
+    [[maybe_unused]] uint32_t pl[NB][NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float p[4];
+    for (int i = 0; i < NB; ++i) {
+      const float vn = CT == kBf16 ? 1.0f : (ref > 0.f ? vs[i] * (kPBias / ref) : 0.f);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float base = mx[n][e & 1] == -INFINITY ? 0.f : mx[n][e & 1];  // no visible key yet: P = 0, not NaN
-        p[e] = ex2_approx(s[n][e] - base);
-        l[n][e & 1] += p[e];
-      }
-      if constexpr (CT == kBf16) {
+      for (int n = 0; n < NT; ++n) {
+        float p[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t hi = pack_bf2(p[2 * i], p[2 * i + 1]);
-          ph[n][i] = transpose8(hi);
-          pl[n][i] = transpose8(pack_bf2(p[2 * i] - lo_bf(hi), p[2 * i + 1] - hi_bf(hi)));
+        for (int e = 0; e < 4; ++e) {
+          const float base = mx[n][e & 1] == -INFINITY ? 0.f : mx[n][e & 1];  // no visible key yet: P = 0, not NaN
+          p[e] = ex2_approx(s[i][n][e] - base);
+          l[n][e & 1] += p[e];
         }
-      } else {
-        ph[n][0] = transpose8(pack_h2(p[0] * vn, p[1] * vn));
-        ph[n][1] = transpose8(pack_h2(p[2] * vn, p[3] * vn));
+        if constexpr (CT == kBf16) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t hi = pack_bf2(p[2 * h], p[2 * h + 1]);
+            ph[i][n][h] = transpose8(hi);
+            pl[i][n][h] = transpose8(pack_bf2(p[2 * h] - lo_bf(hi), p[2 * h + 1] - hi_bf(hi)));
+          }
+        } else {
+          ph[i][n][0] = transpose8(pack_h2(p[0] * vn, p[1] * vn));
+          ph[i][n][1] = transpose8(pack_h2(p[2] * vn, p[3] * vn));
+        }
       }
     }
-    if constexpr (CT == kBf16) {
 #pragma unroll
-      for (int w = 0; w < KSTEPS; ++w) {
-        const uint32_t a0 = __byte_perm(x.v[0][w], x.v[1][w], 0x5410), a1 = __byte_perm(x.v[0][w], x.v[1][w], 0x7632);
-        const uint32_t a2 = __byte_perm(x.v[2][w], x.v[3][w], 0x5410), a3 = __byte_perm(x.v[2][w], x.v[3][w], 0x7632);
+    for (int i = 0; i < NB; ++i) {
+      uint32_t v[4][B::VW];
+      B::fetch_v(stage + (NB + i) * B::HALF, lane, ids[i] < 0 ? -1 : last - ids[i] * kBlk, v);
+      if constexpr (CT == kBf16) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma_bf16(o[n][w], a0, a1, a2, a3, ph[n][0], ph[n][1]);
-          mma_bf16(o[n][w], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+        for (int w = 0; w < KSTEPS; ++w) {
+          const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5410), a1 = __byte_perm(v[0][w], v[1][w], 0x7632);
+          const uint32_t a2 = __byte_perm(v[2][w], v[3][w], 0x5410), a3 = __byte_perm(v[2][w], v[3][w], 0x7632);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_bf16(o[n][w], a0, a1, a2, a3, ph[i][n][0], ph[i][n][1]);
+            mma_bf16(o[n][w], a0, a1, a2, a3, pl[i][n][0], pl[i][n][1]);
+          }
         }
-      }
-    } else {
+      } else {
 #pragma unroll
-      for (int w = 0; w < KSTEPS / 2; ++w) {
-        // keys 2c, 2c+1 (and 2c+8, 2c+9) of dims 4w .. 4w+3, two keys of a dim side by side
-        uint32_t a0, a1, a2, a3;
-        widen<CT>(__byte_perm(x.v[0][w], x.v[1][w], 0x5140), a0, a1);
-        widen<CT>(__byte_perm(x.v[2][w], x.v[3][w], 0x5140), a2, a3);
+        for (int w = 0; w < KSTEPS / 2; ++w) {
+          // keys 2c, 2c+1 (and 2c+8, 2c+9) of dims 4w .. 4w+3, two keys of a dim side by side
+          uint32_t a0, a1, a2, a3;
+          widen<CT>(__byte_perm(v[0][w], v[1][w], 0x5140), a0, a1);
+          widen<CT>(__byte_perm(v[2][w], v[3][w], 0x5140), a2, a3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w], a0, a1, a2, a3, ph[n][0], ph[n][1]);
-        widen<CT>(__byte_perm(x.v[0][w], x.v[1][w], 0x7362), a0, a1);
-        widen<CT>(__byte_perm(x.v[2][w], x.v[3][w], 0x7362), a2, a3);
+          for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w], a0, a1, a2, a3, ph[i][n][0], ph[i][n][1]);
+          widen<CT>(__byte_perm(v[0][w], v[1][w], 0x7362), a0, a1);
+          widen<CT>(__byte_perm(v[2][w], v[3][w], 0x7362), a2, a3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w + 1], a0, a1, a2, a3, ph[n][0], ph[n][1]);
+          for (int n = 0; n < NT; ++n) mma_f16(o[n][2 * w + 1], a0, a1, a2, a3, ph[i][n][0], ph[i][n][1]);
+        }
       }
     }
   }
 };
 
-template <int HD>
-struct Merge {
-  static constexpr int STRIDE = HD + 4;
+// Shared memory: W rings of stages; after the loop the same space takes the warps' states, and
+// behind it the CTA's joined state (read by the cluster's other CTAs) and the barriers.
+template <int HD, int CT, int NT, int W>
+struct Layout {
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int STAGES = W > 8 ? 2 : 3;
+  static constexpr int RING = STAGES * Block<HD, CT>::STAGE;
+  static constexpr int STRIDE = HD + 4;  // floats of a state row
+  static constexpr int STATES = W * ROWS * (STRIDE + 2) * 4;
+  static constexpr int JOINED = (W * RING > STATES ? W * RING : STATES + 15) / 16 * 16;
+  static constexpr int BARS = JOINED + ROWS * (STRIDE + 2) * 4;
+  static constexpr int BYTES = BARS + W * STAGES * 8 + 8;
 };
 
 // grid: (splits, row tiles, KV heads).  Dense (LISTED = false): tile y holds the packed rows
 // (token, head of the group) [8 NT y, 8 NT (y + 1)) of its KV head.  Listed: tile y is head
 // tile y % head_tiles of token y / head_tiles, and the split takes its share of the list.
-template <int HD, int CT, int NT, bool LISTED>
-__global__ void __launch_bounds__(kWarps * 32, (CT == kBf16 || NT == 2) ? 2 : 3)
+// JOIN: the kCluster splits of a tile are one cluster and leave finished rows; otherwise more
+// than one split leaves partials for attention_blocks_join_kernel.
+template <int HD, int CT, int NT, bool LISTED, int W, bool JOIN>
+__global__ void __launch_bounds__(W * 32, W > 4 ? 1 : (CT == kBf16 || NT == 2) ? 2 : 3)
     attention_blocks_kernel(const __grid_constant__ Args a) {
-  constexpr int KSTEPS = HD / 16, ROWS = 8 * NT;
-  __shared__ __align__(16) float s_o[kWarps][ROWS][HD + 4];
-  __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+  using L = Layout<HD, CT, NT, W>;
+  using B = Block<HD, CT>;
+  constexpr int KSTEPS = HD / 16, ROWS = L::ROWS;
+  extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int G = a.Hq / a.Hk;
@@ -310,77 +368,36 @@ __global__ void __launch_bounds__(kWarps * 32, (CT == kBf16 || NT == 2) ? 2 : 3)
   const int tok0 = LISTED ? tile / a.head_tiles : 0;
   const int row0 = LISTED ? tok0 * G + (tile % a.head_tiles) * ROWS : tile * ROWS;  // packed row
   const int row_end = LISTED ? tok0 * G + G : a.m * G;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS) + warp * L::STAGES;
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BARS + W * L::STAGES * 8);
+  if (lane == 0) {
+    for (int s = 0; s < L::STAGES; ++s) mbar_init(&bars[s], 1);
+    fence_barrier_init();
+  }
+  if (threadIdx.x == 0) *abort = 0;
+  __syncthreads();
   pdl_wait();
   pdl_launch_next();
 
-  State<HD, CT, NT> st;
+  // as an operand owner a lane has query rows 8n + g: their positions first, then the first
+  // blocks are on their way while q is loaded
+  int pos[NT];
   int last = -1;  // last key any row of the tile sees
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    // as an operand owner: query row 8n + g, dims [c * HD/4, ..)
     const int pr = row0 + 8 * n + g;
-    const bool ok = pr < row_end;
-    const int tok = ok ? pr / G : 0;
     int p = -1;
-    if (ok) {
-      p = a.positions[tok];
+    if (pr < row_end) {
+      p = a.positions[pr / G];
       if (p >= a.n_ctx) {
         if (split == 0 && hk == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
         p = a.n_ctx - 1;
       }
       p = max(p, -1);
     }
-    uint32_t w[HD / 8];
-#pragma unroll
-    for (int i = 0; i < HD / 8; i += 4) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (ok)
-        x = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD + c * (HD / 4)) + i / 4);
-      w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
-    }
-    float factor = a.scale_log2;
-    if constexpr (CT == kBf16) {
-#pragma unroll
-      for (int t = 0; t < KSTEPS; ++t) {
-        st.qf[n][t][0] = w[2 * t];
-        st.qf[n][t][1] = w[2 * t + 1];
-      }
-    } else {
-      // to fp16 through a power of two that puts the row's largest value in [2^14, 2^15):
-      // exact down to 2^-38 of it
-      uint32_t mag = 0;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) mag = __vmaxu2(mag, w[i] & 0x7fff7fffu);
-      uint32_t am = max(mag & 0xffffu, mag >> 16);
-      am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
-      am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
-      const int e = int(am >> 7);  // biased exponent of the largest value
-      int sh = 14 + 127 - e;       // multiply by 2^sh
-      sh = am == 0 ? 0 : max(-126, min(sh, 126));
-      const float up = __uint_as_float(uint32_t(sh + 127) << 23);
-      factor *= __uint_as_float(uint32_t(127 - sh) << 23);
-#pragma unroll
-      for (int t = 0; t < KSTEPS; ++t) {
-        st.qf[n][t][0] = pack_h2(lo_bf(w[2 * t]) * up, hi_bf(w[2 * t]) * up);
-        st.qf[n][t][1] = pack_h2(lo_bf(w[2 * t + 1]) * up, hi_bf(w[2 * t + 1]) * up);
-      }
-    }
-    // as a column owner: rows 8n + 2c and 8n + 2c + 1
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      st.f[n][r] = __shfl_sync(0xffffffffu, factor, 4 * (2 * c + r));
-      st.lim[n][r] = __shfl_sync(0xffffffffu, p, 4 * (2 * c + r));
-      st.mx[n][r] = -INFINITY;
-      st.l[n][r] = 0.f;
-    }
-#pragma unroll
-    for (int t = 0; t < KSTEPS; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) st.o[n][t][e] = 0.f;
+    pos[n] = p;
     last = max(last, __reduce_max_sync(0xffffffffu, p));
   }
-  st.ref = 0.f;
-
   const int nb = (last + kBlk) / kBlk;  // visible blocks
   const int n_items = LISTED ? a.top : nb;
   const int per = (n_items + a.splits - 1) / a.splits;
@@ -398,19 +415,123 @@ __global__ void __launch_bounds__(kWarps * 32, (CT == kBf16 || NT == 2) ? 2 : 3)
     }
     return b < nb ? b : -1;  // wholly past the row's position: nothing visible
   };
-  int i = split * per + warp;
-  Block<HD, CT> cur, nxt;
-  int b = block_of(i);
-  if (b >= 0) cur.load(a, hk, b, last, lane);
-  for (; i < i1; i += kWarps) {
-    const int bn = block_of(i + kWarps);
-    if (bn >= 0) nxt.load(a, hk, bn, last, lane);
-    if (b >= 0) st.step(cur, b, lane);
-    cur = nxt;
-    b = bn;
-  }
+  uint8_t* ring = smem + warp * L::RING;
+  constexpr int NB = B::NB;
+  int ids[L::STAGES][NB];                           // blocks in the ring, -1: none
+  float ks[L::STAGES][NB] = {}, vs[L::STAGES][NB] = {};  // their scales
+  int i = split * per + warp * NB;
+  auto fill = [&](int s, int at) {
+#pragma unroll
+    for (int e = 0; e < NB; ++e) ids[s][e] = block_of(at + e);
+    bool any = ids[s][0] >= 0;
+    if constexpr (NB == 2) any |= ids[s][1] >= 0;
+    if (any) B::request(a, ring + s * B::STAGE, &bars[s], hk, ids[s], lane);
+    if constexpr (CT != kBf16) {
+#pragma unroll
+      for (int e = 0; e < NB; ++e) {
+        const int64_t b = int64_t(hk) * a.n_blocks + ids[s][e];
+        ks[s][e] = ids[s][e] < 0 ? 0.f : __ldg(a.ks + b);
+        vs[s][e] = ids[s][e] < 0 ? 0.f : __ldg(a.vs + b);
+      }
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < L::STAGES; ++s) fill(s, i + s * W * NB);
 
-  // the warps' states meet in shared memory
+  State<HD, CT, NT> st;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    // query row 8n + g, the dims of this lane's pieces of K (16 / ES dims each)
+    const int pr = row0 + 8 * n + g;
+    const bool ok = pr < row_end;
+    const int tok = ok ? pr / G : 0;
+    uint32_t w[HD / 8];
+#pragma unroll
+    for (int e = 0; e < HD / 8; e += 4) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (ok)
+        x = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
+                  (B::ES == 2 ? e + c : 8 * (e / 8) + 2 * c + (e / 4) % 2));
+      w[e] = x.x, w[e + 1] = x.y, w[e + 2] = x.z, w[e + 3] = x.w;
+    }
+    float factor = a.scale_log2;
+    if constexpr (CT == kBf16) {
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        st.qf[n][t][0] = w[2 * t];
+        st.qf[n][t][1] = w[2 * t + 1];
+      }
+    } else {
+      // to fp16 through a power of two that puts the row's largest value in [2^14, 2^15):
+      // exact down to 2^-38 of it
+      uint32_t mag = 0;
+#pragma unroll
+      for (int e = 0; e < HD / 8; ++e) mag = __vmaxu2(mag, w[e] & 0x7fff7fffu);
+      uint32_t am = max(mag & 0xffffu, mag >> 16);
+      am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      const int sh = am == 0 ? 0 : max(-126, min(126, 14 + 127 - int(am >> 7)));  // multiply by 2^sh
+      const float up = __uint_as_float(uint32_t(sh + 127) << 23);
+      factor *= __uint_as_float(uint32_t(127 - sh) << 23);
+#pragma unroll
+      for (int t = 0; t < KSTEPS; ++t) {
+        st.qf[n][t][0] = pack_h2(lo_bf(w[2 * t]) * up, hi_bf(w[2 * t]) * up);
+        st.qf[n][t][1] = pack_h2(lo_bf(w[2 * t + 1]) * up, hi_bf(w[2 * t + 1]) * up);
+      }
+    }
+    // as a column owner: rows 8n + 2c and 8n + 2c + 1
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      st.f[n][r] = __shfl_sync(0xffffffffu, factor, 4 * (2 * c + r));
+      st.lim[n][r] = __shfl_sync(0xffffffffu, pos[n], 4 * (2 * c + r));
+      st.mx[n][r] = -INFINITY;
+      st.l[n][r] = 0.f;
+    }
+#pragma unroll
+    for (int t = 0; t < KSTEPS; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.o[n][t][e] = 0.f;
+  }
+  st.ref = 0.f;
+
+  uint32_t phase = 0;  // bit s: parity of stage s's next arrival
+  bool ok = true;
+  auto filled = [&](int s) {
+    bool any = ids[s][0] >= 0;
+    if constexpr (NB == 2) any |= ids[s][1] >= 0;
+    return any;
+  };
+  while (i < i1 && ok) {
+#pragma unroll
+    for (int s = 0; s < L::STAGES; ++s) {
+      if (filled(s)) {
+        ok = ok && mbar_wait(&bars[s], (phase >> s) & 1, abort, &g_err_word);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        phase ^= 1u << s;
+        st.step(ring + s * B::STAGE, ids[s], ks[s], vs[s], last, lane);
+        __syncwarp();  // every lane has read the stage: it may be filled again
+      }
+      fill(s, i + (s + L::STAGES) * W * NB);
+    }
+    i += L::STAGES * W * NB;
+  }
+  if (!ok) {  // a copy never came: let those still out land (bounded) before the ring is reused
+    uint32_t out = 0;
+#pragma unroll
+    for (int s = 0; s < L::STAGES; ++s) out |= filled(s) ? 1u << s : 0u;
+    const uint64_t t0 = global_ns();
+#pragma unroll 1
+    for (int s = 0; s < L::STAGES; ++s)
+      while ((out >> s) & 1) {
+        if (mbar_try_wait(&bars[s], (phase >> s) & 1) || global_ns() - t0 > kWaitLimitNs) break;
+      }
+  }
+  __syncthreads();  // the rings are free: they become the warps' states
+
+  float* s_o = reinterpret_cast<float*>(smem);  // [W][ROWS][STRIDE]
+  float* s_m = s_o + W * ROWS * L::STRIDE;      // [W][ROWS]
+  float* s_l = s_m + W * ROWS;
   const float oscale = CT == kBf16 ? 1.0f : st.ref / kPBias;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -421,48 +542,91 @@ __global__ void __launch_bounds__(kWarps * 32, (CT == kBf16 || NT == 2) ? 2 : 3)
       for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
       const int row = 8 * n + 2 * c + r;
       if (g == 0) {
-        s_m[warp][row] = st.mx[n][r];
-        s_l[warp][row] = l;
+        s_m[warp * ROWS + row] = st.mx[n][r];
+        s_l[warp * ROWS + row] = l;
       }
 #pragma unroll
       for (int t = 0; t < KSTEPS; t += 2)
-        *reinterpret_cast<float4*>(&s_o[warp][row][g * (HD / 8) + 2 * t]) =
+        // V dims 2t .. 2t + 3 of the lane: piece t / 4 (8 dims) of a bf16 row, else its only one
+        *reinterpret_cast<float4*>(s_o + (warp * ROWS + row) * L::STRIDE +
+                                   (CT == kBf16 ? 64 * (t / 4) + 8 * g + 2 * (t % 4) : g * (HD / 8) + 2 * t)) =
             make_float4(st.o[n][t][r] * oscale, st.o[n][t][2 + r] * oscale, st.o[n][t + 1][r] * oscale,
                         st.o[n][t + 1][2 + r] * oscale);
     }
   __syncthreads();
   constexpr int QV = HD / 4;  // float4 columns of a row
+  auto store_row = [&](int pr, int col, const float4& o, float l) {
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const int tok = pr / G;
+    *reinterpret_cast<uint2*>(a.out + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD + col) =
+        make_uint2(pack_bf2(o.x * inv, o.y * inv), pack_bf2(o.z * inv, o.w * inv));
+  };
+  float* j_o = reinterpret_cast<float*>(smem + L::JOINED);  // [ROWS][STRIDE], then m and l
   const int64_t prow0 = ((int64_t(split) * gridDim.y + tile) * a.Hk + hk) * ROWS;
-  for (int j = threadIdx.x; j < ROWS * QV; j += kWarps * 32) {
+  for (int j = threadIdx.x; j < ROWS * QV; j += W * 32) {
     const int row = j / QV, col = (j - row * QV) * 4;
     const int pr = row0 + row;
     if (pr >= row_end) continue;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_m[w][row]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, s_m[w * ROWS + row]);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (m > -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float wt = ex2_approx(s_m[w][row] - m);
-        const float4 x = *reinterpret_cast<const float4*>(&s_o[w][row][col]);
-        l = fmaf(wt, s_l[w][row], l);
+      for (int w = 0; w < W; ++w) {
+        const float wt = ex2_approx(s_m[w * ROWS + row] - m);
+        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * L::STRIDE + col);
+        l = fmaf(wt, s_l[w * ROWS + row], l);
         o.x = fmaf(wt, x.x, o.x);
         o.y = fmaf(wt, x.y, o.y);
         o.z = fmaf(wt, x.z, o.z);
         o.w = fmaf(wt, x.w, o.w);
       }
     }
-    if (a.splits > 1) {
+    if constexpr (JOIN) {
+      *reinterpret_cast<float4*>(j_o + row * L::STRIDE + col) = o;
+      if (col == 0) {
+        j_o[ROWS * L::STRIDE + row] = m;
+        j_o[ROWS * (L::STRIDE + 1) + row] = l;
+      }
+    } else if (a.splits > 1) {
       *reinterpret_cast<float4*>(a.part_o + (prow0 + row) * HD + col) = o;
       if (col == 0) a.part_ml[prow0 + row] = make_float2(m, l);
     } else {
-      const float inv = l > 0.f ? 1.0f / l : 0.f;
-      const int tok = pr / G;
-      *reinterpret_cast<uint2*>(a.out + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD + col) =
-          make_uint2(pack_bf2(o.x * inv, o.y * inv), pack_bf2(o.z * inv, o.w * inv));
+      store_row(pr, col, o, l);
     }
+  }
+  if constexpr (JOIN) {
+    // the cluster's CTAs each finish a share of the columns from everybody's joined states
+    cluster_sync();
+    const int rank = split;  // the cluster spans the splits
+    const int n_cols = min(ROWS, row_end - row0) * QV;
+    for (int j = rank * (W * 32) + threadIdx.x; j < n_cols; j += kCluster * W * 32) {
+      const int row = j / QV, col = (j - row * QV) * 4;
+      float mr[kCluster], m = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        mr[r] = ld_cluster(cluster_smem_addr(j_o + ROWS * L::STRIDE + row, r));
+        m = fmaxf(m, mr[r]);
+      }
+      float l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (m > -INFINITY) {
+#pragma unroll
+        for (int r = 0; r < kCluster; ++r) {
+          const float wt = ex2_approx(mr[r] - m);
+          const float4 x = ld_cluster4(cluster_smem_addr(j_o + row * L::STRIDE + col, r));
+          l = fmaf(wt, ld_cluster(cluster_smem_addr(j_o + ROWS * (L::STRIDE + 1) + row, r)), l);
+          o.x = fmaf(wt, x.x, o.x);
+          o.y = fmaf(wt, x.y, o.y);
+          o.z = fmaf(wt, x.z, o.z);
+          o.w = fmaf(wt, x.w, o.w);
+        }
+      }
+      store_row(row0 + row, col, o, l);
+    }
+    cluster_sync();  // no CTA leaves while its shared memory is read
   }
 }
 
@@ -536,32 +700,71 @@ __global__ void __launch_bounds__(256) attention_blocks_join_kernel(const __grid
 
 struct Plan {
   int nt, tiles, head_tiles, splits;
+  bool join;  // the splits are one cluster
   int64_t bytes;
 };
 
-// Rows of one KV head in tiles of 8 (or 16), and the blocks split over CTAs until about
-// three CTAs per SM run, but no finer than one block per warp.
-Plan plan(int m, int G, int Hk, int HD, int items, bool listed) {
+// Bytes of cache that one CTA of a cluster streams at most: beyond, the few SMs of the clusters
+// would be slower than all SMs with a second kernel for the join.
+constexpr int64_t kClusterBytes = 192 * 1024;
+
+// Rows of one KV head in tiles of 8 (or 16).  With too few tiles to fill the SMs the blocks are
+// split: over the eight CTAs of a cluster while that moves few bytes per CTA (one launch, no
+// workspace), else over enough CTAs for three per SM, no finer than one block per warp.
+Plan plan(int m, int G, int Hk, int HD, int es, int items, bool listed) {
   Plan p;
   p.nt = (listed ? G : int64_t(m) * G) > 8 ? 2 : 1;
   p.head_tiles = listed ? ceil_div(G, 8 * p.nt) : 1;
   p.tiles = listed ? m * p.head_tiles : ceil_div(int64_t(m) * G, 8 * p.nt);
   const int64_t ctas = int64_t(p.tiles) * Hk;
-  const int want = int(std::min<int64_t>(std::max<int64_t>(1, 3 * num_sms() / ctas), ceil_div(items, kWarps)));
-  p.splits = std::max(1, want);
-  p.bytes = p.splits > 1 ? int64_t(p.splits) * ctas * 8 * p.nt * (int64_t(HD) * 4 + 8) : 0;
+  const int64_t cta_bytes = int64_t(items) * kBlk * HD * es * 2 / kCluster;
+  p.splits = 1;
+  p.join = false;
+  if (items > 4 && ctas * kCluster <= 2 * num_sms() && cta_bytes <= kClusterBytes) {
+    p.splits = kCluster;
+    p.join = true;
+  } else {
+    p.splits = int(std::min<int64_t>(std::max<int64_t>(1, (listed ? 3 : 1) * num_sms() / ctas), ceil_div(items, listed ? 4 : 8)));
+  }
+  p.bytes = p.splits > 1 && !p.join ? int64_t(p.splits) * ctas * 8 * p.nt * (int64_t(HD) * 4 + 8) : 0;
   return p;
 }
 
 template <int HD, int CT, int NT, bool LISTED>
 int launch(Args a, const Plan& p, void* workspace, cudaStream_t stream) {
+  a.splits = p.splits;
+  a.head_tiles = p.head_tiles;
+  if (p.join) {
+    using L = Layout<HD, CT, NT, 8>;
+    auto kern = attention_blocks_kernel<HD, CT, NT, LISTED, 8, true>;
+    if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), L::BYTES)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits, p.tiles, a.Hk);
+    cfg.blockDim = dim3(8 * 32);
+    cfg.dynamicSmemBytes = L::BYTES;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kCluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kern, a);
+    CKV_LAUNCH_CHECK("ckv_attention_blocks(cluster)");
+    return CKV_OK;
+  }
   if (p.splits > 1) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(p.splits) * p.tiles * a.Hk * 8 * NT * HD);
   }
-  a.splits = p.splits;
-  a.head_tiles = p.head_tiles;
-  launch_pdl(attention_blocks_kernel<HD, CT, NT, LISTED>, dim3(p.splits, p.tiles, a.Hk), dim3(kWarps * 32), 0, stream, a);
+  constexpr int W = LISTED ? 4 : NT == 2 ? 8 : 12;
+  using L = Layout<HD, CT, NT, W>;
+  auto kern = attention_blocks_kernel<HD, CT, NT, LISTED, W, false>;
+  if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), L::BYTES)) return rc;
+  launch_pdl(kern, dim3(p.splits, p.tiles, a.Hk), dim3(W * 32), L::BYTES, stream, a);
   CKV_LAUNCH_CHECK("ckv_attention_blocks");
   if (p.splits > 1) {
     launch_pdl(attention_blocks_join_kernel<HD>, dim3(a.m * (a.Hq / a.Hk), a.Hk), dim3(256), 0, stream, a, p.tiles, 8 * NT,
@@ -575,6 +778,8 @@ template <int HD, int CT, bool LISTED>
 int launch_nt(const Args& a, const Plan& p, void* workspace, cudaStream_t stream) {
   return p.nt == 1 ? launch<HD, CT, 1, LISTED>(a, p, workspace, stream) : launch<HD, CT, 2, LISTED>(a, p, workspace, stream);
 }
+
+int launches(const Plan& p) { return p.splits > 1 && !p.join ? 2 : 1; }
 
 bool shape_ok(int m, int Hq, int Hk, int HD, int n_ctx) {
   return m >= 0 && Hk > 0 && Hk <= 65535 && Hq > 0 && Hq % Hk == 0 && (HD == 64 || HD == 128) && n_ctx > 0 && n_ctx <= (1 << 30);
@@ -602,10 +807,10 @@ int check(const char* name, const Args& a, int HD, int64_t tiles) {
 
 // Few query rows over a whole 8-bit cache; used by ckv_attention_kv8 (attention_kv8.cu).
 int64_t kv8_stream_workspace(int m, int Hq, int Hk, int HD, int n_ctx) {
-  return plan(m, Hq / Hk, Hk, HD, ceil_div(n_ctx, kBlk), false).bytes;
+  return plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false).bytes;
 }
 int kv8_stream_launches(int m, int Hq, int Hk, int HD, int n_ctx) {
-  return plan(m, Hq / Hk, Hk, HD, ceil_div(n_ctx, kBlk), false).splits > 1 ? 2 : 1;
+  return launches(plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false));
 }
 int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs,
                          const int32_t* positions, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, float scale, int type,
@@ -613,7 +818,7 @@ int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8
   const int nb = ceil_div(n_ctx, kBlk);
   Args a{q, k8, v8, ks, vs, positions, nullptr, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, 0, 1, 1,
          scale * 1.4426950408889634f};
-  const Plan p = plan(m, Hq / Hk, Hk, HD, nb, false);
+  const Plan p = plan(m, Hq / Hk, Hk, HD, 1, nb, false);
   if (int rc = check("ckv_attention_kv8", a, HD, p.tiles)) return rc;
   if (HD == 128)
     return type == CKV_KV8_E4M3 ? launch_nt<128, kE4m3, false>(a, p, workspace, stream)
@@ -626,20 +831,20 @@ int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8
 
 using namespace ckv;
 
-extern "C" int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top) {
+extern "C" int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int bits) {
   if (m <= 0 || top <= 0 || !shape_ok(m, n_q_heads, n_kv_heads, head_dim, 1)) return 0;
-  return plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, top, true).bytes;
+  return plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, bits / 8, top, true).bytes;
 }
 
-extern "C" int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top) {
+extern "C" int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int bits) {
   if (m <= 0 || top <= 0 || !shape_ok(m, n_q_heads, n_kv_heads, head_dim, 1)) return 0;
-  return plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, top, true).splits > 1 ? 2 : 1;
+  return launches(plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, bits / 8, top, true));
 }
 
 static int attention_blocks(const char* name, Args a, int HD, int type, void* workspace, int64_t ws_bytes, cudaStream_t s) {
   CKV_REQUIRE(a.top > 0, "%s: lists of %d blocks", name, a.top);
   const bool sane = a.Hk > 0 && a.Hq > 0 && a.m >= 0;
-  const Plan p = sane ? plan(a.m, std::max(1, a.Hq / a.Hk), a.Hk, HD, a.top, true) : Plan{};
+  const Plan p = sane ? plan(a.m, std::max(1, a.Hq / a.Hk), a.Hk, HD, type < 0 ? 2 : 1, a.top, true) : Plan{};
   if (int rc = check(name, a, HD, 0)) return rc;
   if (a.m == 0) return CKV_OK;
   CKV_REQUIRE(a.blocks != nullptr, "%s: null block list", name);

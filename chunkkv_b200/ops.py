@@ -86,7 +86,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the handle alone: torch.cuda.current_stream() builds a Stream object (3.3 us a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _cuda(*ts: torch.Tensor | None) -> None:
@@ -1005,8 +1006,8 @@ def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         _buf("out", out, m * Hq * D)
     _on_device(q, k_cache, v_cache, positions, blocks, out)
     lib = _lib.load()
-    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top), q.device)
-    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top)
+    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top, 16), q.device)
+    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top, 16)
     _run("ckv_attention_blocks", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
          blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, 1.0 / math.sqrt(D) if scale is None else float(scale),
          _ptr(ws), nbytes, _stream(), kernels=kernels)
@@ -1026,8 +1027,8 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
         _buf("out", out, m * Hq * D)
     _on_device(q, positions, blocks, out, cache.k)
     lib = _lib.load()
-    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top), q.device)
-    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top)
+    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top, 8), q.device)
+    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top, 8)
     _run("ckv_attention_blocks_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
          top, 1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), nbytes,

@@ -434,10 +434,11 @@ CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const f
 
 /* Attention of row i over the keys j <= positions[i] of the blocks listed for it (ascending, -1
  * past the end; an entry out of range or not above the one before it is skipped and recorded as
- * CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache.  Rows that see no
- * key give zeros. */
-CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top);
-CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top);
+ * CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache (cache_bits 16 or 8).
+ * Rows that see no key give zeros. */
+CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top,
+                                                    int cache_bits);
+CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int cache_bits);
 CKV_API int ckv_attention_blocks(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
                                  const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int n_q_heads,
                                  int n_kv_heads, int head_dim, int n_ctx, int top, float scale, void* workspace,
