@@ -29,13 +29,17 @@ constexpr int kBlk = CKV_PAGE_TOKENS;
 constexpr int kScoreWarps = 8;
 constexpr int kTok = 16;  // query tokens per score CTA (they share the digest rows it loads)
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
-constexpr int kMaxBlocks = 49152;  // keys of one (token, head) held in shared memory
+constexpr int kMaxBlocks = 32768;  // keys of one (token, head) held in a CTA's registers
 constexpr int kMaxTop = 4096;
 
-// order-preserving map of an fp32 score to uint32 (-0 first made +0)
+// keys of one (token, head): rows of whole 16-byte vectors
+__host__ __device__ __forceinline__ int64_t key_stride(int n_blocks) { return (int64_t(n_blocks) + 3) & ~int64_t(3); }
+
+// order-preserving map of an fp32 score to uint32 (-0 first made +0); never 0, which stands for
+// no key
 __device__ __forceinline__ uint32_t order_key(float f) {
   const uint32_t b = __float_as_uint(f + 0.0f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return max((b & 0x80000000u) ? ~b : (b | 0x80000000u), 1u);
 }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -141,85 +145,160 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
       for (int w = 0; w < WORDS; ++w) a[i][w] = __ldg(reinterpret_cast<const uint4*>(dig + row * 2 * HD + qd * CH) + w);
       sc[i] = __ldg(dig_scale + row);
     }
-    for (int t = 0; t < n_tok; ++t) {
-      if (b0 >= s_nb[t]) continue;  // nothing of this tile is visible to the token
-      float best[2] = {-INFINITY, -INFINITY};
+    // two tokens at a time: independent chains of mma and reductions
+    for (int t = 0; t < n_tok; t += 2) {
+      const bool see[2] = {b0 < s_nb[t], t + 1 < n_tok && b0 < s_nb[t + 1]};
+      if (!see[0] && !see[1]) continue;  // nothing of this tile is visible to the tokens
+      const int tt[2] = {t, min(t + 1, n_tok - 1)};
+      float best[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) best[u][0] = best[u][1] = -INFINITY;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        int c[4] = {0, 0, 0, 0};
-        const uint8_t* row = s_code + ((t * NT + nt) * 8 + gr) * RS + qd * CS;
+        int c[2][4] = {};
 #pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-          const uint4 b = *reinterpret_cast<const uint4*>(row + 16 * w);
-          mma_s8(c, a[0][w].x, a[1][w].x, a[0][w].y, a[1][w].y, b.x, b.y);
-          mma_s8(c, a[0][w].z, a[1][w].z, a[0][w].w, a[1][w].w, b.z, b.w);
-        }
-        const float* am = s_amax + (t * NT + nt) * 8 + 2 * qd;
+        for (int w = 0; w < WORDS; ++w)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (nt * 8 + 2 * qd + e < G) {
-            best[0] = fmaxf(best[0], __fmul_rn(float(c[e]), am[e]));
-            best[1] = fmaxf(best[1], __fmul_rn(float(c[2 + e]), am[e]));
+          for (int u = 0; u < 2; ++u) {
+            const uint4 b = *reinterpret_cast<const uint4*>(s_code + ((tt[u] * NT + nt) * 8 + gr) * RS + qd * CS + 16 * w);
+            mma_s8(c[u], a[0][w].x, a[1][w].x, a[0][w].y, a[1][w].y, b.x, b.y);
+            mma_s8(c[u], a[0][w].z, a[1][w].z, a[0][w].w, a[1][w].w, b.z, b.w);
           }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float* am = s_amax + (tt[u] * NT + nt) * 8 + 2 * qd;
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (nt * 8 + 2 * qd + e < G) {
+              best[u][0] = fmaxf(best[u][0], __fmul_rn(float(c[u][e]), am[e]));
+              best[u][1] = fmaxf(best[u][1], __fmul_rn(float(c[u][2 + e]), am[e]));
+            }
+        }
       }
 #pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        best[0] = fmaxf(best[0], __shfl_xor_sync(0xffffffffu, best[0], o));
-        best[1] = fmaxf(best[1], __shfl_xor_sync(0xffffffffu, best[1], o));
-      }
-      if (qd < 2) {
-        const int b = b0 + gr + 8 * qd;
-        if (b < n_blocks)
-          keys[(int64_t(t0 - t_begin + t) * Hk + hk) * n_blocks + b] = order_key(__fmul_rn(best[qd], sc[qd]));
-      }
+      for (int o = 1; o < 4; o <<= 1)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) best[u][e] = fmaxf(best[u][e], __shfl_xor_sync(0xffffffffu, best[u][e], o));
+      // lane qd = 2u + e writes token u's key of block b0 + gr + 8e
+      const int u = qd >> 1, b = b0 + gr + 8 * (qd & 1);
+      const float top = qd == 0 ? best[0][0] : qd == 1 ? best[0][1] : qd == 2 ? best[1][0] : best[1][1];
+      if ((u ? see[1] : see[0]) && b < n_blocks)
+        keys[(int64_t(t0 - t_begin + t + u) * Hk + hk) * key_stride(n_blocks) + b] =
+            order_key(__fmul_rn(top, (qd & 1) ? sc[1] : sc[0]));
     }
   }
 }
 
 struct TopArgs {
-  const uint32_t* keys;  // [m][Hk][n_blocks], tokens from t_begin on
+  const uint32_t* keys;  // [m][Hk][key_stride(n_blocks)], tokens from t_begin on
   const int32_t* positions;
   int32_t* out;  // [..][Hk][top]
   int m, t_begin, Hk, n_ctx, n_blocks, top, sink, recent;
 };
 
-// count over the group (a warp, or the CTA: partial sums alternate between two shared rows,
-// so one barrier per count is enough)
+// Sums over the group (a warp, or the CTA: partial sums alternate between two shared rows, so
+// one barrier per sum is enough).
 template <int T>
-__device__ __forceinline__ int group_sum(int v, int (*s_part)[32], int& flip) {
-  v = __reduce_add_sync(0xffffffffu, v);
+__device__ __forceinline__ int2 group_sum(int2 v, int2 (*s_part)[32], int& flip) {
+  v.x = __reduce_add_sync(0xffffffffu, v.x);
+  v.y = __reduce_add_sync(0xffffffffu, v.y);
   if constexpr (T > 32) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int* row = s_part[flip];
+    int2* row = s_part[flip];
     flip ^= 1;
     if (lane == 0) row[warp] = v;
     __syncthreads();
-    v = __reduce_add_sync(0xffffffffu, lane < T / 32 ? row[lane] : 0);
+    v = lane < T / 32 ? row[lane] : make_int2(0, 0);
+    v.x = __reduce_add_sync(0xffffffffu, v.x);
+    v.y = __reduce_add_sync(0xffffffffu, v.y);
   }
   return v;
 }
 
+// The largest value that at least `need` of the group's values reach (0: absent; at least
+// `need` are present), built two bits at a time from the first bit in which they differ, by
+// counting the values at or above three trial values: no atomics, an order that never varies.
+// Stops as soon as a trial value is reached by exactly `need` values (then true).
+template <int T, int N>
+__device__ __forceinline__ bool kth_largest(const uint32_t (&v)[N], int n, int need, uint32_t& thr, int2 (*s_part)[32],
+                                            int (*s_mm)[32], int& flip) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t hi_v = 0, lo_v = 0xffffffffu;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < n && v[i] != 0) {
+      hi_v = max(hi_v, v[i]);
+      lo_v = min(lo_v, v[i]);
+    }
+  hi_v = __reduce_max_sync(0xffffffffu, hi_v);
+  lo_v = __reduce_min_sync(0xffffffffu, lo_v);
+  if constexpr (T > 32) {
+    __syncthreads();
+    if (lane == 0) {
+      s_mm[0][warp] = int(hi_v);
+      s_mm[1][warp] = int(lo_v);
+    }
+    __syncthreads();
+    hi_v = __reduce_max_sync(0xffffffffu, lane < T / 32 ? uint32_t(s_mm[0][lane]) : 0u);
+    lo_v = __reduce_min_sync(0xffffffffu, lane < T / 32 ? uint32_t(s_mm[1][lane]) : 0xffffffffu);
+  }
+  if (hi_v == lo_v) {
+    thr = hi_v;
+    return false;
+  }
+  const int low0 = (31 - __clz(hi_v ^ lo_v)) & ~1;  // the pair of bits that the first difference lies in
+  thr = low0 == 30 ? 0u : (hi_v >> (low0 + 2)) << (low0 + 2);
+  for (int low = low0; low >= 0; low -= 2) {
+    const uint32_t t1 = thr | (1u << low), t2 = thr | (2u << low), t3 = thr | (3u << low);
+    int c1 = 0, c2 = 0, c3 = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) {
+        c1 += v[i] >= t1;
+        c2 += v[i] >= t2;
+        c3 += v[i] >= t3;
+      }
+    const int2 c = group_sum<T>(make_int2(c1 | (c2 << 16), c3), s_part, flip);
+    c1 = c.x & 0xffff, c2 = int(uint32_t(c.x) >> 16), c3 = c.y;
+    int reached = -1;
+    if (c3 >= need) thr = t3, reached = c3;
+    else if (c2 >= need) thr = t2, reached = c2;
+    else if (c1 >= need) thr = t1, reached = c1;
+    if (reached == need) return true;
+  }
+  return false;
+}
+
 // The `top` blocks of one (token, head): T threads, thread t holding the KPT consecutive
-// keys from t * KPT on (KPT = 0: the keys stay in shared memory, any number of them).  The
-// K-th largest key is built bit by bit from the top by counting the keys at or above a
-// trial value: no atomics, an order that never varies, and it stops as soon as a trial value
-// is reached by exactly K keys.
+// keys from t * KPT on.  The K-th largest key is searched among few values: the K-th largest
+// of the maxima of groups of four keys is a lower bound for it that few more than K keys
+// reach; those are gathered and searched.  Only where that does not apply (fewer groups than
+// K, or too many keys at or above the bound, which takes ties) every key is counted.
 template <int T, int KPT>
 __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __grid_constant__ TopArgs a) {
   constexpr int kGroups = T > 32 ? 1 : 8;  // (token, head) pairs per CTA
-  extern __shared__ uint32_t s_keys[];
-  __shared__ int s_part[2][32];
-  __shared__ int s_scan[32];
-  __shared__ int s_scan2[32];
+  constexpr int kFew = T > 512 ? T : T > 32 ? 512 : 128;  // gathered keys at most
+  constexpr int GM = KPT / 4;
+  __shared__ int2 s_part[2][32];
+  __shared__ int s_mm[2][32];
+  __shared__ uint32_t s_few[kGroups][kFew];
+  __shared__ int s_count[kGroups];
   const int t = T > 32 ? int(threadIdx.x) : int(threadIdx.x & 31);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t id = int64_t(blockIdx.x) * kGroups + (T > 32 ? 0 : warp);
+  const int grp = T > 32 ? 0 : warp;
+  const int64_t id = int64_t(blockIdx.x) * kGroups + grp;
+  auto group_barrier = [] {
+    if constexpr (T > 32) __syncthreads();
+    else __syncwarp();
+  };
   pdl_wait();
   pdl_launch_next();
-  if (id >= int64_t(a.m) * a.Hk) return;
-  const int tok = a.t_begin + int(id / a.Hk), hk = int(id % a.Hk);
+  if (id >= int64_t(a.m) * a.Hk) return;  // the whole group
+  const int tok = a.t_begin + int(id / a.Hk);
   const int nb = (token_pos(a.positions, tok, a.n_ctx, false) + kBlk) / kBlk;
-  int32_t* out = a.out + (int64_t(tok) * a.Hk + hk) * a.top;
+  int32_t* out = a.out + (int64_t(tok) * a.Hk + id % a.Hk) * a.top;
   if (nb <= a.top) {  // every visible block
     for (int i = t; i < a.top; i += T) out[i] = i < nb ? i : -1;
     return;
@@ -227,110 +306,75 @@ __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __gri
   // candidates: blocks in [sink, nb - recent); the others are taken (below nb) or absent
   const int lo_b = a.sink, hi_b = nb - a.recent;
   const int need = a.top - a.sink - a.recent;
-  const uint32_t* keys = a.keys + id * a.n_blocks;
-  constexpr int R = KPT > 0 ? KPT : 1;
-  uint32_t k[R];
-  const int per = KPT > 0 ? KPT : (nb + T - 1) / T;
-  const int first = t * per;
-  uint32_t kmax = 0, kmin = 0xffffffffu;
-  if constexpr (KPT > 0) {
+  const uint32_t* keys = a.keys + id * key_stride(a.n_blocks);
+  const int first = t * KPT;
+  uint32_t k[KPT];
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      const int b = first + i;
-      const bool cand = b >= lo_b && b < hi_b;
-      k[i] = cand ? __ldcg(keys + b) : 0u;
-      if (cand) {
-        kmax = max(kmax, k[i]);
-        kmin = min(kmin, k[i]);
-      }
-    }
-  } else {
-    for (int b = t; b < nb; b += T) {
-      const bool cand = b >= lo_b && b < hi_b;
-      const uint32_t v = cand ? __ldcg(keys + b) : 0u;
-      s_keys[b] = v;
-      if (cand) {
-        kmax = max(kmax, v);
-        kmin = min(kmin, v);
-      }
-    }
-    __syncthreads();
+  for (int i = 0; i < KPT; i += 4) {
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (first + i < hi_b) x = __ldcg(reinterpret_cast<const uint4*>(keys + first + i));
+    k[i] = x.x, k[i + 1] = x.y, k[i + 2] = x.z, k[i + 3] = x.w;
   }
-  auto key_at = [&](int i) -> uint32_t {
-    if constexpr (KPT > 0) return k[i];
-    return first + i < nb ? s_keys[first + i] : 0u;
-  };
-  kmax = __reduce_max_sync(0xffffffffu, kmax);
-  kmin = __reduce_min_sync(0xffffffffu, kmin);
-  if constexpr (T > 32) {
-    if (lane == 0) {
-      s_scan[warp] = int(kmax);
-      s_scan2[warp] = int(kmin);
-    }
-    __syncthreads();
-    kmax = __reduce_max_sync(0xffffffffu, lane < T / 32 ? uint32_t(s_scan[lane]) : 0u);
-    kmin = __reduce_min_sync(0xffffffffu, lane < T / 32 ? uint32_t(s_scan2[lane]) : 0xffffffffu);
-    __syncthreads();
-  }
+#pragma unroll
+  for (int i = 0; i < KPT; ++i)
+    if (first + i < lo_b || first + i >= hi_b) k[i] = 0u;
+  if (t == 0) s_count[grp] = 0;
   int flip = 0;
-  uint32_t thr;        // keys above it are taken, and the first `ties` equal to it
+  uint32_t thr = 0xffffffffu;  // keys above it are taken, and the first `ties` equal to it
   int ties = 0;
   bool exact = false;  // every key at or above thr is taken
-  if (need <= 0) {
-    thr = 0xffffffffu;
-  } else {
-    const int top_bit = kmax == kmin ? -1 : 31 - __clz(kmax ^ kmin);
-    thr = top_bit < 0 ? kmax : (top_bit == 31 ? 0u : (kmax >> (top_bit + 1)) << (top_bit + 1));
-    for (int bit = top_bit; bit >= 0; --bit) {
-      const uint32_t trial = thr | (1u << bit);
-      int cnt = 0;
-      if constexpr (KPT > 0) {
+  if (need > 0) {
+    bool found = false;
+    if ((hi_b - lo_b) / 4 - 1 >= need) {  // at least `need` whole groups
+      uint32_t gm[GM], bound;
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) cnt += k[i] >= trial;
-      } else {
-        for (int i = 0; i < per; ++i) cnt += key_at(i) >= trial;
-      }
-      cnt = group_sum<T>(cnt, s_part, flip);
-      if (cnt >= need) {
-        thr = trial;
-        if (cnt == need) {
-          exact = true;
-          break;
+      for (int i = 0; i < GM; ++i) gm[i] = max(max(k[4 * i], k[4 * i + 1]), max(k[4 * i + 2], k[4 * i + 3]));
+      kth_largest<T, GM>(gm, GM, need, bound, s_part, s_mm, flip);
+      group_barrier();  // s_count is 0
+#pragma unroll
+      for (int i = 0; i < KPT; ++i)
+        if (k[i] >= bound) {
+          const int at = atomicAdd(&s_count[grp], 1);
+          if (at < kFew) s_few[grp][at] = k[i];
         }
-      }
-    }
-    if (!exact) {
-      int above = 0;
-      if constexpr (KPT > 0) {
+      group_barrier();
+      const int c = s_count[grp];
+      if (c <= kFew) {
+        uint32_t few[kFew / T];
 #pragma unroll
-        for (int i = 0; i < KPT; ++i) above += k[i] > thr;
-      } else {
-        for (int i = 0; i < per; ++i) above += key_at(i) > thr;
+        for (int i = 0; i < kFew / T; ++i) few[i] = t + i * T < c ? s_few[grp][t + i * T] : 0u;
+        exact = c == need;
+        thr = bound;
+        if (!exact) exact = kth_largest<T, kFew / T>(few, (c + T - 1) / T, need, thr, s_part, s_mm, flip);
+        found = true;
       }
-      ties = need - group_sum<T>(above, s_part, flip);
     }
+    if (!found) exact = kth_largest<T, KPT>(k, KPT, need, thr, s_part, s_mm, flip);
   }
-  // ascending output: taken blocks before this thread's, and equal keys before them
-  auto cand_at = [&](int i) { return first + i >= lo_b && first + i < hi_b; };
-  int n_sure = 0, n_tie = 0;
-  if constexpr (KPT > 0) {
+  // blocks taken for sure and blocks whose key equals thr, as bits of this thread's keys
+  uint32_t sure_m = 0, tie_m = 0;
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      const int b = first + i;
-      const bool c = cand_at(i);
-      n_sure += b < nb && (!c || (need > 0 && (exact ? k[i] >= thr : k[i] > thr)));
-      n_tie += c && !exact && need > 0 && k[i] == thr;
-    }
-  } else {
-    for (int i = 0; i < per; ++i) {
-      const int b = first + i;
-      const bool c = cand_at(i);
-      const uint32_t v = key_at(i);
-      n_sure += b < nb && (!c || (need > 0 && (exact ? v >= thr : v > thr)));
-      n_tie += c && !exact && need > 0 && v == thr;
-    }
+  for (int i = 0; i < KPT; ++i) {
+    if (k[i] > thr) sure_m |= 1u << i;
+    if (k[i] == thr) tie_m |= 1u << i;
+  }
+  if (need <= 0) sure_m = tie_m = 0;
+  if (exact) sure_m |= tie_m, tie_m = 0;
+  // the first `sink` blocks and the last `recent` visible ones (their keys are 0)
+  auto below = [&](int end) -> uint32_t {  // bits of this thread's blocks below `end`
+    const int n = max(0, min(KPT, end - first));
+    return n >= 32 ? 0xffffffffu : (1u << n) - 1;
+  };
+  const uint32_t forced = below(lo_b) | (below(nb) & ~below(hi_b));
+  sure_m = (sure_m & ~forced) | forced;
+  tie_m &= ~forced;
+  int above = 0;
+  if (!exact && need > 0) {
+    above = group_sum<T>(make_int2(__popc(sure_m & ~forced), 0), s_part, flip).x;
+    ties = need - above;
   }
   // exclusive scans of both counts over the threads
+  const int n_sure = __popc(sure_m), n_tie = __popc(tie_m);
   int sure = n_sure, tie = n_tie;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -340,37 +384,30 @@ __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __gri
       tie += y;
     }
   }
-  int sure_base = 0, tie_base = 0;
   if constexpr (T > 32) {
+    __syncthreads();  // s_mm was last read before the counts
     if (lane == 31) {
-      s_scan[warp] = sure;
-      s_scan2[warp] = tie;
+      s_mm[0][warp] = sure;
+      s_mm[1][warp] = tie;
     }
     __syncthreads();
-    sure_base = __reduce_add_sync(0xffffffffu, lane < warp ? s_scan[lane] : 0);
-    tie_base = __reduce_add_sync(0xffffffffu, lane < warp ? s_scan2[lane] : 0);
+    sure += __reduce_add_sync(0xffffffffu, lane < warp ? s_mm[0][lane] : 0);
+    tie += __reduce_add_sync(0xffffffffu, lane < warp ? s_mm[1][lane] : 0);
   }
-  sure += sure_base - n_sure;  // taken for sure, before this thread's keys
-  tie += tie_base - n_tie;     // ties before them
-  auto emit = [&](int i, uint32_t v) {
-    const int b = first + i;
-    if (b >= nb) return;
-    const bool c = cand_at(i);
-    bool take = !c || (need > 0 && (exact ? v >= thr : v > thr));
-    int at = sure + min(tie, ties);
-    if (c && !exact && need > 0 && v == thr) {
+  sure -= n_sure;  // taken for sure, before this thread's blocks
+  tie -= n_tie;    // ties before them
+  // ascending: a block's place is what was taken before it
+  for (uint32_t both = sure_m | tie_m; both != 0; both &= both - 1) {
+    const uint32_t bit = both & (0u - both);
+    bool take = true;
+    const int at = sure + min(tie, ties);
+    if (tie_m & bit) {
       take = tie < ties;
       ++tie;
-    } else if (take) {
+    } else {
       ++sure;
     }
-    if (take && at < a.top) out[at] = b;
-  };
-  if constexpr (KPT > 0) {
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) emit(i, k[i]);
-  } else {
-    for (int i = 0; i < per; ++i) emit(i, key_at(i));
+    if (take && at < a.top) out[at] = first + 31 - __clz(bit);
   }
 }
 
@@ -393,18 +430,14 @@ int launch_score(const uint16_t* q, const int8_t* dig, const float* dig_scale, c
 template <int T, int KPT>
 int launch_top(const TopArgs& a, cudaStream_t stream) {
   const int64_t ids = int64_t(a.m) * a.Hk;
-  const int smem = KPT > 0 ? 0 : a.n_blocks * 4;
-  auto kern = block_top_kernel<T, KPT>;
-  if (smem > 48 * 1024)
-    if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), smem)) return rc;
-  launch_pdl(kern, dim3(unsigned(T > 32 ? ids : (ids + 7) / 8)), dim3(T > 32 ? T : 256), size_t(smem), stream, a);
+  launch_pdl(block_top_kernel<T, KPT>, dim3(unsigned(T > 32 ? ids : (ids + 7) / 8)), dim3(T > 32 ? T : 256), 0, stream, a);
   CKV_LAUNCH_CHECK("ckv_block_select(top)");
   return CKV_OK;
 }
 
 // tokens whose keys the workspace holds at once: all of them, or as many as 256 MB take
 int64_t chunk_tokens(int m, int Hk, int n_blocks) {
-  const int64_t per = int64_t(Hk) * n_blocks * 4;
+  const int64_t per = int64_t(Hk) * key_stride(n_blocks) * 4;
   return std::min<int64_t>(m, std::max<int64_t>(kTok, (int64_t(256) << 20) / per / kTok * kTok));
 }
 
@@ -421,7 +454,7 @@ using namespace ckv;
 extern "C" int64_t ckv_block_select_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!select_shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
   const int nb = ceil_div(n_ctx, kBlk);
-  return chunk_tokens(m, n_kv_heads, nb) * n_kv_heads * nb * 4;
+  return chunk_tokens(m, n_kv_heads, nb) * n_kv_heads * key_stride(nb) * 4;
 }
 
 extern "C" int ckv_block_select_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
@@ -448,8 +481,9 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
   CKV_REQUIRE(aligned16(q) && aligned16(dig_codes) && aligned16(workspace), "ckv_block_select: tensors must be 16-byte aligned");
   const int nb = ceil_div(n_ctx, kBlk);
   const int64_t step = chunk_tokens(m, n_kv_heads, nb);
-  CKV_REQUIRE(workspace_bytes >= step * n_kv_heads * nb * 4, "ckv_block_select: workspace of %lld bytes, needs %lld",
-              static_cast<long long>(workspace_bytes), static_cast<long long>(step * n_kv_heads * nb * 4));
+  const int64_t need = step * n_kv_heads * key_stride(nb) * 4;
+  CKV_REQUIRE(workspace_bytes >= need, "ckv_block_select: workspace of %lld bytes, needs %lld",
+              static_cast<long long>(workspace_bytes), static_cast<long long>(need));
   CKV_REQUIRE(m <= 1048560 && int64_t(m) * n_kv_heads < (int64_t(1) << 31) - 8, "ckv_block_select: too many rows");
   const cudaStream_t s = as_stream(stream);
   uint32_t* keys = static_cast<uint32_t*>(workspace);
@@ -465,11 +499,12 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
                : launch_score<64, 1>(q, dig_codes, dig_scale, positions, n, int(t), n_q_heads, n_kv_heads, n_ctx, nb, keys, s);
     if (rc) return rc;
     const TopArgs a{keys, positions, blocks, n, int(t), n_kv_heads, n_ctx, nb, top, sink, recent};
-    // a warp per (token, head) while its keys fit the warp's registers, a CTA beyond
+    // a warp per (token, head) while its keys fit the warp's registers, then a CTA
     if (nb <= 512) rc = launch_top<32, 16>(a, s);
-    else if (nb <= 2048) rc = launch_top<256, 8>(a, s);
-    else if (nb <= 8192) rc = launch_top<1024, 8>(a, s);
-    else rc = launch_top<1024, 0>(a, s);
+    else if (nb <= 1024) rc = launch_top<32, 32>(a, s);
+    else if (nb <= 4096) rc = launch_top<256, 16>(a, s);
+    else if (nb <= 8192) rc = launch_top<256, 32>(a, s);
+    else rc = launch_top<1024, 32>(a, s);
     if (rc) return rc;
   }
   return CKV_OK;
