@@ -80,13 +80,18 @@ SIGNATURES: dict[str, list] = {
     "ckv_attention_blocks": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _p],
     "ckv_attention_blocks_kv8": [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p,
                                  _i64, _p],
+    "ckv_attention_sparse_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_sparse": [_p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _p,
+                             _i64, _p],
+    "ckv_attention_sparse_kv8": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                 _i32, _f32, _i32, _p, _i64, _p],
     "ckv_gemv": [_p, _p, _p, _i32, _i32, _i32, _p],
     "ckv_log_softmax": [_p, _i32, _p, _p],
     "ckv_greedy_next": [_p, _i32, _p, _p, _p],
 }
 _RESTYPES = {"ckv_version": C.c_char_p, "ckv_last_error": C.c_char_p, "ckv_attention_workspace_size": C.c_int64,
              "ckv_attention_kv8_workspace_size": C.c_int64, "ckv_block_select_workspace_size": C.c_int64,
-             "ckv_attention_blocks_workspace_size": C.c_int64}
+             "ckv_attention_blocks_workspace_size": C.c_int64, "ckv_attention_sparse_workspace_size": C.c_int64}
 
 CKV_OK, CKV_ERR_ARG, CKV_ERR_CUDA, CKV_ERR_DEVICE, CKV_ERR_UNSUPPORTED = range(5)
 DEV_ERR_BITS = {

@@ -803,6 +803,33 @@ int check(const char* name, const Args& a, int HD, int64_t tiles) {
   return CKV_OK;
 }
 
+// What ckv_attention_sparse(_kv8) needs: the selection's keys and the attention's partials, one
+// after the other in the same space, and behind them the digest when the call builds it.
+struct SparseSpace {
+  int64_t step, digest;
+  int64_t total() const { return step + digest; }
+};
+SparseSpace sparse_space(int m, int Hq, int Hk, int HD, int es, int n_ctx, int top, bool build) {
+  const int64_t sel = ckv_block_select_workspace_size(m, Hq, Hk, HD, n_ctx);
+  const int64_t att = plan(m, Hq / Hk, Hk, HD, es, top, true).bytes;
+  const int64_t nb = ceil_div(n_ctx, kBlk);
+  SparseSpace x;
+  x.step = (std::max(sel, att) + 15) / 16 * 16;
+  x.digest = build ? int64_t(Hk) * nb * (2 * HD + 4) : 0;
+  return x;
+}
+
+int check_space(const char* name, int m, int Hq, int Hk, int HD, int es, int n_ctx, int top, bool build, const void* workspace,
+                int64_t ws_bytes) {
+  CKV_REQUIRE(m >= 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && n_ctx > 0 && top > 0, "%s: bad sizes", name);
+  if (m == 0) return CKV_OK;
+  const int64_t need = sparse_space(m, Hq, Hk, HD, es, n_ctx, top, build).total();
+  CKV_REQUIRE(ws_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
+              "%s: workspace of %lld bytes, needs %lld (16-byte aligned)", name, static_cast<long long>(ws_bytes),
+              static_cast<long long>(need));
+  return CKV_OK;
+}
+
 }  // namespace
 
 // Few query rows over a whole 8-bit cache; used by ckv_attention_kv8 (attention_kv8.cu).
@@ -897,4 +924,52 @@ extern "C" int ckv_attention_blocks_kv8(const uint16_t* q, const uint8_t* k8, co
   const Args a{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, n_q_heads,
                n_kv_heads, n_ctx, nb, top, 1, 1, scale * 1.4426950408889634f};
   return attention_blocks("ckv_attention_blocks_kv8", a, head_dim, type, workspace, workspace_bytes, as_stream(stream));
+}
+
+extern "C" int64_t ckv_attention_sparse_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top,
+                                                       int cache_bits, int build_digest) {
+  if (m <= 0 || top <= 0 || !shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
+  return sparse_space(m, n_q_heads, n_kv_heads, head_dim, cache_bits / 8, n_ctx, top, build_digest != 0).total();
+}
+
+extern "C" int ckv_attention_sparse(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                    const int8_t* dig_codes, const float* dig_scale, const int32_t* positions, int32_t* blocks,
+                                    uint16_t* out, int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top, int sink,
+                                    int recent, float scale, void* workspace, int64_t workspace_bytes, ckv_stream_t stream) {
+  const bool build = dig_codes == nullptr;
+  CKV_REQUIRE(build == (dig_scale == nullptr), "ckv_attention_sparse: digest pointers");
+  if (int rc = check_space("ckv_attention_sparse", m, n_q_heads, n_kv_heads, head_dim, 2, n_ctx, top, build, workspace,
+                           workspace_bytes))
+    return rc;
+  if (m == 0) return CKV_OK;
+  const SparseSpace x = sparse_space(m, n_q_heads, n_kv_heads, head_dim, 2, n_ctx, top, build);
+  if (build) {
+    int8_t* codes = reinterpret_cast<int8_t*>(static_cast<uint8_t*>(workspace) + x.step);
+    float* scales = reinterpret_cast<float*>(codes + int64_t(n_kv_heads) * ceil_div(n_ctx, kBlk) * 2 * head_dim);
+    if (int rc = ckv_block_digest(k_cache, int64_t(n_ctx) * head_dim, head_dim, n_ctx, n_ctx, 0, nullptr, codes, scales, n_kv_heads,
+                                  head_dim, n_ctx, stream))
+      return rc;
+    dig_codes = codes, dig_scale = scales;
+  }
+  if (int rc = ckv_block_select(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
+                                recent, workspace, x.step, stream))
+    return rc;
+  return ckv_attention_blocks(q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, scale,
+                              workspace, x.step, stream);
+}
+
+extern "C" int ckv_attention_sparse_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                                        const float* v_scale, const int8_t* dig_codes, const float* dig_scale,
+                                        const int32_t* positions, int32_t* blocks, uint16_t* out, int m, int n_q_heads,
+                                        int n_kv_heads, int head_dim, int n_ctx, int top, int sink, int recent, float scale, int type,
+                                        void* workspace, int64_t workspace_bytes, ckv_stream_t stream) {
+  if (int rc = check_space("ckv_attention_sparse_kv8", m, n_q_heads, n_kv_heads, head_dim, 1, n_ctx, top, false, workspace,
+                           workspace_bytes))
+    return rc;
+  if (m == 0) return CKV_OK;
+  if (int rc = ckv_block_select(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
+                                recent, workspace, workspace_bytes, stream))
+    return rc;
+  return ckv_attention_blocks_kv8(q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx,
+                                  top, scale, type, workspace, workspace_bytes, stream);
 }

@@ -911,6 +911,14 @@ def _query(q: torch.Tensor, H: int, D: int, positions: torch.Tensor, m: int | No
     return m, Hq
 
 
+def _rows_out(q: torch.Tensor, m: int, width: int, out: torch.Tensor | None) -> torch.Tensor:
+    """The output rows: the caller's (checked), or new ones shaped as q's first m."""
+    if out is not None:
+        _buf("out", out, m * width)
+        return out
+    return torch.empty_like(q) if m == q.shape[0] else torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
+
+
 def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -940,10 +948,7 @@ def attention_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, out
     one must not overlap."""
     H, D = cache.n_kv_heads, cache.head_dim
     m, Hq = _query(q, H, D, positions, m)
-    if out is None:
-        out = torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
-    else:
-        _buf("out", out, m * Hq * D)
+    out = _rows_out(q, m, Hq * D, out)
     _on_device(q, positions, out, cache.k, workspace)
     lib = _lib.load()
     need = lib.ckv_attention_kv8_workspace_size(m, Hq, H, D, cache.n_ctx)
@@ -1000,10 +1005,7 @@ def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError("k_cache and v_cache differ in length")
     m, Hq = _query(q, H, D, positions, m)
     top = _blocks_arg(blocks, m, H)
-    if out is None:
-        out = torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
-    else:
-        _buf("out", out, m * Hq * D)
+    out = _rows_out(q, m, Hq * D, out)
     _on_device(q, k_cache, v_cache, positions, blocks, out)
     lib = _lib.load()
     ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top, 16), q.device)
@@ -1021,10 +1023,7 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     H, D = cache.n_kv_heads, cache.head_dim
     m, Hq = _query(q, H, D, positions, m)
     top = _blocks_arg(blocks, m, H)
-    if out is None:
-        out = torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
-    else:
-        _buf("out", out, m * Hq * D)
+    out = _rows_out(q, m, Hq * D, out)
     _on_device(q, positions, blocks, out, cache.k)
     lib = _lib.load()
     ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top, 8), q.device)
@@ -1036,32 +1035,71 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     return out
 
 
+def _sparse_kernels(lib, m: int, Hq: int, H: int, D: int, n_ctx: int, top: int, bits: int) -> int:
+    return (lib.ckv_block_select_launches(m, Hq, H, D, n_ctx)
+            + lib.ckv_attention_blocks_launches(m, Hq, H, D, top, bits))
+
+
 def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, top: int,
                      digest: BlockDigest | None = None, sink: int = 1, recent: int = 1,
-                     out: torch.Tensor | None = None, m: int | None = None,
+                     out: torch.Tensor | None = None, blocks: torch.Tensor | None = None, m: int | None = None,
                      scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Block-sparse attention over a bf16 cache: `block_select`, then `attention_blocks`; returns
     (out, blocks).  Without a `digest` that the caller keeps, the whole cache's is built first."""
     if k_cache.dim() != 3:
         raise ValueError(f"k_cache: expected shape (H, n_ctx, D), got {tuple(k_cache.shape)}")
     H, n_ctx, D = k_cache.shape
-    if digest is None:
-        nb = _n_blocks(n_ctx)
-        digest = BlockDigest.wrap(torch.empty((H, nb, 2, D), dtype=torch.int8, device=k_cache.device),
-                                  torch.empty((H, nb), dtype=torch.float32, device=k_cache.device), n_ctx)
-        block_digest(k_cache, digest)
-    elif digest.n_ctx != n_ctx or tuple(digest.codes.shape[::3]) != (H, D):
+    _cache("k_cache", k_cache, H, D)
+    _cache("v_cache", v_cache, H, D)
+    if v_cache.shape[1] != n_ctx:
+        raise ValueError("k_cache and v_cache differ in length")
+    m, Hq = _query(q, H, D, positions, m)
+    if digest is not None and (digest.n_ctx != n_ctx or tuple(digest.codes.shape[::3]) != (H, D)):
         raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache "
                          f"{tuple(k_cache.shape)}")
-    blocks = block_select(q, digest, positions, top, sink, recent, m=m)
-    return attention_blocks(q, k_cache, v_cache, positions, blocks, out=out, m=m, scale=scale), blocks
+    out, blocks = _sparse_out(q, m, Hq, H, D, top, out, blocks)
+    _on_device(q, k_cache, v_cache, positions, out, blocks, None if digest is None else digest.codes)
+    lib = _lib.load()
+    need = lib.ckv_attention_sparse_workspace_size(m, Hq, H, D, n_ctx, top, 16, int(digest is None))
+    ws = _scratch(need, q.device)
+    kernels = 1 if _TIMER is None else _sparse_kernels(lib, m, Hq, H, D, n_ctx, top, 16) + (digest is None)
+    _run("ckv_attention_sparse", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+         None if digest is None else digest.codes.data_ptr(), None if digest is None else digest.scale.data_ptr(),
+         positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, sink, recent,
+         1.0 / math.sqrt(D) if scale is None else float(scale), _ptr(ws), need, _stream(), kernels=kernels)
+    return out, blocks
+
+
+def _sparse_out(q, m: int, Hq: int, H: int, D: int, top: int, out, blocks):
+    """The output rows and block lists: the caller's, or new ones."""
+    if top < 1:
+        raise ValueError(f"top must be at least 1, got {top}")
+    out = _rows_out(q, m, Hq * D, out)
+    if blocks is None:
+        blocks = torch.empty((m, H, top), dtype=torch.int32, device=q.device)
+    else:
+        _buf("blocks", blocks, m * H * top, dtype=torch.int32)
+    return out, blocks
 
 
 def attention_sparse_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, top: int, sink: int = 1,
-                         recent: int = 1, out: torch.Tensor | None = None, m: int | None = None,
-                         scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                         recent: int = 1, out: torch.Tensor | None = None, blocks: torch.Tensor | None = None,
+                         m: int | None = None, scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """`attention_sparse` over an 8-bit cache that keeps its digest (``KV8Cache(digest=True)``)."""
-    if cache.digest is None:
+    dig = cache.digest
+    if dig is None:
         raise ValueError("attention_sparse_kv8: the cache keeps no digest (KV8Cache(..., digest=True))")
-    blocks = block_select(q, cache.digest, positions, top, sink, recent, m=m)
-    return attention_blocks_kv8(q, cache, positions, blocks, out=out, m=m, scale=scale), blocks
+    H, D = cache.n_kv_heads, cache.head_dim
+    m, Hq = _query(q, H, D, positions, m)
+    out, blocks = _sparse_out(q, m, Hq, H, D, top, out, blocks)
+    _on_device(q, positions, out, blocks, cache.k)
+    lib = _lib.load()
+    need = lib.ckv_attention_sparse_workspace_size(m, Hq, H, D, cache.n_ctx, top, 8, 0)
+    ws = _scratch(need, q.device)
+    kernels = 1 if _TIMER is None else _sparse_kernels(lib, m, Hq, H, D, cache.n_ctx, top, 8)
+    _run("ckv_attention_sparse_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+         cache.v_scale.data_ptr(), dig.codes.data_ptr(), dig.scale.data_ptr(), positions.data_ptr(),
+         blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx, top, sink, recent,
+         1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), need, _stream(),
+         kernels=kernels)
+    return out, blocks

@@ -448,6 +448,23 @@ CKV_API int ckv_attention_blocks_kv8(const uint16_t* q, const uint8_t* k8, const
                                      int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top, float scale,
                                      int type, void* workspace, int64_t workspace_bytes, ckv_stream_t stream);
 
+/* ckv_block_select, then attention over the lists it leaves in `blocks`, in one call; with
+ * dig_codes and dig_scale NULL the digest of the whole bf16 K cache is built first (in the
+ * workspace). */
+CKV_API int64_t ckv_attention_sparse_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx,
+                                                    int top, int cache_bits, int build_digest);
+CKV_API int ckv_attention_sparse(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                 const int8_t* dig_codes, const float* dig_scale, const int32_t* positions,
+                                 int32_t* blocks, uint16_t* out, int m, int n_q_heads, int n_kv_heads, int head_dim,
+                                 int n_ctx, int top, int sink, int recent, float scale, void* workspace,
+                                 int64_t workspace_bytes, ckv_stream_t stream);
+CKV_API int ckv_attention_sparse_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                                     const float* v_scale, const int8_t* dig_codes, const float* dig_scale,
+                                     const int32_t* positions, int32_t* blocks, uint16_t* out, int m, int n_q_heads,
+                                     int n_kv_heads, int head_dim, int n_ctx, int top, int sink, int recent,
+                                     float scale, int type, void* workspace, int64_t workspace_bytes,
+                                     ckv_stream_t stream);
+
 /* Small-m projection (lm_head on the logit rows, torch_engine.py:75-76,165):
  * out [m][n] = bf16(x [m][k] @ w[n][k]^T), m <= 8. */
 CKV_API int ckv_gemv(const uint16_t* x, const uint16_t* w, uint16_t* out, int m, int n, int k,
