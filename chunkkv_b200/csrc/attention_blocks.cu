@@ -708,6 +708,10 @@ struct Plan {
 // would be slower than all SMs with a second kernel for the join.
 constexpr int64_t kClusterBytes = 192 * 1024;
 
+// CTAs of clusters that surely run at once: eight to a GPC's SMs, one each (its shared memory is
+// taken by the rings); with 16 clusters the last waits for the others (15 us instead of 9).
+constexpr int kClusterCtas = 96;
+
 // Rows of one KV head in tiles of 8 (or 16).  With too few tiles to fill the SMs the blocks are
 // split: over the eight CTAs of a cluster while that moves few bytes per CTA (one launch, no
 // workspace), else over enough CTAs for three per SM, no finer than one block per warp.
@@ -720,7 +724,7 @@ Plan plan(int m, int G, int Hk, int HD, int es, int items, bool listed) {
   const int64_t cta_bytes = int64_t(items) * kBlk * HD * es * 2 / kCluster;
   p.splits = 1;
   p.join = false;
-  if (items > 4 && ctas * kCluster <= 2 * num_sms() && cta_bytes <= kClusterBytes) {
+  if (items > 4 && ctas * kCluster <= kClusterCtas && cta_bytes <= kClusterBytes) {
     p.splits = kCluster;
     p.join = true;
   } else {

@@ -1,7 +1,7 @@
 // Attention over the 8-bit K/V cache (one fp32 scale per KV head and block of 16 tokens).
 //
 // Few packed rows (token x head of a group) stream the cache through attention_blocks.cu;
-// from kTileRows rows on, the tcgen05 kernel below takes them in 128-row tiles.
+// past kStreamRows rows, the tcgen05 kernel below takes them in 128-row tiles.
 //
 // It is the bf16 kernel's scheme (attention_tc.cu: two Q tiles per CTA, S and P in TMEM,
 // lazy rescale, persistent items, key splits) with the operands made on the SM: a warpgroup
@@ -690,8 +690,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         uint8_t* stg8 = reinterpret_cast<uint8_t*>(stg);
         const int swz = (lane >> 2) & 1;
         int chunk = 0;
+        const bool rows_here = __any_sync(0xffffffffu, row.valid);  // a warp of padding rows stores nothing
 #pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
+        for (int c = 0; c < HD && rows_here; c += 32) {
           float o[32];
           tmem_ld32(obuf + c, o);
 #pragma unroll
@@ -769,10 +770,16 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   }
 }
 
-// Packed rows per KV head from which the tile kernel takes over.
-constexpr int kTileRows = 33;
+// Packed rows per KV head up to which attention_blocks.cu takes the call, 16 rows to a tile, each
+// streaming the cache.  At 28/4 heads, 56 rows (four tiles) take 15.8 / 35.8 / 116 us over 8192 /
+// 32,896 / 131,072 keys there and 30.8 / 49.2 / 134 us here; 84 rows 18.7 / 48.8 / 169 and
+// 31.8 / 49.4 / 134 us.
+constexpr int kStreamRows = 64;
+// A second launch for the join, in key-tile times.
+constexpr double kJoinCost = 3.0;
 
-bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) >= kTileRows; }
+bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) > kStreamRows; }
+SplitPlan tile_plan(int m, int Hq, int Hk, int HD, int n_ctx) { return plan_splits(m, Hq, Hk, HD, n_ctx, kJoinCost); }
 
 template <int HD, bool E4M3>
 int launch_tiles(Args a, const SplitPlan& p, void* workspace, cudaStream_t stream) {
@@ -828,14 +835,14 @@ using namespace ckv;
 
 extern "C" int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
-  return use_tiles(m, n_q_heads, n_kv_heads) ? kSchedBytes + plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
+  return use_tiles(m, n_q_heads, n_kv_heads) ? kSchedBytes + tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
                                              : kv8_stream_workspace(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
 extern "C" int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
   if (use_tiles(m, n_q_heads, n_kv_heads))
-    return plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx).max_splits > 1 ? 2 : 1;
+    return tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx).max_splits > 1 ? 2 : 1;
   return kv8_stream_launches(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
@@ -864,7 +871,7 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
                                 workspace, as_stream(stream));
   const Args a{q, k8, v8, k_scale, v_scale, positions, out, nullptr, nullptr, nullptr, m, n_q_heads, n_kv_heads, n_ctx,
                ceil_div(n_ctx, kBlk), 0, 0, 0, scale * 1.4426950408889634f};
-  const SplitPlan p = plan_splits(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
+  const SplitPlan p = tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
   const cudaStream_t s = as_stream(stream);
   if (head_dim == 128)
     return type == CKV_KV8_E4M3 ? launch_tiles<128, true>(a, p, workspace, s) : launch_tiles<128, false>(a, p, workspace, s);

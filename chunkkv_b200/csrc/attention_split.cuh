@@ -155,7 +155,7 @@ constexpr double kSplitItemCost = 1.0;
 // when split, the combine (reading every partial at the HBM rate: one tile time per
 // 14.3 MB).  Row block b is assumed to reach position (b + 1) / blocks * n_ctx (sorted
 // positions spread over the context, as the engine passes them).
-double plan_cost(int blocks, int Hk, int HD, int n_ctx, int tps, int sms) {
+double plan_cost(int blocks, int Hk, int HD, int n_ctx, int tps, int sms, double join_cost) {
   const bool split = tps < ceil_div(n_ctx, BN);
   const double cta_cost = kItemCost + (split ? kSplitItemCost : 0.0);
   double total = 0.0;
@@ -169,13 +169,14 @@ double plan_cost(int blocks, int Hk, int HD, int n_ctx, int tps, int sms) {
     max_item = std::max(max_item, std::min(kt, tps));
   }
   total *= Hk;
-  const double combine = split ? double(items_all) * Hk * NQ * BM * (HD * 4 + 8) / 14.3e6 : 0.0;
+  const double combine = split ? join_cost + double(items_all) * Hk * NQ * BM * (HD * 4 + 8) / 14.3e6 : 0.0;
   return total / sms + 0.5 * (max_item + cta_cost) + combine;
 }
 
 // Key-split plan: the tiles-per-split with the smallest estimated makespan (no split
 // included).  Plans are cached per shape.
-SplitPlan plan_splits(int M, int Hq, int Hk, int HD, int n_ctx) {
+// `join_cost`: what a second launch costs by itself, in key-tile times (one value per kernel).
+SplitPlan plan_splits(int M, int Hq, int Hk, int HD, int n_ctx, double join_cost = 0.0) {
   struct Key {
     int M, Hq, Hk, HD, n_ctx, sms;
   };
@@ -193,12 +194,12 @@ SplitPlan plan_splits(int M, int Hq, int Hk, int HD, int n_ctx) {
   SplitPlan p;
   p.blocks = ceil_div(M, NQ * T);
   const int max_kt = ceil_div(n_ctx, BN);
-  const double unsplit = plan_cost(p.blocks, Hk, HD, n_ctx, max_kt, sms);
+  const double unsplit = plan_cost(p.blocks, Hk, HD, n_ctx, max_kt, sms, join_cost);
   int best_tps = max_kt;
   double best = unsplit;
   // at most 32 splits: the combine gives each split one lane
   for (int tps = std::max(2, ceil_div(max_kt, 32)); tps < max_kt; tps = tps < 8 ? tps + 1 : tps + tps / 4) {
-    const double c = plan_cost(p.blocks, Hk, HD, n_ctx, tps, sms);
+    const double c = plan_cost(p.blocks, Hk, HD, n_ctx, tps, sms, join_cost);
     if (c < best) {
       best = c;
       best_tps = tps;
