@@ -720,7 +720,7 @@ Plan plan(int m, int G, int Hk, int HD, int es, int items, bool listed) {
   p.nt = (listed ? G : int64_t(m) * G) > 8 ? 2 : 1;
   p.head_tiles = listed ? ceil_div(G, 8 * p.nt) : 1;
   p.tiles = listed ? m * p.head_tiles : ceil_div(int64_t(m) * G, 8 * p.nt);
-  const int64_t ctas = int64_t(p.tiles) * Hk;
+  const int64_t ctas = std::max<int64_t>(1, int64_t(p.tiles) * Hk);
   const int64_t cta_bytes = int64_t(items) * kBlk * HD * es * 2 / kCluster;
   p.splits = 1;
   p.join = false;
@@ -874,10 +874,9 @@ extern "C" int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_head
 
 static int attention_blocks(const char* name, Args a, int HD, int type, void* workspace, int64_t ws_bytes, cudaStream_t s) {
   CKV_REQUIRE(a.top > 0, "%s: lists of %d blocks", name, a.top);
-  const bool sane = a.Hk > 0 && a.Hq > 0 && a.m >= 0;
-  const Plan p = sane ? plan(a.m, std::max(1, a.Hq / a.Hk), a.Hk, HD, type < 0 ? 2 : 1, a.top, true) : Plan{};
   if (int rc = check(name, a, HD, 0)) return rc;
   if (a.m == 0) return CKV_OK;
+  const Plan p = plan(a.m, a.Hq / a.Hk, a.Hk, HD, type < 0 ? 2 : 1, a.top, true);
   CKV_REQUIRE(a.blocks != nullptr, "%s: null block list", name);
   CKV_REQUIRE(ws_bytes >= p.bytes && (p.bytes == 0 || (workspace && aligned16(workspace))),
               "%s: workspace of %lld bytes, needs %lld (16-byte aligned)", name, static_cast<long long>(ws_bytes),

@@ -401,12 +401,24 @@ class TorchEngine:
 
     # -- decode ----------------------------------------------------------------
     @torch.inference_mode()
-    def generate(self, result: PrefillResult, max_tokens: int = 32) -> list[int]:
+    def generate(self, result: PrefillResult, max_tokens: int = 32, kv_dtype: torch.dtype | None = None,
+                 top_blocks: int | None = None) -> list[int]:
         """Greedy decode continuing a prefill (torch_engine.py:180-198), on the same kernels:
         the cache is sized once for the new tokens instead of a torch.cat per step.  The
         projections are the m = 1 GEMV kernels; the next token and the position stay on
         the device, and after the first step one decode step is replayed as a CUDA graph
-        (one-GPU engines), so the host only reads back each token id."""
+        (one-GPU engines), so the host only reads back each token id.
+
+        Two options the reference does not have, for long contexts.  `kv_dtype` (torch.int8 or
+        torch.float8_e4m3fn) holds the decode's K/V cache in 8 bits with one scale per KV head
+        and block of 16 tokens: half the memory and half the bytes a step reads.  `top_blocks`
+        lets every step attend only to that many blocks of 16 keys per KV head (the first block,
+        the one being written, and the others by score): what a step reads no longer grows with
+        the context, but for the score's block digests.  Either changes the logits."""
+        if kv_dtype is not None and kv_dtype not in ops.KV8_DTYPES:
+            raise NotImplementedError(f"kv_dtype {kv_dtype} is not supported (int8 and float8_e4m3fn are)")
+        if top_blocks is not None and top_blocks < 2:
+            raise ValueError(f"top_blocks must be at least 2 (the first and the current block), got {top_blocks}")
         s = self.shape
         L, H, Hq, D, hid = s.n_layers, s.n_kv, s.n_heads, s.head_dim, s.hidden
         dev = self.device
@@ -414,10 +426,24 @@ class TorchEngine:
             torch.cat(list(result.keys), 0), torch.cat(list(result.values), 0))
         pos = K0.shape[2]
         cap = pos + max(1, max_tokens)
-        K = torch.zeros((L, H, cap, D), dtype=torch.bfloat16, device=dev)
-        V = torch.zeros_like(K)
-        K[:, :, :pos].copy_(K0)
-        V[:, :, :pos].copy_(V0)
+        if kv_dtype is None:
+            K = torch.zeros((L, H, cap, D), dtype=torch.bfloat16, device=dev)
+            V = torch.zeros_like(K)
+            K[:, :, :pos].copy_(K0)
+            V[:, :, :pos].copy_(V0)
+            kv8 = None
+        else:
+            # the 8-bit caches, and one layer's worth of bf16 rows that every layer's projection
+            # writes its new row into (kv8_write takes it from there)
+            K = torch.zeros((1, H, cap, D), dtype=torch.bfloat16, device=dev).expand(L, -1, -1, -1)
+            V = torch.zeros((1, H, cap, D), dtype=torch.bfloat16, device=dev).expand(L, -1, -1, -1)
+            kv8 = [ops.KV8Cache(H, cap, D, kv_dtype, dev, digest=top_blocks is not None) for _ in range(L)]
+            for li, c in enumerate(kv8):
+                ops.kv8_write(c, K0[li].to(dev, torch.bfloat16), V0[li].to(dev, torch.bfloat16), 0)
+        digests = None
+        if top_blocks is not None and kv8 is None:
+            digests = [ops.block_digest(K[li], ops.BlockDigest(H, cap, D, dev), 0, pos) for li in range(L)]
+        blocks = None if top_blocks is None else torch.empty((1, H, top_blocks), dtype=torch.int32, device=dev)
         out: list[int] = []
         nxt = int(result.logits[-1].float().argmax().item())
         bf = dict(dtype=torch.bfloat16, device=dev)
@@ -438,6 +464,19 @@ class TorchEngine:
         rope_tab = self.rope_table(cap)
         attn_ws = self._attn_workspace(1, cap)
 
+        def attend(li):  # the new row's attention over layer li's cache, the row included
+            if kv8 is not None:
+                ops.kv8_write(kv8[li], K[li], V[li], posd, by_position=True)
+                if top_blocks is None:
+                    ops.attention_kv8(q, kv8[li], posd, out=attn)
+                else:
+                    ops.attention_sparse_kv8(q, kv8[li], posd, top_blocks, out=attn, blocks=blocks)
+            elif top_blocks is not None:
+                ops.block_digest(K[li], digests[li], posd)
+                ops.attention_sparse(q, K[li], V[li], posd, top_blocks, digest=digests[li], out=attn, blocks=blocks)
+            else:
+                ops.attention(q, K[li], V[li], posd, attn, m=1, workspace=attn_ws)
+
         def step():  # token tok at position posd -> next token in tok, posd + 1
             ops.embed(self.w.embed, tok, None, h)
             x_ready = False
@@ -451,7 +490,7 @@ class TorchEngine:
                     if not x_ready:
                         ops.rmsnorm(h, lw.ln1, s.rms_eps, out=x)
                     ops.gemv_qkv_rope(x, lw.w_qkv, lw.b_qkv, Hq, H, D, posd, rope_tab, q, K[li], V[li])
-                ops.attention(q, K[li], V[li], posd, attn, m=1, workspace=attn_ws)
+                attend(li)
                 x_ready = self._block_tail(li, attn, h, x, act, part, 1, exch, 0)
             last = x if x_ready else ops.rmsnorm(h, self.w.norm, s.rms_eps, out=xf)
             ops.gemv(last, self.w.lm_head, out=logits)

@@ -701,6 +701,7 @@ def log_softmax(row: torch.Tensor, out: torch.Tensor | None = None) -> torch.Ten
 
 # --------------------------------------------------------- K/V cache in 8 bits
 _KV8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # CKV_KV8_INT8, CKV_KV8_E4M3
+KV8_DTYPES = tuple(_KV8_TYPES)
 
 
 def _on_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
