@@ -23,7 +23,11 @@
 // Warps: 0..3 and 4..7 softmax / epilogue of Q tiles 0 and 1, 8..11 converters, 12 item
 // scheduler, 13 MMA issuer and TMEM owner, 14 and 15 idle.  The 512 threads start with 128
 // registers each; setmaxnreg moves them to the softmax warps (168 + 104 + 72: 65,536 in all).
+#include <algorithm>
+#include <functional>
+#include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "ckv_common.cuh"
 
@@ -775,11 +779,96 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
 // 32,896 / 131,072 keys there and 30.8 / 49.2 / 134 us here; 84 rows 18.7 / 48.8 / 169 and
 // 31.8 / 49.4 / 134 us.
 constexpr int kStreamRows = 64;
-// A second launch for the join, in key-tile times.
-constexpr double kJoinCost = 3.0;
-
 bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) > kStreamRows; }
-SplitPlan tile_plan(int m, int Hq, int Hk, int HD, int n_ctx) { return plan_splits(m, Hq, Hk, HD, n_ctx, kJoinCost); }
+
+// Costs in key-tile times (2.5 us at head_dim 128), fitted to the times of every split length at
+// eight shapes of 36 to 938 rows over 2048 to 32,896 keys (within 17 % of the best choice at
+// each): an item's start and epilogue, the same with fp32 partials, and the second launch that
+// joins them, alone, per split (a row's splits are added one after the other) and per byte.
+constexpr double kItemCost = 1.0, kSplitItemCost = 4.0, kJoinCost = 4.0, kJoinSplitCost = 0.3, kJoinBytes = 8e6;
+
+// Time of a plan: the items' makespan when the SMs take them in slot order (longest first),
+// followed exactly while they are few, for then it is the last wave that counts, and the join.
+// Row block b is assumed to reach position (b + 1) / blocks * n_ctx (rows spread over the
+// context) or n_ctx - m + (b + 1) * rows (the last m positions).
+double plan_cost(int m, int blocks, int Hk, int G, int HD, int n_ctx, int tps, int sms, bool spread) {
+  const int max_kt = ceil_div(n_ctx, BN);
+  const bool split = tps < max_kt;
+  const int max_splits = ceil_div(max_kt, tps);
+  const double fixed = split ? kSplitItemCost : kItemCost;
+  const int64_t rows = int64_t(NQ) * (BM / G);
+  int64_t items = 0;
+  double total = 0.0, makespan = 0.0;
+  std::vector<double> heap;  // the SMs' finishing times, earliest first
+  const bool follow = int64_t(blocks) * Hk * max_splits <= 4096;
+  if (follow) heap.assign(size_t(sms), 0.0);
+  for (int gi = 0; gi < max_splits; ++gi)
+    for (int b = blocks - 1; b >= 0; --b) {
+      const int64_t reach = spread ? (int64_t(b) + 1) * n_ctx / blocks
+                                   : std::max<int64_t>(1, n_ctx - m + std::min<int64_t>(m, (int64_t(b) + 1) * rows));
+      const int kt = std::max(1, ceil_div(reach, BN));
+      const int n_split = ceil_div(kt, tps);
+      const int z = n_split - max_splits + gi;
+      if (z < 0) continue;
+      const double c = std::min(tps, kt - z * tps) + fixed;
+      items += Hk;
+      total += c * Hk;
+      for (int h = 0; h < Hk && follow; ++h) {
+        std::pop_heap(heap.begin(), heap.end(), std::greater<double>());
+        heap.back() += c;
+        makespan = std::max(makespan, heap.back());
+        std::push_heap(heap.begin(), heap.end(), std::greater<double>());
+      }
+    }
+  if (!follow) makespan = total / sms + 0.5 * (tps + fixed);
+  const double join =
+      split ? kJoinCost + kJoinSplitCost * max_splits + double(items) * NQ * BM * (HD * 4 + 8) / kJoinBytes : 0.0;
+  return makespan + join;
+}
+
+// The tiles per split with the shortest time (no split included); kept per shape.
+SplitPlan tile_plan(int m, int Hq, int Hk, int HD, int n_ctx) {
+  struct Key {
+    int m, Hq, Hk, HD, n_ctx, sms;
+    bool operator==(const Key& o) const {
+      return m == o.m && Hq == o.Hq && Hk == o.Hk && HD == o.HD && n_ctx == o.n_ctx && sms == o.sms;
+    }
+  };
+  static std::mutex mu;
+  static std::vector<std::pair<Key, SplitPlan>> cache;
+  const int sms = num_sms();
+  const Key key{m, Hq, Hk, HD, n_ctx, sms};
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    for (const auto& e : cache)
+      if (e.first == key) return e.second;
+  }
+  SplitPlan p;
+  p.blocks = ceil_div(m, int64_t(NQ) * (BM / (Hq / Hk)));
+  const int max_kt = ceil_div(n_ctx, BN);
+  p.tps = max_kt;
+  // splitting only pays while whole rows do not fill the SMs several times over
+  if (int64_t(p.blocks) * Hk < 4 * int64_t(sms)) {
+    auto cost = [&](int tps) {
+      return plan_cost(m, p.blocks, Hk, Hq / Hk, HD, n_ctx, tps, sms, true) +
+             plan_cost(m, p.blocks, Hk, Hq / Hk, HD, n_ctx, tps, sms, false);
+    };
+    double best = cost(max_kt);
+    // at most 32 splits: the combine gives each split one lane
+    for (int tps = std::max(2, ceil_div(max_kt, 32)); tps < max_kt; tps = tps < 16 ? tps + 1 : tps + tps / 8) {
+      const double c = cost(tps);
+      if (c < best) {
+        best = c;
+        p.tps = tps;
+      }
+    }
+  }
+  p.max_splits = ceil_div(max_kt, p.tps);
+  p.bytes = p.max_splits > 1 ? int64_t(p.blocks) * Hk * p.max_splits * NQ * BM * (int64_t(HD) * 4 + 8) : 0;
+  std::lock_guard<std::mutex> lock(mu);
+  if (cache.size() < 256) cache.push_back({key, p});
+  return p;
+}
 
 template <int HD, bool E4M3>
 int launch_tiles(Args a, const SplitPlan& p, void* workspace, cudaStream_t stream) {

@@ -1,11 +1,7 @@
 // What the two tcgen05 attention kernels (attention_tc.cu over the bf16 cache,
-// attention_kv8.cu over the 8-bit one) share: tile sizes, work items, the key-split plan and
-// the kernel that merges the split partials.  Included after CKV_DEFINE_ERR_WORD.
+// attention_kv8.cu over the 8-bit one) share: tile sizes, work items, the shape of a
+// key-split plan and the kernel that merges the split partials.  Included after CKV_DEFINE_ERR_WORD.
 #pragma once
-
-#include <algorithm>
-#include <mutex>
-#include <vector>
 
 #include "ckv_common.cuh"
 
@@ -145,75 +141,6 @@ struct SplitPlan {
 // The workspace starts with the scheduler's two words (next slot, CTAs done), padded to
 // 256 bytes; the split partials follow.
 constexpr int64_t kSchedBytes = 256;
-// Fixed cost of one item, in key-tile times, for the persistent kernel: its first S
-// MMA and the epilogue are only partly hidden behind the neighbouring items; a split
-// item also writes its fp32 partial O.
-constexpr double kItemCost = 0.7;
-constexpr double kSplitItemCost = 1.0;
-// Estimated makespan, in key-tile times, of a split plan: the list-scheduling estimate
-// total work / SMs + half the largest item (items go out roughly largest first), plus,
-// when split, the combine (reading every partial at the HBM rate: one tile time per
-// 14.3 MB).  Row block b is assumed to reach position (b + 1) / blocks * n_ctx (sorted
-// positions spread over the context, as the engine passes them).
-double plan_cost(int blocks, int Hk, int HD, int n_ctx, int tps, int sms, double join_cost) {
-  const bool split = tps < ceil_div(n_ctx, BN);
-  const double cta_cost = kItemCost + (split ? kSplitItemCost : 0.0);
-  double total = 0.0;
-  int64_t items_all = 0;
-  int max_item = 0;
-  for (int b = 0; b < blocks; ++b) {
-    const int kt = std::max(1, ceil_div((int64_t(b) + 1) * n_ctx / blocks, BN));
-    const int items = ceil_div(kt, tps);
-    total += kt + items * cta_cost;
-    items_all += items;
-    max_item = std::max(max_item, std::min(kt, tps));
-  }
-  total *= Hk;
-  const double combine = split ? join_cost + double(items_all) * Hk * NQ * BM * (HD * 4 + 8) / 14.3e6 : 0.0;
-  return total / sms + 0.5 * (max_item + cta_cost) + combine;
-}
-
-// Key-split plan: the tiles-per-split with the smallest estimated makespan (no split
-// included).  Plans are cached per shape.
-// `join_cost`: what a second launch costs by itself, in key-tile times (one value per kernel).
-SplitPlan plan_splits(int M, int Hq, int Hk, int HD, int n_ctx, double join_cost = 0.0) {
-  struct Key {
-    int M, Hq, Hk, HD, n_ctx, sms;
-  };
-  static std::mutex mu;
-  static std::vector<std::pair<Key, SplitPlan>> cache;
-  const int sms = num_sms();
-  {
-    std::lock_guard<std::mutex> lock(mu);
-    for (const auto& e : cache)
-      if (e.first.M == M && e.first.Hq == Hq && e.first.Hk == Hk && e.first.HD == HD &&
-          e.first.n_ctx == n_ctx && e.first.sms == sms)
-        return e.second;
-  }
-  const int T = BM / (Hq / Hk);
-  SplitPlan p;
-  p.blocks = ceil_div(M, NQ * T);
-  const int max_kt = ceil_div(n_ctx, BN);
-  const double unsplit = plan_cost(p.blocks, Hk, HD, n_ctx, max_kt, sms, join_cost);
-  int best_tps = max_kt;
-  double best = unsplit;
-  // at most 32 splits: the combine gives each split one lane
-  for (int tps = std::max(2, ceil_div(max_kt, 32)); tps < max_kt; tps = tps < 8 ? tps + 1 : tps + tps / 4) {
-    const double c = plan_cost(p.blocks, Hk, HD, n_ctx, tps, sms, join_cost);
-    if (c < best) {
-      best = c;
-      best_tps = tps;
-    }
-  }
-  // split only when the estimate promises at least 10 %
-  if (best > 0.90 * unsplit) best_tps = max_kt;
-  p.tps = best_tps;
-  p.max_splits = ceil_div(max_kt, p.tps);
-  p.bytes = p.max_splits > 1 ? int64_t(p.blocks) * Hk * p.max_splits * NQ * BM * (int64_t(HD) * 4 + 8) : 0;
-  std::lock_guard<std::mutex> lock(mu);
-  if (cache.size() < 256) cache.push_back({Key{M, Hq, Hk, HD, n_ctx, sms}, p});
-  return p;
-}
 
 }  // namespace
 }  // namespace ckv
