@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   uint64_t* o_full = q_ready + NQ;    // [NQ]: the item's last P V of tile w is done
   uint64_t* item_full = o_full + NQ;  // [kItemSlots]
   uint64_t* item_empty = item_full + kItemSlots;  // [kItemSlots]
-  uint64_t* drain = item_empty + kItemSlots;
+  uint64_t* claim = item_empty + kItemSlots;  // the converters have begun the item's last tile
+  uint64_t* drain = claim + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -220,6 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
       mbar_init(&item_full[s], 1);
       mbar_init(&item_empty[s], 1 + NQ * 4 + 4);  // the MMA thread, each softmax and converter warp
     }
+    mbar_init(claim, 1);
     mbar_init(drain, 1);
     *abort = 0;
     fence_barrier_init();
@@ -245,6 +247,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         int pv[NQ * BM / 32];  // the item's token positions, lane + 32 j (clamped)
 #pragma unroll
         for (int j = 0; j < NQ * BM / 32; ++j) pv[j] = -1;
+        // one item ahead, no more: claimed when the converters begin the last tile of the item
+        // before (an SM that claims as many as its ring holds keeps them from idle ones: 938
+        // rows over 32,896 keys took 705 us instead of 373)
+        if (it > 0) {
+          const bool begun = warp_wait(claim, (it - 1) & 1, abort);
+          if (!begun) break;
+        }
         while (true) {
           int slot = cursor;
           if (a.sched != nullptr) {
@@ -449,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
       conv_barrier();  // s_red may be rewritten for the next item
       for (int j = 0; j < rec.n_kt; ++j) {
         const int gt = g + j, kt = rec.kt0 + j;
+        if (j + 1 == rec.n_kt && t == 0) mbar_arrive(claim);
         load(a.v, rec.hk, kt, last, y);
         float ks = 0.f, vs = 0.f;
         if (t < GRP && kt * BN + t * kBlk <= last) {
@@ -782,10 +792,10 @@ constexpr int kStreamRows = 64;
 bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) > kStreamRows; }
 
 // Costs in key-tile times (2.5 us at head_dim 128), fitted to the times of every split length at
-// eight shapes of 36 to 938 rows over 2048 to 32,896 keys (within 17 % of the best choice at
+// eight shapes of 36 to 938 rows over 2048 to 32,896 keys (within 5 % of the best choice at
 // each): an item's start and epilogue, the same with fp32 partials, and the second launch that
 // joins them, alone, per split (a row's splits are added one after the other) and per byte.
-constexpr double kItemCost = 1.0, kSplitItemCost = 4.0, kJoinCost = 4.0, kJoinSplitCost = 0.3, kJoinBytes = 8e6;
+constexpr double kItemCost = 0.5, kSplitItemCost = 3.0, kJoinCost = 1.0, kJoinSplitCost = 0.2, kJoinBytes = 5e6;
 
 // Time of a plan: the items' makespan when the SMs take them in slot order (longest first),
 // followed exactly while they are few, for then it is the last wave that counts, and the join.
