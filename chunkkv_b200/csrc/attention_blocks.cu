@@ -339,7 +339,9 @@ struct State {
 template <int HD, int CT, int NT, int W>
 struct Layout {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int STAGES = W > 8 ? 2 : 3;
+  // two stages where more CTAs (W = 4) or warps share the SM: at 938 rows of 64 listed blocks three
+  // CTAs of two stages take 255 us (bf16) and 183 us (8 bits), two of three 303 and 241 us
+  static constexpr int STAGES = W == 8 ? 3 : 2;
   static constexpr int RING = STAGES * Block<HD, CT>::STAGE;
   static constexpr int STRIDE = HD + 4;  // floats of a state row
   static constexpr int STATES = W * ROWS * (STRIDE + 2) * 4;
@@ -354,7 +356,7 @@ struct Layout {
 // JOIN: the kCluster splits of a tile are one cluster and leave finished rows; otherwise more
 // than one split leaves partials for attention_blocks_join_kernel.
 template <int HD, int CT, int NT, bool LISTED, int W, bool JOIN>
-__global__ void __launch_bounds__(W * 32, W > 4 ? 1 : (CT == kBf16 || NT == 2) ? 2 : 3)
+__global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     attention_blocks_kernel(const __grid_constant__ Args a) {
   using L = Layout<HD, CT, NT, W>;
   using B = Block<HD, CT>;

@@ -418,9 +418,10 @@ int launch_score(const uint16_t* q, const int8_t* dig, const float* dig_scale, c
   auto kern = block_score_kernel<HD, NT>;
   if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), smem)) return rc;
   const int groups = ceil_div(m, kTok);
-  // enough CTAs for about two per SM, no more than there are tiles
+  // about six CTAs per SM (early tokens see fewer blocks: the spare ones even that out), no more
+  // than there are tiles
   const int tiles = ceil_div(n_blocks, 16);
-  const int x = std::max(1, std::min(ceil_div(tiles, kScoreWarps), ceil_div(2 * num_sms(), int64_t(groups) * Hk)));
+  const int x = std::max(1, std::min(ceil_div(tiles, kScoreWarps), ceil_div(6 * num_sms(), int64_t(groups) * Hk)));
   launch_pdl(kern, dim3(x, groups, Hk), dim3(kScoreWarps * 32), smem, stream, q, dig, dig_scale, positions, m, t_begin, Hq,
              Hk, n_ctx, n_blocks, keys);
   CKV_LAUNCH_CHECK("ckv_block_select(score)");
@@ -499,10 +500,17 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
                : launch_score<64, 1>(q, dig_codes, dig_scale, positions, n, int(t), n_q_heads, n_kv_heads, n_ctx, nb, keys, s);
     if (rc) return rc;
     const TopArgs a{keys, positions, blocks, n, int(t), n_kv_heads, n_ctx, nb, top, sink, recent};
-    // a warp per (token, head) while its keys fit the warp's registers, then a CTA
-    if (nb <= 512) rc = launch_top<32, 16>(a, s);
+    // Few (token, head) pairs: a CTA each, its latency counts (one row over 16,384 / 32,896 tokens:
+    // 8.9 / 8.9 us with a warp or half the threads 10.7 / 10.1).  Many: a warp each while its
+    // keys fit the warp's registers, then 128 threads (938 rows over 32,896: 114 us, 256: 123).
+    if (int64_t(n) * n_kv_heads <= num_sms()) {
+      if (nb <= 1024) rc = launch_top<256, 4>(a, s);
+      else if (nb <= 4096) rc = launch_top<256, 16>(a, s);
+      else if (nb <= 8192) rc = launch_top<256, 32>(a, s);
+      else rc = launch_top<1024, 32>(a, s);
+    } else if (nb <= 512) rc = launch_top<32, 16>(a, s);
     else if (nb <= 1024) rc = launch_top<32, 32>(a, s);
-    else if (nb <= 4096) rc = launch_top<256, 16>(a, s);
+    else if (nb <= 4096) rc = launch_top<128, 32>(a, s);
     else if (nb <= 8192) rc = launch_top<256, 32>(a, s);
     else rc = launch_top<1024, 32>(a, s);
     if (rc) return rc;
