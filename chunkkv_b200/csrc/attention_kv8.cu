@@ -27,7 +27,6 @@
 #include <functional>
 #include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include "ckv_common.cuh"
 
@@ -797,6 +796,8 @@ bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) > kStreamR
 // joins them, alone, per split (a row's splits are added one after the other) and per byte.
 constexpr double kItemCost = 0.5, kSplitItemCost = 3.0, kJoinCost = 1.0, kJoinSplitCost = 0.2, kJoinBytes = 5e6;
 
+constexpr int kMaxSms = 256;
+
 // Time of a plan: the items' makespan when the SMs take them in slot order (longest first),
 // followed exactly while they are few, for then it is the last wave that counts, and the join.
 // Row block b is assumed to reach position (b + 1) / blocks * n_ctx (rows spread over the
@@ -809,9 +810,8 @@ double plan_cost(int m, int blocks, int Hk, int G, int HD, int n_ctx, int tps, i
   const int64_t rows = int64_t(NQ) * (BM / G);
   int64_t items = 0;
   double total = 0.0, makespan = 0.0;
-  std::vector<double> heap;  // the SMs' finishing times, earliest first
-  const bool follow = int64_t(blocks) * Hk * max_splits <= 4096;
-  if (follow) heap.assign(size_t(sms), 0.0);
+  double heap[kMaxSms] = {};  // the SMs' finishing times, earliest first
+  const bool follow = int64_t(blocks) * Hk * max_splits <= 6 * int64_t(sms);
   for (int gi = 0; gi < max_splits; ++gi)
     for (int b = blocks - 1; b >= 0; --b) {
       const int64_t reach = spread ? (int64_t(b) + 1) * n_ctx / blocks
@@ -824,48 +824,53 @@ double plan_cost(int m, int blocks, int Hk, int G, int HD, int n_ctx, int tps, i
       items += Hk;
       total += c * Hk;
       for (int h = 0; h < Hk && follow; ++h) {
-        std::pop_heap(heap.begin(), heap.end(), std::greater<double>());
-        heap.back() += c;
-        makespan = std::max(makespan, heap.back());
-        std::push_heap(heap.begin(), heap.end(), std::greater<double>());
+        std::pop_heap(heap, heap + sms, std::greater<double>());
+        heap[sms - 1] += c;
+        makespan = std::max(makespan, heap[sms - 1]);
+        std::push_heap(heap, heap + sms, std::greater<double>());
       }
     }
-  if (!follow) makespan = total / sms + 0.5 * (tps + fixed);
+  if (!follow) makespan = total / sms + 0.5 * (std::min(tps, max_kt) + fixed);
   const double join =
       split ? kJoinCost + kJoinSplitCost * max_splits + double(items) * NQ * BM * (HD * 4 + 8) / kJoinBytes : 0.0;
   return makespan + join;
 }
 
-// The tiles per split with the shortest time (no split included); kept per shape.
+// The number of splits with the shortest time over both assumptions (no split included).  Kept
+// per shape, the oldest forgotten (a plan takes up to 0.4 ms on the host).
 SplitPlan tile_plan(int m, int Hq, int Hk, int HD, int n_ctx) {
-  struct Key {
+  struct Entry {
     int m, Hq, Hk, HD, n_ctx, sms;
-    bool operator==(const Key& o) const {
-      return m == o.m && Hq == o.Hq && Hk == o.Hk && HD == o.HD && n_ctx == o.n_ctx && sms == o.sms;
-    }
+    SplitPlan plan;
   };
+  constexpr int kKept = 256;
   static std::mutex mu;
-  static std::vector<std::pair<Key, SplitPlan>> cache;
-  const int sms = num_sms();
-  const Key key{m, Hq, Hk, HD, n_ctx, sms};
+  static Entry kept[kKept];
+  static int n_kept = 0, oldest = 0;
+  const int sms = std::min(num_sms(), kMaxSms);
   {
     std::lock_guard<std::mutex> lock(mu);
-    for (const auto& e : cache)
-      if (e.first == key) return e.second;
+    for (int i = 0; i < n_kept; ++i) {
+      const Entry& e = kept[i];
+      if (e.m == m && e.Hq == Hq && e.Hk == Hk && e.HD == HD && e.n_ctx == n_ctx && e.sms == sms) return e.plan;
+    }
   }
   SplitPlan p;
   p.blocks = ceil_div(m, int64_t(NQ) * (BM / (Hq / Hk)));
   const int max_kt = ceil_div(n_ctx, BN);
   p.tps = max_kt;
-  // splitting only pays while whole rows do not fill the SMs several times over
-  if (int64_t(p.blocks) * Hk < 4 * int64_t(sms)) {
+  const int64_t whole = int64_t(p.blocks) * Hk;
+  // splitting only pays while whole rows do not fill the SMs several times over; at most 32
+  // splits (the combine gives each one lane)
+  if (whole < 4 * int64_t(sms)) {
     auto cost = [&](int tps) {
       return plan_cost(m, p.blocks, Hk, Hq / Hk, HD, n_ctx, tps, sms, true) +
              plan_cost(m, p.blocks, Hk, Hq / Hk, HD, n_ctx, tps, sms, false);
     };
     double best = cost(max_kt);
-    // at most 32 splits: the combine gives each split one lane
-    for (int tps = std::max(2, ceil_div(max_kt, 32)); tps < max_kt; tps = tps < 16 ? tps + 1 : tps + tps / 8) {
+    const int most = std::min(whole >= 2 * int64_t(sms) ? 4 : 32, max_kt / 2);
+    for (int n = 2; n <= most; n = n < 16 ? n + 1 : (n < most ? std::min(most, n + n / 4) : most + 1)) {
+      const int tps = ceil_div(max_kt, n);
       const double c = cost(tps);
       if (c < best) {
         best = c;
@@ -876,7 +881,8 @@ SplitPlan tile_plan(int m, int Hq, int Hk, int HD, int n_ctx) {
   p.max_splits = ceil_div(max_kt, p.tps);
   p.bytes = p.max_splits > 1 ? int64_t(p.blocks) * Hk * p.max_splits * NQ * BM * (int64_t(HD) * 4 + 8) : 0;
   std::lock_guard<std::mutex> lock(mu);
-  if (cache.size() < 256) cache.push_back({key, p});
+  const int at = n_kept < kKept ? n_kept++ : (oldest = (oldest + 1) % kKept);
+  kept[at] = {m, Hq, Hk, HD, n_ctx, sms, p};
   return p;
 }
 

@@ -485,7 +485,7 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
   const int64_t need = step * n_kv_heads * key_stride(nb) * 4;
   CKV_REQUIRE(workspace_bytes >= need, "ckv_block_select: workspace of %lld bytes, needs %lld",
               static_cast<long long>(workspace_bytes), static_cast<long long>(need));
-  CKV_REQUIRE(m <= 1048560 && int64_t(m) * n_kv_heads < (int64_t(1) << 31) - 8, "ckv_block_select: too many rows");
+  CKV_REQUIRE(m <= 1000000 && int64_t(m) * n_kv_heads < (int64_t(1) << 31) - 8, "ckv_block_select: too many rows");
   const cudaStream_t s = as_stream(stream);
   uint32_t* keys = static_cast<uint32_t*>(workspace);
   for (int64_t t = 0; t < m; t += step) {

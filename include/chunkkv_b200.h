@@ -406,7 +406,9 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
 
 /* ckv_attention over the 8-bit cache: q/out [m][Hq][D] bf16, key j visible to row i iff
  * j <= positions[i]; a row whose position is negative sees no key and gives zeros, one at or
- * past n_ctx sees every key (recorded).  At most 128 query heads per KV head, head_dim 64 or
+ * past n_ctx sees every key (recorded).  Codes and scales past every row's position may hold
+ * anything; those some row sees must be finite (ckv_kv8_write leaves no other), for a weight of 0
+ * does not silence a NaN in a row that shares a tile.  At most 128 query heads per KV head, head_dim 64 or
  * 128.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
  * 0) needs no initialisation; calls that share one must not overlap on the GPU. */
 CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
