@@ -145,6 +145,56 @@ __device__ __forceinline__ void commit_lead(uint32_t lead, uint64_t* bar) {
 }
 __device__ __forceinline__ void conv_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
+// A warp's 32 rows (32 sub ..) of a Q tile as fp16, each times the power of two that puts its
+// largest value in [2^14, 2^15): exact down to 2^-38 of it.  `base`: the tile's first token and
+// head; n_tok tokens of it exist.  HD / 8 lanes read one row.  Returns the inverse of the power
+// of this thread's row.  Not inlined: it runs once per item, and its registers stay out of the
+// softmax loop's.
+template <int HD>
+__device__ __noinline__ float place_q_rows(const uint16_t* base, uint8_t* tile, int Hq, int G, int n_tok, int sub) {
+  constexpr int LPR = HD / 8, RPP = 32 / LPR, PASSES = 32 / RPP;  // lanes per row, rows per pass
+  const int lane = threadIdx.x & 31, ch = lane % LPR;
+  const uint32_t inv_g = (65536 + G - 1) / G;  // r / G for r < 128
+  constexpr int B = 4;  // passes whose loads are in flight together; the next ones under these
+  uint32_t mine = 127;
+  uint4 z[B], y[B];
+  auto load = [&](int p0, uint4(&x)[B]) {
+#pragma unroll
+    for (int p = 0; p < B; ++p) {
+      const int rr = sub * 32 + (p0 + p) * RPP + lane / LPR, tq = int((uint32_t(rr) * inv_g) >> 16);
+      x[p] = p0 < PASSES && tq < n_tok
+                 ? __ldg(reinterpret_cast<const uint4*>(base + (int64_t(tq) * Hq + (rr - tq * G)) * HD) + ch)
+                 : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  load(0, z);
+  // rolled: the code runs once per item, and most of it would be instruction fetches
+#pragma unroll 1
+  for (int p0 = 0; p0 < PASSES; p0 += B) {
+    load(p0 + B, y);
+#pragma unroll
+    for (int p = 0; p < B; ++p) {
+      const uint32_t mg = __vmaxu2(__vmaxu2(z[p].x & 0x7fff7fffu, z[p].y & 0x7fff7fffu),
+                                   __vmaxu2(z[p].z & 0x7fff7fffu, z[p].w & 0x7fff7fffu));
+      uint32_t am = max(mg & 0xffffu, mg >> 16);
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, o));
+      const int sh = am == 0 ? 0 : max(-126, min(126, 14 + 127 - int(am >> 7)));
+      const float up = __uint_as_float(uint32_t(sh + 127) << 23);
+      const int rr = sub * 32 + (p0 + p) * RPP + lane / LPR;
+      *reinterpret_cast<uint4*>(tile + (ch >> 3) * ATOM_BYTES + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) =
+          make_uint4(pack_h2(lo_bf(z[p].x) * up, hi_bf(z[p].x) * up), pack_h2(lo_bf(z[p].y) * up, hi_bf(z[p].y) * up),
+                     pack_h2(lo_bf(z[p].z) * up, hi_bf(z[p].z) * up), pack_h2(lo_bf(z[p].w) * up, hi_bf(z[p].w) * up));
+      // the exponent goes to the lane that owns the row
+      const uint32_t e = __shfl_sync(0xffffffffu, uint32_t(127 - sh), (lane % RPP) * LPR);
+      if (lane / RPP == p0 + p) mine = e;
+    }
+#pragma unroll
+    for (int p = 0; p < B; ++p) z[p] = y[p];
+  }
+  return __uint_as_float(mine << 23);
+}
+
 struct Args {
   const uint16_t* q;
   const uint8_t *k, *v;
@@ -254,9 +304,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
           if (!begun) break;
         }
         while (true) {
+          // the first slot is the CTA's own; the counter hands out those behind
           int slot = cursor;
-          if (a.sched != nullptr) {
-            if (lane == 0) slot = int(atomicAdd(a.sched, 1u));
+          if (a.sched != nullptr && cursor != int(blockIdx.x)) {
+            if (lane == 0) slot = int(gridDim.x + atomicAdd(a.sched, 1u));
             slot = __shfl_sync(0xffffffffu, slot, 0);
           }
           cursor += gridDim.x;
@@ -518,32 +569,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
       if (lane == 0) mbar_arrive(&item_empty[s]);
       return true;
     };
-    // This thread's row of Q tile w as fp16 times the power of two that puts its largest value
-    // in [2^14, 2^15): exact down to 2^-38 of it.  Returns what undoes it in a score (log2
-    // domain).  The tile is free: the last S MMA that read it has been waited for.
-    auto place_q = [&](const Item& rec, const Row& x) -> float {
-      uint4 z[HD / 8];
-      const uint4* src = reinterpret_cast<const uint4*>(
-          a.q + (int64_t(rec.rb * NQ * T + w * T + tr) * a.Hq + rec.hk * G + (r - tr * G)) * HD);
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i) z[i] = x.valid ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-      uint32_t mg = 0;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i)
-        mg = __vmaxu2(mg, __vmaxu2(__vmaxu2(z[i].x & 0x7fff7fffu, z[i].y & 0x7fff7fffu),
-                                   __vmaxu2(z[i].z & 0x7fff7fffu, z[i].w & 0x7fff7fffu)));
-      const uint32_t am = max(mg & 0xffffu, mg >> 16);
-      const int sh = am == 0 ? 0 : max(-126, min(126, 14 + 127 - int(am >> 7)));
-      const float up = __uint_as_float(uint32_t(sh + 127) << 23);
-      uint8_t* row = sQ + w * C::Q_BYTES + r * 128;
-#pragma unroll
-      for (int i = 0; i < HD / 8; ++i)
-        *reinterpret_cast<uint4*>(row + (i >> 3) * ATOM_BYTES + (((i & 7) ^ (r & 7)) << 4)) =
-            make_uint4(pack_h2(lo_bf(z[i].x) * up, hi_bf(z[i].x) * up), pack_h2(lo_bf(z[i].y) * up, hi_bf(z[i].y) * up),
-                       pack_h2(lo_bf(z[i].z) * up, hi_bf(z[i].z) * up), pack_h2(lo_bf(z[i].w) * up, hi_bf(z[i].w) * up));
+    auto place_q = [&](const Item& rec) -> float {
+      const float f = place_q_rows<HD>(a.q + (int64_t(rec.rb * NQ * T + w * T) * a.Hq + rec.hk * G) * HD, sQ + w * C::Q_BYTES,
+                                       a.Hq, G, min(T, min(NQ * T, a.M - rec.rb * NQ * T) - w * T), sub);
       fence_async_smem();
       mbar_arrive(&q_ready[w]);
-      return a.scale_log2 * __uint_as_float(uint32_t(127 - sh) << 23);
+      return a.scale_log2 * f;
     };
 
     int g = 0;   // key tiles seen (all items): the scale slots
@@ -553,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
     Row row{false, 0};
     bool ok = take(0, cur, row);
     float factor = 0.f;
-    if (ok && cur.rb >= 0 && w < cur.pad1) factor = place_q(cur, row);
+    if (ok && cur.rb >= 0 && w < cur.pad1) factor = place_q(cur);
     for (int it = 0; ok && cur.rb >= 0; ++it) {
       float m = -INFINITY, l = 0.f, ref = 1.0f;
       const bool mine = w < cur.pad1;  // the item has rows on this tile
@@ -682,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
         break;
       }
       float nfactor = 0.f;
-      if (nxt.rb >= 0 && w < nxt.pad1) nfactor = place_q(nxt, nrow);
+      if (nxt.rb >= 0 && w < nxt.pad1) nfactor = place_q(nxt);
       if (!mine) {
         cur = nxt, row = nrow, factor = nfactor;
         continue;
