@@ -60,6 +60,45 @@ __device__ __forceinline__ int token_pos(const int32_t* positions, int t, int n_
   return p < 0 ? -1 : p;
 }
 
+// Codes of one query head (HD / 32 values per lane of the warp) into its row of shared memory,
+// the positive parts and, HD bytes on, the negative ones; returns the largest |q|.
+template <int HD>
+__device__ __forceinline__ float query_codes(const uint16_t* src, uint8_t* row, int lane) {
+  constexpr int CH = 2 * HD / 4, CS = CH + 16, E = HD / 32;
+  uint32_t pos = 0, neg = 0;
+  float amax = 0.f;
+  if (src != nullptr) {
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(src + lane * E + e);
+      f[e] = lo_bf(w);
+      f[e + 1] = hi_bf(w);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(f[e]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (amax < kTiny) amax = 0.f;
+    const float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = max(-127, min(127, __float2int_rn(__fmul_rn(f[e], inv))));
+      pos |= uint32_t(uint8_t(c > 0 ? c : 0)) << (8 * e);
+      neg |= uint32_t(uint8_t(c < 0 ? c : 0)) << (8 * e);
+    }
+  }
+  const int i = lane * E, j = HD + lane * E;  // byte offsets in the 2D-long row
+  if constexpr (E == 4) {
+    *reinterpret_cast<uint32_t*>(row + (i / CH) * CS + i % CH) = pos;
+    *reinterpret_cast<uint32_t*>(row + (j / CH) * CS + j % CH) = neg;
+  } else {
+    *reinterpret_cast<uint16_t*>(row + (i / CH) * CS + i % CH) = uint16_t(pos);
+    *reinterpret_cast<uint16_t*>(row + (j / CH) * CS + j % CH) = uint16_t(neg);
+  }
+  return amax;
+}
+
 // CTA: up to kTok tokens of one KV head against a strided set of 16-block tiles.  The
 // query codes are made once per CTA in shared memory; a warp then holds one tile's digest
 // rows in registers and runs every token of the CTA over them.  Row and chunk strides of
@@ -91,40 +130,8 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
   // query codes: a warp per (token, head) row, HD / 32 values per lane
   for (int r = warp; r < n_tok * NT * 8; r += kScoreWarps) {
     const int t = r / (NT * 8), g = r - t * (NT * 8);
-    constexpr int E = HD / 32;
-    uint32_t pos = 0, neg = 0;  // E codes, the positive and the negative part
-    float amax = 0.f;
-    if (g < G) {
-      const uint16_t* src = q + (int64_t(t0 + t) * Hq + hk * G + g) * HD + lane * E;
-      float f[E];
-#pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(src + e);
-        f[e] = lo_bf(w);
-        f[e + 1] = hi_bf(w);
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(f[e]));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (amax < kTiny) amax = 0.f;
-      const float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.0f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = max(-127, min(127, __float2int_rn(__fmul_rn(f[e], inv))));
-        pos |= uint32_t(uint8_t(c > 0 ? c : 0)) << (8 * e);
-        neg |= uint32_t(uint8_t(c < 0 ? c : 0)) << (8 * e);
-      }
-    }
-    uint8_t* row = s_code + r * RS;
-    const int i = lane * E, j = HD + lane * E;  // byte offsets in the 2D-long row
-    if constexpr (E == 4) {
-      *reinterpret_cast<uint32_t*>(row + (i / CH) * CS + i % CH) = pos;
-      *reinterpret_cast<uint32_t*>(row + (j / CH) * CS + j % CH) = neg;
-    } else {
-      *reinterpret_cast<uint16_t*>(row + (i / CH) * CS + i % CH) = uint16_t(pos);
-      *reinterpret_cast<uint16_t*>(row + (j / CH) * CS + j % CH) = uint16_t(neg);
-    }
+    const float amax =
+        query_codes<HD>(g < G ? q + (int64_t(t0 + t) * Hq + hk * G + g) * HD : nullptr, s_code + r * RS, lane);
     if (lane == 0) s_amax[r] = amax;
   }
   __syncthreads();
@@ -276,8 +283,9 @@ __device__ __forceinline__ bool kth_largest(const uint32_t (&v)[N], int n, int n
 // of the maxima of groups of four keys is a lower bound for it that few more than K keys
 // reach; those are gathered and searched.  Only where that does not apply (fewer groups than
 // K, or too many keys at or above the bound, which takes ties) every key is counted.
-template <int T, int KPT>
-__global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __grid_constant__ TopArgs a) {
+// `load(b)` gives the keys of blocks b .. b + 3.
+template <int T, int KPT, typename Load>
+__device__ __forceinline__ void select_top(const TopArgs& a, int nb, int32_t* out, Load load) {
   constexpr int kGroups = T > 32 ? 1 : 8;  // (token, head) pairs per CTA
   constexpr int kFew = T > 512 ? T : T > 32 ? 512 : 128;  // gathered keys at most
   constexpr int GM = KPT / 4;
@@ -288,17 +296,10 @@ __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __gri
   const int t = T > 32 ? int(threadIdx.x) : int(threadIdx.x & 31);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int grp = T > 32 ? 0 : warp;
-  const int64_t id = int64_t(blockIdx.x) * kGroups + grp;
   auto group_barrier = [] {
     if constexpr (T > 32) __syncthreads();
     else __syncwarp();
   };
-  pdl_wait();
-  pdl_launch_next();
-  if (id >= int64_t(a.m) * a.Hk) return;  // the whole group
-  const int tok = a.t_begin + int(id / a.Hk);
-  const int nb = (token_pos(a.positions, tok, a.n_ctx, false) + kBlk) / kBlk;
-  int32_t* out = a.out + (int64_t(tok) * a.Hk + id % a.Hk) * a.top;
   if (nb <= a.top) {  // every visible block
     for (int i = t; i < a.top; i += T) out[i] = i < nb ? i : -1;
     return;
@@ -306,13 +307,12 @@ __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __gri
   // candidates: blocks in [sink, nb - recent); the others are taken (below nb) or absent
   const int lo_b = a.sink, hi_b = nb - a.recent;
   const int need = a.top - a.sink - a.recent;
-  const uint32_t* keys = a.keys + id * key_stride(a.n_blocks);
   const int first = t * KPT;
   uint32_t k[KPT];
 #pragma unroll
   for (int i = 0; i < KPT; i += 4) {
     uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (first + i < hi_b) x = __ldcg(reinterpret_cast<const uint4*>(keys + first + i));
+    if (first + i < hi_b) x = load(first + i);
     k[i] = x.x, k[i + 1] = x.y, k[i + 2] = x.z, k[i + 3] = x.w;
   }
 #pragma unroll
@@ -411,6 +411,126 @@ __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __gri
   }
 }
 
+// A warp (T = 32) or a CTA per (token, head), its keys in the workspace.
+template <int T, int KPT>
+__global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __grid_constant__ TopArgs a) {
+  pdl_wait();
+  pdl_launch_next();
+  const int64_t id = T > 32 ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (id >= int64_t(a.m) * a.Hk) return;  // the whole group
+  const int tok = a.t_begin + int(id / a.Hk);
+  const int nb = (token_pos(a.positions, tok, a.n_ctx, false) + kBlk) / kBlk;
+  const uint32_t* keys = a.keys + id * key_stride(a.n_blocks);
+  select_top<T, KPT>(a, nb, a.out + (int64_t(tok) * a.Hk + id % a.Hk) * a.top,
+                     [&](int b) { return __ldcg(reinterpret_cast<const uint4*>(keys + b)); });
+}
+
+// Scores and selection of few (token, head) pairs in one launch: a cluster of kCluster CTAs
+// scores the blocks of one pair, every key going straight into the first CTA's shared memory,
+// and that CTA selects.
+constexpr int kCluster = 8;
+template <int HD, int NT, int KPT>
+__global__ void __launch_bounds__(256)
+    block_select_cluster_kernel(const uint16_t* __restrict__ q, const int8_t* __restrict__ dig, const float* __restrict__ dig_scale,
+                                int Hq, const __grid_constant__ TopArgs a) {
+  constexpr int CH = 2 * HD / 4, CS = CH + 16, RS = 4 * CS, WORDS = CH / 16;
+  __shared__ __align__(16) uint8_t s_code[NT * 8 * RS];
+  __shared__ float s_amax[NT * 8];
+  __shared__ __align__(16) uint32_t s_keys[256 * KPT];
+  const int G = Hq / a.Hk;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x, tok = blockIdx.y, hk = blockIdx.z;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has started
+  pdl_wait();
+  pdl_launch_next();
+  const int nb = (token_pos(a.positions, tok, a.n_ctx, hk == 0 && rank == 0) + kBlk) / kBlk;
+  const int gr = lane >> 2, qd = lane & 3;
+  const int tiles = (nb + 15) / 16;
+  const bool all = nb <= a.top;  // no choice to make
+  for (int g = warp; g < NT * 8; g += 8) {
+    const float amax = query_codes<HD>(g < G ? q + (int64_t(tok) * Hq + hk * G + g) * HD : nullptr, s_code + g * RS, lane);
+    if (lane == 0) s_amax[g] = amax;
+  }
+  __syncthreads();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // and so has the first one
+  const uint32_t keys0 = cluster_smem_addr(s_keys, 0);
+  for (int tile = rank * 8 + warp; tile < tiles && !all; tile += kCluster * 8) {
+    const int b0 = tile * 16;
+    uint4 d[2][WORDS];  // digest rows b0 + gr and b0 + gr + 8, this lane's chunk
+    float sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row = int64_t(hk) * a.n_blocks + min(b0 + gr + 8 * i, a.n_blocks - 1);
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) d[i][w] = __ldg(reinterpret_cast<const uint4*>(dig + row * 2 * HD + qd * CH) + w);
+      sc[i] = __ldg(dig_scale + row);
+    }
+    float best[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      int c[4] = {}, c2[4] = {};  // two chains
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        const uint4 b = *reinterpret_cast<const uint4*>(s_code + (nt * 8 + gr) * RS + qd * CS + 16 * w);
+        mma_s8(c, d[0][w].x, d[1][w].x, d[0][w].y, d[1][w].y, b.x, b.y);
+        mma_s8(c2, d[0][w].z, d[1][w].z, d[0][w].w, d[1][w].w, b.z, b.w);
+      }
+      const float* am = s_amax + nt * 8 + 2 * qd;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (nt * 8 + 2 * qd + e < G) {
+          best[0] = fmaxf(best[0], __fmul_rn(float(c[e] + c2[e]), am[e]));
+          best[1] = fmaxf(best[1], __fmul_rn(float(c[2 + e] + c2[2 + e]), am[e]));
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      best[0] = fmaxf(best[0], __shfl_xor_sync(0xffffffffu, best[0], o));
+      best[1] = fmaxf(best[1], __shfl_xor_sync(0xffffffffu, best[1], o));
+    }
+    if (qd < 2) {
+      const int b = b0 + gr + 8 * qd;
+      const uint32_t key = order_key(__fmul_rn(qd ? best[1] : best[0], qd ? sc[1] : sc[0]));
+      if (b < a.n_blocks) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(keys0 + 4u * b), "r"(key) : "memory");
+    }
+  }
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  if (rank != 0) return;
+  select_top<256, KPT>(a, nb, a.out + (int64_t(tok) * a.Hk + hk) * a.top,
+                       [&](int b) { return *reinterpret_cast<const uint4*>(s_keys + b); });
+}
+
+template <int HD, int NT, int KPT>
+int launch_cluster(const uint16_t* q, const int8_t* dig, const float* dig_scale, int Hq, const TopArgs& a, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kCluster, a.m, a.Hk);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kCluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, block_select_cluster_kernel<HD, NT, KPT>, q, dig, dig_scale, Hq, a);
+  CKV_LAUNCH_CHECK("ckv_block_select(cluster)");
+  return CKV_OK;
+}
+
+template <int HD, int NT>
+int launch_few(const uint16_t* q, const int8_t* dig, const float* dig_scale, int Hq, const TopArgs& a, cudaStream_t stream) {
+  if (a.n_blocks <= 1024) return launch_cluster<HD, NT, 4>(q, dig, dig_scale, Hq, a, stream);
+  return launch_cluster<HD, NT, 16>(q, dig, dig_scale, Hq, a, stream);
+}
+
+// Few pairs and contexts up to 65,536 tokens take one launch of clusters, and no workspace.  One row,
+// 4 heads: 6.2 / 8.7 / 10.0 us over 16,384 / 32,896 / 65,536 tokens against 7.6 / 8.9 / 8.9 us and a
+// launch more; over 131,072 tokens with 8 heads the clusters' 64 SMs take 20 us, two kernels 15.
+bool use_cluster(int m, int Hk, int n_blocks) { return int64_t(m) * Hk <= 32 && n_blocks <= 4096; }
+
 template <int HD, int NT>
 int launch_score(const uint16_t* q, const int8_t* dig, const float* dig_scale, const int32_t* positions, int m, int t_begin,
                  int Hq, int Hk, int n_ctx, int n_blocks, uint32_t* keys, cudaStream_t stream) {
@@ -455,11 +575,13 @@ using namespace ckv;
 extern "C" int64_t ckv_block_select_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!select_shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
   const int nb = ceil_div(n_ctx, kBlk);
+  if (m > 0 && use_cluster(m, n_kv_heads, nb)) return 0;
   return chunk_tokens(m, n_kv_heads, nb) * n_kv_heads * key_stride(nb) * 4;
 }
 
 extern "C" int ckv_block_select_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (m <= 0 || !select_shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
+  if (use_cluster(m, n_kv_heads, ceil_div(n_ctx, kBlk))) return 1;
   return 2 * ceil_div(m, chunk_tokens(m, n_kv_heads, ceil_div(n_ctx, kBlk)));
 }
 
@@ -478,9 +600,20 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
     return CKV_ERR_UNSUPPORTED;
   }
   if (m == 0) return CKV_OK;
-  CKV_REQUIRE(q && dig_codes && dig_scale && positions && blocks && workspace, "ckv_block_select: null pointer");
-  CKV_REQUIRE(aligned16(q) && aligned16(dig_codes) && aligned16(workspace), "ckv_block_select: tensors must be 16-byte aligned");
   const int nb = ceil_div(n_ctx, kBlk);
+  const bool few = use_cluster(m, n_kv_heads, nb);
+  CKV_REQUIRE(q && dig_codes && dig_scale && positions && blocks && (few || workspace), "ckv_block_select: null pointer");
+  CKV_REQUIRE(aligned16(q) && aligned16(dig_codes) && (few || aligned16(workspace)),
+              "ckv_block_select: tensors must be 16-byte aligned");
+  if (few) {
+    const TopArgs a{nullptr, positions, blocks, m, 0, n_kv_heads, n_ctx, nb, top, sink, recent};
+    const cudaStream_t s = as_stream(stream);
+    if (head_dim == 128)
+      return n_q_heads / n_kv_heads > 8 ? launch_few<128, 2>(q, dig_codes, dig_scale, n_q_heads, a, s)
+                                        : launch_few<128, 1>(q, dig_codes, dig_scale, n_q_heads, a, s);
+    return n_q_heads / n_kv_heads > 8 ? launch_few<64, 2>(q, dig_codes, dig_scale, n_q_heads, a, s)
+                                      : launch_few<64, 1>(q, dig_codes, dig_scale, n_q_heads, a, s);
+  }
   const int64_t step = chunk_tokens(m, n_kv_heads, nb);
   const int64_t need = step * n_kv_heads * key_stride(nb) * 4;
   CKV_REQUIRE(workspace_bytes >= need, "ckv_block_select: workspace of %lld bytes, needs %lld",
@@ -500,15 +633,9 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
                : launch_score<64, 1>(q, dig_codes, dig_scale, positions, n, int(t), n_q_heads, n_kv_heads, n_ctx, nb, keys, s);
     if (rc) return rc;
     const TopArgs a{keys, positions, blocks, n, int(t), n_kv_heads, n_ctx, nb, top, sink, recent};
-    // Few (token, head) pairs: a CTA each, its latency counts (one row over 16,384 / 32,896 tokens:
-    // 8.9 / 8.9 us with a warp or half the threads 10.7 / 10.1).  Many: a warp each while its
-    // keys fit the warp's registers, then 128 threads (938 rows over 32,896: 114 us, 256: 123).
-    if (int64_t(n) * n_kv_heads <= num_sms()) {
-      if (nb <= 1024) rc = launch_top<256, 4>(a, s);
-      else if (nb <= 4096) rc = launch_top<256, 16>(a, s);
-      else if (nb <= 8192) rc = launch_top<256, 32>(a, s);
-      else rc = launch_top<1024, 32>(a, s);
-    } else if (nb <= 512) rc = launch_top<32, 16>(a, s);
+    // a warp per (token, head) while its keys fit the warp's registers, then 128 threads (938 rows
+    // over 32,896 tokens: 114 us, with 256 threads 123) and more
+    if (nb <= 512) rc = launch_top<32, 16>(a, s);
     else if (nb <= 1024) rc = launch_top<32, 32>(a, s);
     else if (nb <= 4096) rc = launch_top<128, 32>(a, s);
     else if (nb <= 8192) rc = launch_top<256, 32>(a, s);

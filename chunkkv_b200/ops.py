@@ -6,6 +6,7 @@ kernels; nothing here computes on the host.  Tensors are bf16 unless noted.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -936,8 +937,16 @@ def _workspace_arg(workspace: torch.Tensor | None, need: int, device) -> tuple[t
     return workspace, nbytes
 
 
+@functools.lru_cache(maxsize=4096)
+def _size(name: str, dev: int, *shape: int) -> int:
+    """A workspace size of the library, remembered per shape (and device: plans go by its SMs)."""
+    return int(getattr(_lib.load(), name)(*shape))
+
+
 def attention_kv8_workspace_bytes(m: int, n_q_heads: int, n_kv_heads: int, head_dim: int, n_ctx: int) -> int:
-    return int(_lib.load().ckv_attention_kv8_workspace_size(m, n_q_heads, n_kv_heads, head_dim, n_ctx))
+    """Bytes of workspace of an `attention_kv8` call (0: none) on the current device."""
+    return _size("ckv_attention_kv8_workspace_size", torch.cuda.current_device(), m, n_q_heads, n_kv_heads, head_dim,
+                 n_ctx)
 
 
 def attention_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, out: torch.Tensor | None = None,
@@ -951,10 +960,9 @@ def attention_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, out
     m, Hq = _query(q, H, D, positions, m)
     out = _rows_out(q, m, Hq * D, out)
     _on_device(q, positions, out, cache.k, workspace)
-    lib = _lib.load()
-    need = lib.ckv_attention_kv8_workspace_size(m, Hq, H, D, cache.n_ctx)
+    need = _size("ckv_attention_kv8_workspace_size", q.get_device(), m, Hq, H, D, cache.n_ctx)
     workspace, nbytes = _workspace_arg(workspace, need, q.device)
-    kernels = 1 if _TIMER is None else lib.ckv_attention_kv8_launches(m, Hq, H, D, cache.n_ctx)
+    kernels = 1 if _TIMER is None else _lib.load().ckv_attention_kv8_launches(m, Hq, H, D, cache.n_ctx)
     _run("ckv_attention_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), positions.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
          1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(workspace), nbytes,
@@ -975,9 +983,9 @@ def block_select(q: torch.Tensor, digest: BlockDigest, positions: torch.Tensor, 
     else:
         _buf("out", out, m * H * top, dtype=torch.int32)
     _on_device(q, positions, out, digest.codes)
-    lib = _lib.load()
-    ws, nbytes = _workspace_arg(None, lib.ckv_block_select_workspace_size(m, Hq, H, D, digest.n_ctx), q.device)
-    kernels = 1 if _TIMER is None else lib.ckv_block_select_launches(m, Hq, H, D, digest.n_ctx)
+    need = _size("ckv_block_select_workspace_size", q.get_device(), m, Hq, H, D, digest.n_ctx)
+    ws, nbytes = _workspace_arg(None, need, q.device)
+    kernels = 1 if _TIMER is None else _lib.load().ckv_block_select_launches(m, Hq, H, D, digest.n_ctx)
     _run("ckv_block_select", q.data_ptr(), digest.codes.data_ptr(), digest.scale.data_ptr(), positions.data_ptr(),
          out.data_ptr(), m, Hq, H, D, digest.n_ctx, top, sink, recent, _ptr(ws), nbytes, _stream(), kernels=kernels)
     return out
@@ -1008,9 +1016,9 @@ def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
     _on_device(q, k_cache, v_cache, positions, blocks, out)
-    lib = _lib.load()
-    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top, 16), q.device)
-    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top, 16)
+    need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, top, 16)
+    ws, nbytes = _workspace_arg(None, need, q.device)
+    kernels = 1 if _TIMER is None else _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, top, 16)
     _run("ckv_attention_blocks", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
          blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, 1.0 / math.sqrt(D) if scale is None else float(scale),
          _ptr(ws), nbytes, _stream(), kernels=kernels)
@@ -1026,9 +1034,9 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
     _on_device(q, positions, blocks, out, cache.k)
-    lib = _lib.load()
-    ws, nbytes = _workspace_arg(None, lib.ckv_attention_blocks_workspace_size(m, Hq, H, D, top, 8), q.device)
-    kernels = 1 if _TIMER is None else lib.ckv_attention_blocks_launches(m, Hq, H, D, top, 8)
+    need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, top, 8)
+    ws, nbytes = _workspace_arg(None, need, q.device)
+    kernels = 1 if _TIMER is None else _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, top, 8)
     _run("ckv_attention_blocks_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
          top, 1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), nbytes,
@@ -1036,7 +1044,8 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     return out
 
 
-def _sparse_kernels(lib, m: int, Hq: int, H: int, D: int, n_ctx: int, top: int, bits: int) -> int:
+def _sparse_kernels(m: int, Hq: int, H: int, D: int, n_ctx: int, top: int, bits: int) -> int:
+    lib = _lib.load()
     return (lib.ckv_block_select_launches(m, Hq, H, D, n_ctx)
             + lib.ckv_attention_blocks_launches(m, Hq, H, D, top, bits))
 
@@ -1060,10 +1069,9 @@ def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                          f"{tuple(k_cache.shape)}")
     out, blocks = _sparse_out(q, m, Hq, H, D, top, out, blocks)
     _on_device(q, k_cache, v_cache, positions, out, blocks, None if digest is None else digest.codes)
-    lib = _lib.load()
-    need = lib.ckv_attention_sparse_workspace_size(m, Hq, H, D, n_ctx, top, 16, int(digest is None))
+    need = _size("ckv_attention_sparse_workspace_size", q.get_device(), m, Hq, H, D, n_ctx, top, 16, int(digest is None))
     ws = _scratch(need, q.device)
-    kernels = 1 if _TIMER is None else _sparse_kernels(lib, m, Hq, H, D, n_ctx, top, 16) + (digest is None)
+    kernels = 1 if _TIMER is None else _sparse_kernels(m, Hq, H, D, n_ctx, top, 16) + (digest is None)
     _run("ckv_attention_sparse", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
          None if digest is None else digest.codes.data_ptr(), None if digest is None else digest.scale.data_ptr(),
          positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, sink, recent,
@@ -1094,10 +1102,9 @@ def attention_sparse_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     m, Hq = _query(q, H, D, positions, m)
     out, blocks = _sparse_out(q, m, Hq, H, D, top, out, blocks)
     _on_device(q, positions, out, blocks, cache.k)
-    lib = _lib.load()
-    need = lib.ckv_attention_sparse_workspace_size(m, Hq, H, D, cache.n_ctx, top, 8, 0)
+    need = _size("ckv_attention_sparse_workspace_size", q.get_device(), m, Hq, H, D, cache.n_ctx, top, 8, 0)
     ws = _scratch(need, q.device)
-    kernels = 1 if _TIMER is None else _sparse_kernels(lib, m, Hq, H, D, cache.n_ctx, top, 8)
+    kernels = 1 if _TIMER is None else _sparse_kernels(m, Hq, H, D, cache.n_ctx, top, 8)
     _run("ckv_attention_sparse_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), dig.codes.data_ptr(), dig.scale.data_ptr(), positions.data_ptr(),
          blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx, top, sink, recent,

@@ -425,8 +425,8 @@ CKV_API int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uint8_
  * upper bound of q . k over the block from its digest and the query's 8-bit codes, the best
  * head of the group), equal scores to the lower block.  blocks [m][H][top] int32, ascending, -1
  * past a row's last visible block.  At most 16 query heads per KV head, contexts up to 524,288
- * tokens, sink + recent <= top <= 4096, recent >= 1.  The workspace (16-byte aligned) needs no
- * initialisation. */
+ * tokens, sink + recent <= top <= 4096, recent >= 1.  The workspace (16-byte aligned, 0
+ * bytes for few rows) needs no initialisation. */
 CKV_API int64_t ckv_block_select_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 CKV_API int ckv_block_select_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const float* dig_scale,
