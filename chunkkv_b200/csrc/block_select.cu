@@ -224,6 +224,28 @@ __device__ __forceinline__ int2 group_sum(int2 v, int2 (*s_part)[32], int& flip)
   return v;
 }
 
+// What the group's threads before this one hold together, and the whole sum.
+template <int T>
+__device__ __forceinline__ int exclusive_scan(int n, int (*s_mm)[32], int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = n;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  total = __shfl_sync(0xffffffffu, x, 31);
+  if constexpr (T > 32) {
+    __syncthreads();  // s_mm was last read before
+    if (lane == 31) s_mm[0][warp] = x;
+    __syncthreads();
+    const int v = lane < T / 32 ? s_mm[0][lane] : 0;
+    x += __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+    total = __reduce_add_sync(0xffffffffu, v);
+  }
+  return x - n;
+}
+
 // The largest value that at least `need` of the group's values reach (0: absent; at least
 // `need` are present), built two bits at a time from the first bit in which they differ, by
 // counting the values at or above three trial values: no atomics, an order that never varies.
@@ -292,10 +314,8 @@ __device__ __forceinline__ void select_top(const TopArgs& a, int nb, int32_t* ou
   __shared__ int2 s_part[2][32];
   __shared__ int s_mm[2][32];
   __shared__ uint32_t s_few[kGroups][kFew];
-  __shared__ int s_count[kGroups];
   const int t = T > 32 ? int(threadIdx.x) : int(threadIdx.x & 31);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int grp = T > 32 ? 0 : warp;
+  const int grp = T > 32 ? 0 : int(threadIdx.x >> 5);
   auto group_barrier = [] {
     if constexpr (T > 32) __syncthreads();
     else __syncwarp();
@@ -318,7 +338,6 @@ __device__ __forceinline__ void select_top(const TopArgs& a, int nb, int32_t* ou
 #pragma unroll
   for (int i = 0; i < KPT; ++i)
     if (first + i < lo_b || first + i >= hi_b) k[i] = 0u;
-  if (t == 0) s_count[grp] = 0;
   int flip = 0;
   uint32_t thr = 0xffffffffu;  // keys above it are taken, and the first `ties` equal to it
   int ties = 0;
@@ -330,15 +349,19 @@ __device__ __forceinline__ void select_top(const TopArgs& a, int nb, int32_t* ou
 #pragma unroll
       for (int i = 0; i < GM; ++i) gm[i] = max(max(k[4 * i], k[4 * i + 1]), max(k[4 * i + 2], k[4 * i + 3]));
       kth_largest<T, GM>(gm, GM, need, bound, s_part, s_mm, flip);
-      group_barrier();  // s_count is 0
+      uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < KPT; ++i)
-        if (k[i] >= bound) {
-          const int at = atomicAdd(&s_count[grp], 1);
+        if (k[i] >= bound) m |= 1u << i;
+      // places by a scan of the counts (atomics on one counter would queue up)
+      int c, at = exclusive_scan<T>(__popc(m), s_mm, c);
+#pragma unroll
+      for (int i = 0; i < KPT; ++i)
+        if ((m >> i) & 1) {
           if (at < kFew) s_few[grp][at] = k[i];
+          ++at;
         }
       group_barrier();
-      const int c = s_count[grp];
       if (c <= kFew) {
         uint32_t few[kFew / T];
 #pragma unroll
@@ -373,29 +396,10 @@ __device__ __forceinline__ void select_top(const TopArgs& a, int nb, int32_t* ou
     above = group_sum<T>(make_int2(__popc(sure_m & ~forced), 0), s_part, flip).x;
     ties = need - above;
   }
-  // exclusive scans of both counts over the threads
-  const int n_sure = __popc(sure_m), n_tie = __popc(tie_m);
-  int sure = n_sure, tie = n_tie;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, sure, o), y = __shfl_up_sync(0xffffffffu, tie, o);
-    if (lane >= o) {
-      sure += x;
-      tie += y;
-    }
-  }
-  if constexpr (T > 32) {
-    __syncthreads();  // s_mm was last read before the counts
-    if (lane == 31) {
-      s_mm[0][warp] = sure;
-      s_mm[1][warp] = tie;
-    }
-    __syncthreads();
-    sure += __reduce_add_sync(0xffffffffu, lane < warp ? s_mm[0][lane] : 0);
-    tie += __reduce_add_sync(0xffffffffu, lane < warp ? s_mm[1][lane] : 0);
-  }
-  sure -= n_sure;  // taken for sure, before this thread's blocks
-  tie -= n_tie;    // ties before them
+  int total;
+  // both counts in one scan (at most 32768 each)
+  const uint32_t before = uint32_t(exclusive_scan<T>(__popc(sure_m) | (__popc(tie_m) << 16), s_mm, total));
+  int sure = before & 0xffff, tie = before >> 16;  // taken for sure, and ties, before this thread's blocks
   // ascending: a block's place is what was taken before it
   for (uint32_t both = sure_m | tie_m; both != 0; both &= both - 1) {
     const uint32_t bit = both & (0u - both);
