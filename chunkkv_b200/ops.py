@@ -847,8 +847,10 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start, m: int |
     every later position).  `m` defaults to all rows (1 for a device `start`)."""
     H, D = cache.n_kv_heads, cache.head_dim
     _rows_view("k", k, H, D)
-    _rows_view("v", v, H, D)
-    rows = min(k.shape[1], v.shape[1])
+    rows = k.shape[1]
+    if v.shape != k.shape or v.dtype != k.dtype or v.stride(2) != 1:
+        _rows_view("v", v, H, D)
+        rows = min(rows, v.shape[1])
     if m is None:
         m = 1 if isinstance(start, torch.Tensor) else (rows - start if by_position else rows)
     if m < 0 or (not by_position and m > rows):
@@ -871,7 +873,7 @@ def kv8_read(cache: KV8Cache, start: int = 0, m: int | None = None) -> tuple[tor
         raise ValueError(f"kv8_read: tokens [{start}, {start + m}) outside the context of {cache.n_ctx}")
     _on_device(cache.k)
     H, D = cache.n_kv_heads, cache.head_dim
-    k = torch.empty((H, m, D), dtype=BF16, device=cache.k.device)
+    k = cache.tail.new_empty((H, m, D))  # bf16 on the cache's device
     v = torch.empty_like(k)
     _run("ckv_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
          k.data_ptr(), v.data_ptr(), H, D, cache.n_ctx, start, m, _KV8_TYPES[cache.dtype], _stream(),
@@ -918,7 +920,7 @@ def _rows_out(q: torch.Tensor, m: int, width: int, out: torch.Tensor | None) -> 
     if out is not None:
         _buf("out", out, m * width)
         return out
-    return torch.empty_like(q) if m == q.shape[0] else torch.empty((m, *q.shape[1:]), dtype=BF16, device=q.device)
+    return torch.empty_like(q) if m == q.shape[0] else q.new_empty((m, *q.shape[1:]))
 
 
 def _scratch(nbytes: int, device: torch.device) -> torch.Tensor | None:
@@ -979,7 +981,7 @@ def block_select(q: torch.Tensor, digest: BlockDigest, positions: torch.Tensor, 
     H, _, _, D = digest.codes.shape
     m, Hq = _query(q, H, D, positions, m)
     if out is None:
-        out = torch.empty((m, H, top), dtype=torch.int32, device=q.device)
+        out = positions.new_empty((m, H, top))  # int32
     else:
         _buf("out", out, m * H * top, dtype=torch.int32)
     _on_device(q, positions, out, digest.codes)
@@ -1067,7 +1069,7 @@ def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if digest is not None and (digest.n_ctx != n_ctx or tuple(digest.codes.shape[::3]) != (H, D)):
         raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache "
                          f"{tuple(k_cache.shape)}")
-    out, blocks = _sparse_out(q, m, Hq, H, D, top, out, blocks)
+    out, blocks = _sparse_out(q, positions, m, Hq, H, D, top, out, blocks)
     _on_device(q, k_cache, v_cache, positions, out, blocks, None if digest is None else digest.codes)
     need = _size("ckv_attention_sparse_workspace_size", q.get_device(), m, Hq, H, D, n_ctx, top, 16, int(digest is None))
     ws = _scratch(need, q.device)
@@ -1079,13 +1081,13 @@ def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out, blocks
 
 
-def _sparse_out(q, m: int, Hq: int, H: int, D: int, top: int, out, blocks):
+def _sparse_out(q, positions, m: int, Hq: int, H: int, D: int, top: int, out, blocks):
     """The output rows and block lists: the caller's, or new ones."""
     if top < 1:
         raise ValueError(f"top must be at least 1, got {top}")
     out = _rows_out(q, m, Hq * D, out)
     if blocks is None:
-        blocks = torch.empty((m, H, top), dtype=torch.int32, device=q.device)
+        blocks = positions.new_empty((m, H, top))  # int32
     else:
         _buf("blocks", blocks, m * H * top, dtype=torch.int32)
     return out, blocks
@@ -1100,7 +1102,7 @@ def attention_sparse_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
         raise ValueError("attention_sparse_kv8: the cache keeps no digest (KV8Cache(..., digest=True))")
     H, D = cache.n_kv_heads, cache.head_dim
     m, Hq = _query(q, H, D, positions, m)
-    out, blocks = _sparse_out(q, m, Hq, H, D, top, out, blocks)
+    out, blocks = _sparse_out(q, positions, m, Hq, H, D, top, out, blocks)
     _on_device(q, positions, out, blocks, cache.k)
     need = _size("ckv_attention_sparse_workspace_size", q.get_device(), m, Hq, H, D, cache.n_ctx, top, 8, 0)
     ws = _scratch(need, q.device)
