@@ -787,14 +787,21 @@ int launch_nt(const Args& a, const Plan& p, void* workspace, cudaStream_t stream
 
 int launches(const Plan& p) { return p.splits > 1 && !p.join ? 2 : 1; }
 
+// query rows (token, head) of a call: tile and row numbers stay within 32 bits
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - (1 << 20);
+
 bool shape_ok(int m, int Hq, int Hk, int HD, int n_ctx) {
-  return m >= 0 && Hk > 0 && Hk <= 65535 && Hq > 0 && Hq % Hk == 0 && (HD == 64 || HD == 128) && n_ctx > 0 && n_ctx <= (1 << 30);
+  return m >= 0 && Hk > 0 && Hk <= 65535 && Hq > 0 && Hq % Hk == 0 && (HD == 64 || HD == 128) && n_ctx > 0 && n_ctx <= (1 << 30) &&
+         int64_t(m) * Hq <= kMaxRows;
 }
 
 int check(const char* name, const Args& a, int HD, int64_t tiles) {
   CKV_REQUIRE(a.m >= 0 && a.Hk > 0 && a.Hk <= 65535 && a.Hq > 0 && a.Hq % a.Hk == 0, "%s: %d query heads over %d KV heads", name,
               a.Hq, a.Hk);
   CKV_REQUIRE(a.n_ctx > 0 && a.n_ctx <= (1 << 30), "%s: context of %d", name, a.n_ctx);
+  CKV_REQUIRE(a.scale_log2 >= 0.f && a.scale_log2 <= 3.0e38f, "%s: scale %g (finite, not negative)", name,
+              double(a.scale_log2 / 1.4426950408889634f));
+  CKV_REQUIRE(int64_t(a.m) * a.Hq <= kMaxRows, "%s: %d rows of %d heads in one call", name, a.m, a.Hq);
   if (HD != 64 && HD != 128) {
     set_error("%s: head_dim %d (64 or 128)", name, HD);
     return CKV_ERR_UNSUPPORTED;
@@ -827,7 +834,8 @@ SparseSpace sparse_space(int m, int Hq, int Hk, int HD, int es, int n_ctx, int t
 
 int check_space(const char* name, int m, int Hq, int Hk, int HD, int es, int n_ctx, int top, bool build, const void* workspace,
                 int64_t ws_bytes) {
-  CKV_REQUIRE(m >= 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && n_ctx > 0 && top > 0, "%s: bad sizes", name);
+  CKV_REQUIRE(m >= 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && n_ctx > 0 && top > 0 && int64_t(m) * Hq <= kMaxRows,
+              "%s: bad sizes", name);
   if (m == 0) return CKV_OK;
   const int64_t need = sparse_space(m, Hq, Hk, HD, es, n_ctx, top, build).total();
   CKV_REQUIRE(ws_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),

@@ -53,6 +53,7 @@ constexpr int kWarpConv = 8, kWarpSched = 12, kWarpMma = 13;
 constexpr uint32_t TMEM_COLS = 512;  // S/P of tile w at [128w, 128w+128), O of tile w at 256+128w
 constexpr uint32_t O_COL = 256;
 constexpr float kPBits = 7.0f;  // P' is 2^7 times its weight
+constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
 constexpr int kRegsSoftmax = 168, kRegsConv = 104, kRegsRest = 72;
 static_assert(8 * kRegsSoftmax + 4 * kRegsConv + 4 * kRegsRest == 16 * 128, "the split is what the launch holds");
 
@@ -525,8 +526,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
           // a block of zeros (scale 0) adds nothing whatever its weight: any scale will do
           const int sl = (gt % kScaleSlots) * GRP + t;
           s_ks[sl] = ks;
-          s_lv[sl] = (vs > 0.f ? log2f(vs / ref) : 0.f) + kPBits;
-          s_iv[sl] = vs > 0.f ? ref / vs : 1.0f;
+          // at least 2^-100 of the reference, so that the inverse is finite and the weights do not
+          // underflow in the row's sum (their products round to 0 from 2^-31 on)
+          const float rel = vs > 0.f ? fmaxf(vs / ref, kTiny) : 1.0f;
+          s_lv[sl] = log2f(rel) + kPBits;
+          s_iv[sl] = 1.0f / rel;
         }
         fence_async_smem();
         mbar_arrive(&k_full[gt % KS]);
@@ -995,6 +999,7 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
               n_q_heads / n_kv_heads, n_ctx);
     return CKV_ERR_UNSUPPORTED;
   }
+  CKV_REQUIRE(scale >= 0.f && scale <= 3.0e38f, "ckv_attention_kv8: scale %g (finite, not negative)", double(scale));
   CKV_REQUIRE(q && k8 && v8 && k_scale && v_scale && positions && out, "ckv_attention_kv8: null pointer");
   CKV_REQUIRE(aligned16(q) && aligned16(k8) && aligned16(v8) && aligned16(out),
               "ckv_attention_kv8: tensors must be 16-byte aligned");

@@ -717,6 +717,13 @@ def _on_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
         raise ValueError(f"tensors lie on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _same_device(name: str, first: torch.Tensor, **others: torch.Tensor) -> None:
+    """The buffers of one object lie on one device (its ops look at the first alone)."""
+    for other, t in others.items():
+        if t.device != first.device:
+            raise ValueError(f"{other} lies on {t.device}, {name} on {first.device}")
+
+
 def _n_blocks(n_ctx: int) -> int:
     return (n_ctx + PAGE_TOKENS - 1) // PAGE_TOKENS
 
@@ -749,6 +756,7 @@ class BlockDigest:
             raise ValueError(f"scale: expected shape ({codes.shape[0]}, {nb}), got {tuple(scale.shape)}")
         _buf("codes", codes, 0, dtype=torch.int8)
         _buf("scale", scale, 0, dtype=torch.float32)
+        _same_device("codes", codes, scale=scale)
         self.codes, self.scale, self.n_ctx = codes, scale, int(n_ctx)
 
 
@@ -805,6 +813,8 @@ class KV8Cache:
         _buf("tail", tail, 0)
         if digest is not None and (tuple(digest.codes.shape) != (H, nb, 2, D) or digest.n_ctx != n_ctx):
             raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache")
+        _same_device("k", k, v=v, k_scale=k_scale, v_scale=v_scale, tail=tail,
+                     digest=k if digest is None else digest.codes)
         self.k, self.v, self.k_scale, self.v_scale, self.tail, self.digest = k, v, k_scale, v_scale, tail, digest
         end = int(tail_start) if tail_start % PAGE_TOKENS else 0
         self.tail_end = torch.full((2, H), end, dtype=torch.int32, device=k.device)

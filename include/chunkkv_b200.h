@@ -407,9 +407,12 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
 /* ckv_attention over the 8-bit cache: q/out [m][Hq][D] bf16, key j visible to row i iff
  * j <= positions[i]; a row whose position is negative sees no key and gives zeros, one at or
  * past n_ctx sees every key (recorded).  Codes and scales past every row's position may hold
- * anything; those some row sees must be finite (ckv_kv8_write leaves no other), for a weight of 0
- * does not silence a NaN in a row that shares a tile.  At most 128 query heads per KV head, head_dim 64 or
- * 128.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
+ * anything; codes some row sees must be finite and scales 0 or in [2^-110, 2^120] (ckv_kv8_write
+ * leaves no other), for a weight of 0 does not silence a NaN in a row that shares a tile.  Weights
+ * meet the codes in fp16, relative to the largest value scale of the keys worked on together:
+ * an output is exact to 2^-31 of the largest value there, so a row that sees only values smaller
+ * than 2^-20 of it loses bits.  `scale` is finite and not negative (a negative one is refused).
+ * At most 128 query heads per KV head, head_dim 64 or 128.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
  * 0) needs no initialisation; calls that share one must not overlap on the GPU. */
 CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 /* Kernels one ckv_attention_kv8 call launches at this shape (0 for a shape it refuses). */
@@ -437,7 +440,7 @@ CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const f
 /* Attention of row i over the keys j <= positions[i] of the blocks listed for it (ascending, -1
  * past the end; an entry out of range or not above the one before it is skipped and recorded as
  * CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache (cache_bits 16 or 8).
- * Rows that see no key give zeros. */
+ * Rows that see no key give zeros.  `scale` as in ckv_attention_kv8; m * n_q_heads below 2^31 - 2^20. */
 CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top,
                                                     int cache_bits);
 CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int cache_bits);

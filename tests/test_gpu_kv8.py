@@ -331,3 +331,46 @@ def test_caches_past_two_gigabytes():
     blocks = torch.arange(n // 16 - 20, n // 16, dtype=torch.int32, device=DEV).expand(2, H, 20).contiguous()
     out = ops.attention_blocks_kv8(q, c, p, blocks)
     check_attention(out[:, H - 1:].contiguous(), q[:, H - 1:].contiguous(), kd, vd, p, blocks[:, H - 1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m", [1, 9, 70])
+def test_value_scales_more_than_32_bits_of_exponent_apart(m, dtype):
+    """Every third block of V lies 2^-130 below the others (their scales' ratio leaves fp32): its
+    values vanish beside theirs, its weights still count in the softmax's sum."""
+    H, D, n = 2, 128, 400
+    k, v = rows(H, n, D, 71, 0.2), rows(H, n, D, 72, 0.2).float()
+    tiny = (torch.arange(n, device=DEV) // 16 % 3 == 1)[None, :, None]
+    v = torch.where(tiny, v * 2.0 ** -90, v * 2.0 ** 40).to(BF)
+    c = ops.KV8Cache(H, n, D, dtype, DEV)
+    ops.kv8_write(c, k, v, 0)
+    q = queries(m, 4, D, 73, 0.5)
+    pos = torch.linspace(n - 1, 20, m, device=DEV).to(torch.int32)
+    out = ops.attention_kv8(q, c, pos)
+    check_attention(out, q, ref.values(c.k.float(), c.k_scale), ref.values(c.v.float(), c.v_scale), pos)
+
+
+@pytest.mark.parametrize("m,n", [(150, 6000), (700, 900)])
+def test_tiles_in_two_graphs_at_once(m, n):
+    """The same for many rows: key splits (150 rows) and a counter of work items (both)."""
+    Hq, H, D = 28, 4, 128
+    c, k, v = filled(H, n, D, torch.float8_e4m3fn, seed=2)
+    p = torch.arange(n - m, n, dtype=torch.int32, device=DEV)
+    qs = [queries(m, Hq, D, s) for s in (1, 2)]
+    want = [ops.attention_kv8(q, c, p) for q in qs]
+    torch.cuda.synchronize()
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for q, s in zip(qs, streams):
+        g = torch.cuda.CUDAGraph()
+        out = torch.zeros_like(q)
+        with torch.cuda.graph(g, stream=s):
+            for _ in range(4):
+                ops.attention_kv8(q, c, p, out=out)
+        graphs.append(g)
+        outs.append(out)
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])

@@ -236,3 +236,20 @@ def test_sparse_decode_step_replayed_in_a_graph():
             assert torch.equal(blocks.cpu().long(), ref.select(q, d[0], d[1], p, 16))
             kq, vq = (ref.quantize(t[:, :pos + 1], torch.int8) for t in (k, v))
             check_attention(out, q, ref.values(*kq)[:, :pos + 1], ref.values(*vq)[:, :pos + 1], p, blocks)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("Hq,H,m", [(2, 2, 40_000), (20, 1, 17_000)])
+def test_more_rows_than_one_grid_holds(Hq, H, m, kind):
+    """Past 32,768 row tiles (20 heads of one KV head make two) the call goes in several runs."""
+    D, n, top = 64, 200, 3
+    attend, kd, vd, _, _ = caches(kind, H, n, D, seed=5)
+    q = queries(m, Hq, D, 6)
+    g = torch.Generator().manual_seed(7)
+    p = torch.randint(-1, n, (m,), generator=g, dtype=torch.int32).to(DEV)
+    b0 = torch.randint(0, 4, (m, H, 1), generator=g)
+    blocks = torch.cat([b0, b0 + 3, b0 + 8], -1).to(torch.int32).to(DEV)
+    out = attend(q, p, blocks)
+    for rows in (slice(0, 64), slice(16_300, 16_450), slice(32_700, 32_830), slice(m - 40, m)):
+        if rows.start < m:
+            check_attention(out[rows], q[rows], kd, vd, p[rows], blocks[rows])

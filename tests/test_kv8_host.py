@@ -167,3 +167,35 @@ def test_oracle_bound_holds_every_key():
     true = (k[0].double() @ q[0, 0].double()).view(10, 16).amax(-1)
     # each of 64 products is off by half a step of either side: |q| s/2 + |k| a/254 <= a s (127/2 + 127/2 + 1/4) / 127
     assert bool((true <= bound + 64 * a * ds[0] * (127.25 / 127)).all())
+
+
+def test_buffers_of_one_cache_lie_on_one_device():
+    c = cache(digest=True)
+    ok = dict(k=c.k, v=c.v, k_scale=c.k_scale, v_scale=c.v_scale, n_ctx=40, tail=c.tail, digest=c.digest)
+    ops.KV8Cache.wrap(**ok)
+    for name in ("v", "k_scale", "v_scale", "tail"):
+        with pytest.raises(ValueError, match=f"{name} lies on meta"):
+            ops.KV8Cache.wrap(**{**ok, name: ok[name].to("meta")})
+    with pytest.raises(ValueError, match="digest lies on meta"):
+        ops.KV8Cache.wrap(**{**ok, "digest": ops.BlockDigest(2, 40, 64, "meta")})
+    with pytest.raises(ValueError, match="scale lies on meta"):
+        ops.BlockDigest.wrap(c.digest.codes, c.digest.scale.to("meta"), 40)
+
+
+def test_entry_points_refuse_scales_and_row_counts():
+    """Nothing is launched for any of these."""
+    P = 16
+    for scale in (-1.0, float("inf"), float("nan")):
+        for m in (1, 100):
+            with pytest.raises(ValueError, match="scale"):
+                _lib.call("ckv_attention_kv8", *(P,) * 7, m, 4, 2, 64, 100, scale, 0, P, 1 << 40, None)
+        with pytest.raises(ValueError, match="scale"):
+            _lib.call("ckv_attention_blocks", *(P,) * 6, 1, 4, 2, 64, 800, 4, scale, P, 1 << 40, None)
+        with pytest.raises(ValueError, match="scale"):
+            _lib.call("ckv_attention_blocks_kv8", *(P,) * 8, 1, 4, 2, 64, 800, 4, scale, 0, P, 1 << 40, None)
+    many = (1 << 31) - 1
+    with pytest.raises(ValueError, match="rows of 4 heads"):
+        _lib.call("ckv_attention_blocks", *(P,) * 6, many, 4, 2, 64, 800, 4, 1.0, P, 1 << 40, None)
+    with pytest.raises(ValueError, match="bad sizes"):
+        _lib.call("ckv_attention_sparse", *(P,) * 8, many, 4, 2, 64, 800, 4, 1, 1, 1.0, P, 1 << 40, None)
+    assert _lib.load().ckv_attention_blocks_workspace_size(many, 4, 2, 64, 4, 16) == 0
