@@ -11,10 +11,12 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
+CALL = PKG / "_call.so"
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libchunkkv_b200.so"
@@ -71,7 +73,27 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB)
         manifest.write_text(names)
+    _build_call(force, verbose)
     return LIB
+
+
+def _build_call(force: bool, verbose: bool) -> None:
+    """The CPython module of the calls that go past ctypes (host code only).  Where Python's
+    headers are missing the same entry points are called through ctypes."""
+    src, header = CSRC / "py_call.cpp", INCLUDE / "chunkkv_b200.h"
+    python = Path(sysconfig.get_paths()["include"])
+    if not (python / "Python.h").exists():
+        print(f"no Python.h in {python}: entry points are called through ctypes", file=sys.stderr)
+        return
+    if not force and CALL.exists() and CALL.stat().st_mtime >= max(src.stat().st_mtime, header.stat().st_mtime):
+        return
+    tmp = CALL.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall",
+           f"-I{INCLUDE}", f"-I{python}", str(src), "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, CALL)
 
 
 if __name__ == "__main__":

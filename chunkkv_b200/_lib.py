@@ -12,6 +12,11 @@ import ctypes as C
 import threading
 from pathlib import Path
 
+try:
+    from . import _call
+except ImportError:  # built without Python's headers
+    _call = None
+
 LIB_PATH = Path(__file__).resolve().parent / "libchunkkv_b200.so"
 
 _p = C.c_void_p
@@ -127,6 +132,9 @@ def load() -> C.CDLL:
                 fn = getattr(lib, name)
                 fn.argtypes = argtypes
                 fn.restype = _RESTYPES.get(name, C.c_int)
+            # the per-token calls past ctypes' conversion of arguments (csrc/py_call.cpp)
+            for name in _call.names if _call is not None else ():
+                setattr(lib, name, _call.bind(name, C.cast(getattr(lib, name), _p).value))
             _lib = lib
     return _lib
 
@@ -142,7 +150,7 @@ def last_error() -> str:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise on failure."""
-    rc = getattr(load(), name)(*args)
+    rc = getattr(_lib or load(), name)(*args)
     if rc == CKV_OK:
         return
     msg = f"{name}: {last_error()}"

@@ -705,16 +705,19 @@ _KV8_TYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}  # CKV_KV8_INT8, CKV_KV8_E4
 KV8_DTYPES = tuple(_KV8_TYPES)
 
 
-def _on_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    """Every tensor lies on the current CUDA device, whose current stream the call uses."""
+def _on_device(first: torch.Tensor, *ts: torch.Tensor | None) -> int:
+    """Every tensor lies on the current CUDA device; returns its current stream, which the call
+    uses."""
     if not first.is_cuda:
         raise ValueError("chunkkv_b200 ops take CUDA tensors (there is no CPU path)")
     dev = first.get_device()
     for t in ts:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors lie on different devices ({first.device} and {t.device})")
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"tensors lie on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+    current = torch._C._cuda_getDevice()
+    if dev != current:
+        raise ValueError(f"tensors lie on {first.device}, the current device is cuda:{current}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _same_device(name: str, first: torch.Tensor, **others: torch.Tensor) -> None:
@@ -826,14 +829,17 @@ class KV8Cache:
         return self.k.numel() * 2 + self.k_scale.numel() * 8
 
 
-def _rows_view(name: str, t: torch.Tensor, H: int, D: int) -> None:
-    """bf16 rows [H, n, D] with contiguous rows (any 16-byte aligned row and head strides)."""
+def _rows_view(name: str, t: torch.Tensor, H: int, D: int) -> tuple[int, int, int]:
+    """bf16 rows [H, n, D] with contiguous rows (any 16-byte aligned row and head strides);
+    returns n and the strides of heads and rows."""
     if t.dtype != BF16:
         raise ValueError(f"{name}: expected {BF16}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[0] != H or t.shape[2] != D:
-        raise ValueError(f"{name}: expected shape ({H}, n, {D}), got {tuple(t.shape)}")
-    if t.stride(2) != 1:
-        raise ValueError(f"{name}: expected rows of contiguous elements, got strides {t.stride()}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != H or shape[2] != D:
+        raise ValueError(f"{name}: expected shape ({H}, n, {D}), got {tuple(shape)}")
+    if stride[2] != 1:
+        raise ValueError(f"{name}: expected rows of contiguous elements, got strides {stride}")
+    return shape[1], stride[0], stride[1]
 
 
 def _start(start, m: int, n_ctx: int, rows: int, by_position: bool, name: str):
@@ -856,23 +862,21 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start, m: int |
     tensor (then `m` rows are read from wherever it points at launch: a captured call serves
     every later position).  `m` defaults to all rows (1 for a device `start`)."""
     H, D = cache.n_kv_heads, cache.head_dim
-    _rows_view("k", k, H, D)
-    rows = k.shape[1]
-    if v.shape != k.shape or v.dtype != k.dtype or v.stride(2) != 1:
-        _rows_view("v", v, H, D)
-        rows = min(rows, v.shape[1])
+    rows, k_head, k_row = _rows_view("k", k, H, D)
+    v_rows, v_head, v_row = _rows_view("v", v, H, D)
+    rows = min(rows, v_rows)
     if m is None:
         m = 1 if isinstance(start, torch.Tensor) else (rows - start if by_position else rows)
     if m < 0 or (not by_position and m > rows):
         raise ValueError(f"kv8_write: {m} rows asked for, the source has {rows}")
     s, s_dev = _start(start, m, cache.n_ctx, rows, by_position, "kv8_write")
-    _on_device(k, v, cache.k, start if s_dev is not None else None)
+    stream = _on_device(k, v, cache.k, start if s_dev is not None else None)
     dig = cache.digest
-    _run("ckv_kv8_write", k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1), rows,
+    _run("ckv_kv8_write", k.data_ptr(), v.data_ptr(), k_head, k_row, v_head, v_row, rows,
          int(by_position), m, s, s_dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), cache.tail.data_ptr(), cache.tail_end.data_ptr(),
          None if dig is None else dig.codes.data_ptr(), None if dig is None else dig.scale.data_ptr(), H, D,
-         cache.n_ctx, _KV8_TYPES[cache.dtype], _stream(), nbytes=6.0 * H * m * D)
+         cache.n_ctx, _KV8_TYPES[cache.dtype], stream, nbytes=6.0 * H * m * D)
     return cache
 
 
@@ -881,12 +885,12 @@ def kv8_read(cache: KV8Cache, start: int = 0, m: int | None = None) -> tuple[tor
     m = cache.n_ctx - start if m is None else m
     if start < 0 or m < 0 or start + m > cache.n_ctx:
         raise ValueError(f"kv8_read: tokens [{start}, {start + m}) outside the context of {cache.n_ctx}")
-    _on_device(cache.k)
+    stream = _on_device(cache.k)
     H, D = cache.n_kv_heads, cache.head_dim
     k = cache.tail.new_empty((H, m, D))  # bf16 on the cache's device
     v = torch.empty_like(k)
     _run("ckv_kv8_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-         k.data_ptr(), v.data_ptr(), H, D, cache.n_ctx, start, m, _KV8_TYPES[cache.dtype], _stream(),
+         k.data_ptr(), v.data_ptr(), H, D, cache.n_ctx, start, m, _KV8_TYPES[cache.dtype], stream,
          nbytes=6.0 * H * m * D)
     return k, v
 
@@ -895,15 +899,15 @@ def block_digest(k_cache: torch.Tensor, digest: BlockDigest, start=0, m: int | N
     """Bring `digest` up to date with a bf16 K cache [H, n_ctx, D] whose tokens [start, start + m)
     are new (`start` an int or an int32 device tensor, m then 1 unless given)."""
     H, nb, _, D = digest.codes.shape
-    _rows_view("k_cache", k_cache, H, D)
+    rows, head, row = _rows_view("k_cache", k_cache, H, D)
     if m is None:
-        m = 1 if isinstance(start, torch.Tensor) else min(digest.n_ctx, k_cache.shape[1]) - start
+        m = 1 if isinstance(start, torch.Tensor) else min(digest.n_ctx, rows) - start
     if m < 0:
         raise ValueError(f"block_digest: {m} rows")
-    s, s_dev = _start(start, m, digest.n_ctx, k_cache.shape[1], True, "block_digest")
-    _on_device(k_cache, digest.codes, start if s_dev is not None else None)
-    _run("ckv_block_digest", k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.shape[1], m, s, s_dev,
-         digest.codes.data_ptr(), digest.scale.data_ptr(), H, D, digest.n_ctx, _stream(), nbytes=2.0 * H * m * D)
+    s, s_dev = _start(start, m, digest.n_ctx, rows, True, "block_digest")
+    stream = _on_device(k_cache, digest.codes, start if s_dev is not None else None)
+    _run("ckv_block_digest", k_cache.data_ptr(), head, row, rows, m, s, s_dev,
+         digest.codes.data_ptr(), digest.scale.data_ptr(), H, D, digest.n_ctx, stream, nbytes=2.0 * H * m * D)
     return digest
 
 
@@ -971,14 +975,14 @@ def attention_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, out
     H, D = cache.n_kv_heads, cache.head_dim
     m, Hq = _query(q, H, D, positions, m)
     out = _rows_out(q, m, Hq * D, out)
-    _on_device(q, positions, out, cache.k, workspace)
+    stream = _on_device(q, positions, out, cache.k, workspace)
     need = _size("ckv_attention_kv8_workspace_size", q.get_device(), m, Hq, H, D, cache.n_ctx)
     workspace, nbytes = _workspace_arg(workspace, need, q.device)
     kernels = 1 if _TIMER is None else _lib.load().ckv_attention_kv8_launches(m, Hq, H, D, cache.n_ctx)
     _run("ckv_attention_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), positions.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
          1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(workspace), nbytes,
-         _stream(), flops=flops, kernels=kernels)
+         stream, flops=flops, kernels=kernels)
     return out
 
 
@@ -994,12 +998,12 @@ def block_select(q: torch.Tensor, digest: BlockDigest, positions: torch.Tensor, 
         out = positions.new_empty((m, H, top))  # int32
     else:
         _buf("out", out, m * H * top, dtype=torch.int32)
-    _on_device(q, positions, out, digest.codes)
+    stream = _on_device(q, positions, out, digest.codes)
     need = _size("ckv_block_select_workspace_size", q.get_device(), m, Hq, H, D, digest.n_ctx)
     ws, nbytes = _workspace_arg(None, need, q.device)
     kernels = 1 if _TIMER is None else _lib.load().ckv_block_select_launches(m, Hq, H, D, digest.n_ctx)
     _run("ckv_block_select", q.data_ptr(), digest.codes.data_ptr(), digest.scale.data_ptr(), positions.data_ptr(),
-         out.data_ptr(), m, Hq, H, D, digest.n_ctx, top, sink, recent, _ptr(ws), nbytes, _stream(), kernels=kernels)
+         out.data_ptr(), m, Hq, H, D, digest.n_ctx, top, sink, recent, _ptr(ws), nbytes, stream, kernels=kernels)
     return out
 
 
@@ -1027,13 +1031,13 @@ def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     m, Hq = _query(q, H, D, positions, m)
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
-    _on_device(q, k_cache, v_cache, positions, blocks, out)
+    stream = _on_device(q, k_cache, v_cache, positions, blocks, out)
     need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, top, 16)
     ws, nbytes = _workspace_arg(None, need, q.device)
     kernels = 1 if _TIMER is None else _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, top, 16)
     _run("ckv_attention_blocks", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
          blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, 1.0 / math.sqrt(D) if scale is None else float(scale),
-         _ptr(ws), nbytes, _stream(), kernels=kernels)
+         _ptr(ws), nbytes, stream, kernels=kernels)
     return out
 
 
@@ -1045,14 +1049,14 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     m, Hq = _query(q, H, D, positions, m)
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
-    _on_device(q, positions, blocks, out, cache.k)
+    stream = _on_device(q, positions, blocks, out, cache.k)
     need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, top, 8)
     ws, nbytes = _workspace_arg(None, need, q.device)
     kernels = 1 if _TIMER is None else _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, top, 8)
     _run("ckv_attention_blocks_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
          top, 1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), nbytes,
-         _stream(), kernels=kernels)
+         stream, kernels=kernels)
     return out
 
 
@@ -1080,14 +1084,14 @@ def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache "
                          f"{tuple(k_cache.shape)}")
     out, blocks = _sparse_out(q, positions, m, Hq, H, D, top, out, blocks)
-    _on_device(q, k_cache, v_cache, positions, out, blocks, None if digest is None else digest.codes)
+    stream = _on_device(q, k_cache, v_cache, positions, out, blocks, None if digest is None else digest.codes)
     need = _size("ckv_attention_sparse_workspace_size", q.get_device(), m, Hq, H, D, n_ctx, top, 16, int(digest is None))
     ws = _scratch(need, q.device)
     kernels = 1 if _TIMER is None else _sparse_kernels(m, Hq, H, D, n_ctx, top, 16) + (digest is None)
     _run("ckv_attention_sparse", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
          None if digest is None else digest.codes.data_ptr(), None if digest is None else digest.scale.data_ptr(),
          positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, sink, recent,
-         1.0 / math.sqrt(D) if scale is None else float(scale), _ptr(ws), need, _stream(), kernels=kernels)
+         1.0 / math.sqrt(D) if scale is None else float(scale), _ptr(ws), need, stream, kernels=kernels)
     return out, blocks
 
 
@@ -1113,13 +1117,13 @@ def attention_sparse_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     H, D = cache.n_kv_heads, cache.head_dim
     m, Hq = _query(q, H, D, positions, m)
     out, blocks = _sparse_out(q, positions, m, Hq, H, D, top, out, blocks)
-    _on_device(q, positions, out, blocks, cache.k)
+    stream = _on_device(q, positions, out, blocks, cache.k)
     need = _size("ckv_attention_sparse_workspace_size", q.get_device(), m, Hq, H, D, cache.n_ctx, top, 8, 0)
     ws = _scratch(need, q.device)
     kernels = 1 if _TIMER is None else _sparse_kernels(m, Hq, H, D, cache.n_ctx, top, 8)
     _run("ckv_attention_sparse_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), dig.codes.data_ptr(), dig.scale.data_ptr(), positions.data_ptr(),
          blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx, top, sink, recent,
-         1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), need, _stream(),
+         1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), need, stream,
          kernels=kernels)
     return out, blocks

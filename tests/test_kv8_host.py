@@ -199,3 +199,29 @@ def test_entry_points_refuse_scales_and_row_counts():
     with pytest.raises(ValueError, match="bad sizes"):
         _lib.call("ckv_attention_sparse", *(P,) * 8, many, 4, 2, 64, 800, 4, 1, 1, 1.0, P, 1 << 40, None)
     assert _lib.load().ckv_attention_blocks_workspace_size(many, 4, 2, 64, 4, 16) == 0
+
+
+def test_direct_calls_convert_like_ctypes():
+    """The entry points that go past ctypes (where the module is built): argument counts, ranges
+    and types are checked, None is a null pointer."""
+    lib = _lib.load()
+    read = lib.ckv_kv8_read  # k8, v8, ks, vs, ko, vo, H, D, n_ctx, start, m, type, stream
+    ok = (None,) * 6 + (4, 128, 64, 0, 0, 0, None)
+    assert read(*ok) == _lib.CKV_OK
+    assert read(*(None,) * 6, 4, 128, 64, 0, 1, 0, None) == _lib.CKV_ERR_ARG and "null pointer" in _lib.last_error()
+    if _lib._call is None:
+        pytest.skip("built without Python's headers")
+    assert set(_lib._call.names) <= set(_lib.SIGNATURES)
+    for bad in (ok[:-1], ok + (0,), ()):
+        with pytest.raises(TypeError, match="13 expected"):
+            read(*bad)
+    with pytest.raises(OverflowError):
+        read(*(None,) * 6, 4, 128, 1 << 31, 0, 0, 0, None)
+    with pytest.raises(OverflowError):
+        read(-1, *(None,) * 5, 4, 128, 64, 0, 0, 0, None)
+    with pytest.raises(TypeError):
+        read(*(None,) * 6, 4, 128, 64.0, 0, 0, 0, None)
+    with pytest.raises(TypeError):
+        lib.ckv_attention_kv8(*(None,) * 7, 0, 4, 2, 64, 8, "1.0", 0, None, 0, None)
+    with pytest.raises(KeyError):
+        _lib._call.bind("ckv_no_such_call", 0)
