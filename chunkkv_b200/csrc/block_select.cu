@@ -50,9 +50,8 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// position of a token, clamped to the context (recorded when past it); negative: no key
-__device__ __forceinline__ int token_pos(const int32_t* positions, int t, int n_ctx, bool report) {
-  const int p = positions[t];
+// a token's position p, clamped to the context (recorded when past it); negative: no key
+__device__ __forceinline__ int token_pos(int p, int n_ctx, bool report) {
   if (p >= n_ctx) {
     if (report) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
     return n_ctx - 1;
@@ -125,7 +124,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
   pdl_launch_next();
   if (threadIdx.x < kTok)
     s_nb[threadIdx.x] = threadIdx.x < n_tok
-                            ? (token_pos(positions, t0 + threadIdx.x, n_ctx, hk == 0 && blockIdx.x == 0) + kBlk) / kBlk
+                            ? (token_pos(positions[t0 + threadIdx.x], n_ctx, hk == 0 && blockIdx.x == 0) + kBlk) / kBlk
                             : 0;
   // query codes: a warp per (token, head) row, HD / 32 values per lane
   for (int r = warp; r < n_tok * NT * 8; r += kScoreWarps) {
@@ -423,7 +422,7 @@ __global__ void __launch_bounds__(T > 32 ? T : 256) block_top_kernel(const __gri
   const int64_t id = T > 32 ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   if (id >= int64_t(a.m) * a.Hk) return;  // the whole group
   const int tok = a.t_begin + int(id / a.Hk);
-  const int nb = (token_pos(a.positions, tok, a.n_ctx, false) + kBlk) / kBlk;
+  const int nb = (token_pos(a.positions[tok], a.n_ctx, false) + kBlk) / kBlk;
   const uint32_t* keys = a.keys + id * key_stride(a.n_blocks);
   select_top<T, KPT>(a, nb, a.out + (int64_t(tok) * a.Hk + id % a.Hk) * a.top,
                      [&](int b) { return __ldcg(reinterpret_cast<const uint4*>(keys + b)); });
@@ -447,28 +446,43 @@ __global__ void __launch_bounds__(256)
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA has started
   pdl_wait();
   pdl_launch_next();
-  const int nb = (token_pos(a.positions, tok, a.n_ctx, hk == 0 && rank == 0) + kBlk) / kBlk;
+  // everything that does not wait for something else is requested first: the position, the
+  // first tile's digest rows (visible or not) and q
+  const int p = a.positions[tok];
   const int gr = lane >> 2, qd = lane & 3;
-  const int tiles = (nb + 15) / 16;
-  const bool all = nb <= a.top;  // no choice to make
+  uint4 nd[2][WORDS];  // digest rows b0 + gr and b0 + gr + 8 of the next tile, this lane's chunk
+  float nsc[2];
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t row = int64_t(hk) * a.n_blocks + min(tile * 16 + gr + 8 * i, a.n_blocks - 1);
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) nd[i][w] = __ldg(reinterpret_cast<const uint4*>(dig + row * 2 * HD + qd * CH) + w);
+      nsc[i] = __ldg(dig_scale + row);
+    }
+  };
+  load(rank * 8 + warp);
   for (int g = warp; g < NT * 8; g += 8) {
     const float amax = query_codes<HD>(g < G ? q + (int64_t(tok) * Hq + hk * G + g) * HD : nullptr, s_code + g * RS, lane);
     if (lane == 0) s_amax[g] = amax;
   }
+  const int nb = (token_pos(p, a.n_ctx, hk == 0 && rank == 0) + kBlk) / kBlk;
+  const int tiles = (nb + 15) / 16;
+  const bool all = nb <= a.top;  // no choice to make
   __syncthreads();
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // and so has the first one
   const uint32_t keys0 = cluster_smem_addr(s_keys, 0);
   for (int tile = rank * 8 + warp; tile < tiles && !all; tile += kCluster * 8) {
     const int b0 = tile * 16;
-    uint4 d[2][WORDS];  // digest rows b0 + gr and b0 + gr + 8, this lane's chunk
+    uint4 d[2][WORDS];
     float sc[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t row = int64_t(hk) * a.n_blocks + min(b0 + gr + 8 * i, a.n_blocks - 1);
 #pragma unroll
-      for (int w = 0; w < WORDS; ++w) d[i][w] = __ldg(reinterpret_cast<const uint4*>(dig + row * 2 * HD + qd * CH) + w);
-      sc[i] = __ldg(dig_scale + row);
+      for (int w = 0; w < WORDS; ++w) d[i][w] = nd[i][w];
+      sc[i] = nsc[i];
     }
+    if (tile + kCluster * 8 < tiles) load(tile + kCluster * 8);
     float best[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -531,7 +545,7 @@ int launch_few(const uint16_t* q, const int8_t* dig, const float* dig_scale, int
 }
 
 // Few pairs and contexts up to 65,536 tokens take one launch of clusters, and no workspace.  One row,
-// 4 heads: 6.2 / 8.7 / 10.0 us over 16,384 / 32,896 / 65,536 tokens against 7.6 / 8.9 / 8.9 us and a
+// 4 heads: 6.0 / 8.0 / 9.2 us over 16,384 / 32,896 / 65,536 tokens against 7.6 / 8.9 / 8.9 us and a
 // launch more; over 131,072 tokens with 8 heads the clusters' 64 SMs take 20 us, two kernels 15.
 bool use_cluster(int m, int Hk, int n_blocks) { return int64_t(m) * Hk <= 32 && n_blocks <= 4096; }
 
