@@ -129,14 +129,14 @@ struct Block {
   // Lane i < 2 NB copies K or V of one block.
   static __device__ __forceinline__ void request(const Args& a, uint8_t* stage, uint64_t* bar, int hk, const int (&ids)[NB],
                                                  int lane) {
-    uint32_t total = 0, bytes = 0;
-    int b = -1;
-#pragma unroll
-    for (int e = 0; e < NB; ++e) {
-      const uint32_t n = ids[e] < 0 ? 0u : uint32_t(min(int64_t(kBlk), a.head_rows - int64_t(ids[e]) * kBlk)) * ROW;
-      total += 2 * n;
-      if (lane % NB == e) b = ids[e], bytes = n;
-    }
+    auto rows_of = [&](int id) { return id < 0 ? 0u : uint32_t(min(int64_t(kBlk), a.head_rows - int64_t(id) * kBlk)) * ROW; };
+    const int id0 = ids[0], id1 = ids[NB - 1];
+    const uint32_t n0 = rows_of(id0), n1 = NB == 2 ? rows_of(id1) : 0u;
+    const uint32_t total = 2 * (n0 + n1);
+    // by a mask: a choice between array elements would put the array in local memory
+    const uint32_t odd = NB == 2 && (lane & 1) ? ~0u : 0u;
+    const int b = int(uint32_t(id0) ^ ((uint32_t(id0) ^ uint32_t(id1)) & odd));
+    const uint32_t bytes = n0 ^ ((n0 ^ n1) & odd);
     if (lane == 0) mbar_expect_tx(bar, total);
     if (lane < 2 * NB && b >= 0)
       bulk_load(stage + lane * HALF, (lane < NB ? a.k : a.v) + (int64_t(hk) * a.head_rows + int64_t(b) * kBlk) * ROW, bytes, bar);
@@ -741,12 +741,15 @@ int launch(Args a, const Plan& p, void* workspace, cudaStream_t stream) {
   a.splits = p.splits;
   a.head_tiles = p.head_tiles;
   if (p.join) {
-    using L = Layout<HD, CT, NT, 8>;
-    auto kern = attention_blocks_kernel<HD, CT, NT, LISTED, 8, true>;
+    // 12 warps where pairs of blocks halve the steps (5248 tokens: 9.2 us, with eight 9.6; 64 to 128 listed
+    // blocks: 6.9 and 7.3); eight with three stages over a bf16 cache (32 blocks: 5.7 us, with twelve 5.9)
+    constexpr int WJ = NT == 1 && CT != kBf16 ? 12 : 8;
+    using L = Layout<HD, CT, NT, WJ>;
+    auto kern = attention_blocks_kernel<HD, CT, NT, LISTED, WJ, true>;
     if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), L::BYTES)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.splits, p.tiles, a.Hk);
-    cfg.blockDim = dim3(8 * 32);
+    cfg.blockDim = dim3(WJ * 32);
     cfg.dynamicSmemBytes = L::BYTES;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
