@@ -59,33 +59,32 @@ __device__ __forceinline__ int token_pos(int p, int n_ctx, bool report) {
   return p < 0 ? -1 : p;
 }
 
-// Codes of one query head (HD / 32 values per lane of the warp) into its row of shared memory,
-// the positive parts and, HD bytes on, the negative ones; returns the largest |q|.
+// One query head's values, HD / 32 per lane of the warp (packed bf16; zeros for a null row).
 template <int HD>
-__device__ __forceinline__ float query_codes(const uint16_t* src, uint8_t* row, int lane) {
+__device__ __forceinline__ void query_load(const uint16_t* src, int lane, uint32_t (&w)[HD / 64]) {
+#pragma unroll
+  for (int e = 0; e < HD / 64; ++e) w[e] = src == nullptr ? 0u : *reinterpret_cast<const uint32_t*>(src + lane * (HD / 32) + 2 * e);
+}
+// Their codes into the head's row of shared memory, the positive parts and, HD bytes on, the
+// negative ones; returns the largest |q| (NaN left out).
+template <int HD>
+__device__ __forceinline__ float query_codes(const uint32_t (&w)[HD / 64], uint8_t* row, int lane) {
   constexpr int CH = 2 * HD / 4, CS = CH + 16, E = HD / 32;
-  uint32_t pos = 0, neg = 0;
-  float amax = 0.f;
-  if (src != nullptr) {
-    float f[E];
+  uint32_t pos = 0, neg = 0, mag = 0;
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(src + lane * E + e);
-      f[e] = lo_bf(w);
-      f[e + 1] = hi_bf(w);
-    }
+  for (int e = 0; e < E / 2; ++e) {
+    const uint32_t a = w[e] & 0x7fffu, b = (w[e] >> 16) & 0x7fffu;
+    mag = max(mag, max(a > 0x7f80u ? 0u : a, b > 0x7f80u ? 0u : b));
+  }
+  float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, mag) << 16);
+  if (amax < kTiny) amax = 0.f;
+  const float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) amax = fmaxf(amax, fabsf(f[e]));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (amax < kTiny) amax = 0.f;
-    const float inv = amax > 0.f ? __fdiv_rn(127.0f, amax) : 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = max(-127, min(127, __float2int_rn(__fmul_rn(f[e], inv))));
-      pos |= uint32_t(uint8_t(c > 0 ? c : 0)) << (8 * e);
-      neg |= uint32_t(uint8_t(c < 0 ? c : 0)) << (8 * e);
-    }
+  for (int e = 0; e < E; ++e) {
+    const float f = (e & 1) ? hi_bf(w[e / 2]) : lo_bf(w[e / 2]);
+    const int c = max(-127, min(127, __float2int_rn(__fmul_rn(f, inv))));
+    pos |= uint32_t(uint8_t(c > 0 ? c : 0)) << (8 * e);
+    neg |= uint32_t(uint8_t(c < 0 ? c : 0)) << (8 * e);
   }
   const int i = lane * E, j = HD + lane * E;  // byte offsets in the 2D-long row
   if constexpr (E == 4) {
@@ -101,7 +100,9 @@ __device__ __forceinline__ float query_codes(const uint16_t* src, uint8_t* row, 
 // CTA: up to kTok tokens of one KV head against a strided set of 16-block tiles.  The
 // query codes are made once per CTA in shared memory; a warp then holds one tile's digest
 // rows in registers and runs every token of the CTA over them.  Row and chunk strides of
-// the codes keep the eight lanes of a 16-byte shared load in distinct banks.
+// the codes keep the eight lanes of a 16-byte shared load in distinct banks.  938 rows over 32,896
+// tokens, 28 heads over 4: 61 us, bound by issue slots (per 16 blocks and token 8 mma and, to
+// reduce and order the result, about as many other instructions as those take).
 template <int HD, int NT>
 __global__ void __launch_bounds__(kScoreWarps * 32)
     block_score_kernel(const uint16_t* __restrict__ q, const int8_t* __restrict__ dig, const float* __restrict__ dig_scale,
@@ -117,8 +118,9 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
   __shared__ int s_nb[kTok];
   const int G = Hq / Hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.z;
-  const int t0 = t_begin + blockIdx.y * kTok;
+  const int hk = blockIdx.y;
+  // the last tokens first: they usually see the most blocks
+  const int t0 = t_begin + int(gridDim.z - 1 - blockIdx.z) * kTok;
   const int n_tok = min(kTok, t_begin + m - t0);
   pdl_wait();
   pdl_launch_next();
@@ -126,12 +128,22 @@ __global__ void __launch_bounds__(kScoreWarps * 32)
     s_nb[threadIdx.x] = threadIdx.x < n_tok
                             ? (token_pos(positions[t0 + threadIdx.x], n_ctx, hk == 0 && blockIdx.x == 0) + kBlk) / kBlk
                             : 0;
-  // query codes: a warp per (token, head) row, HD / 32 values per lane
-  for (int r = warp; r < n_tok * NT * 8; r += kScoreWarps) {
-    const int t = r / (NT * 8), g = r - t * (NT * 8);
-    const float amax =
-        query_codes<HD>(g < G ? q + (int64_t(t0 + t) * Hq + hk * G + g) * HD : nullptr, s_code + r * RS, lane);
-    if (lane == 0) s_amax[r] = amax;
+  // query codes: a warp per (token, head) row, the loads of four rows in flight together
+  constexpr int R = 4;
+  for (int r0 = warp; r0 < n_tok * NT * 8; r0 += kScoreWarps * R) {
+    uint32_t w[R][HD / 64];
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const int r = r0 + u * kScoreWarps, t = r / (NT * 8), g = r - t * (NT * 8);
+      query_load<HD>(t < n_tok && g < G ? q + (int64_t(t0 + t) * Hq + hk * G + g) * HD : nullptr, lane, w[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < R; ++u) {
+      const int r = r0 + u * kScoreWarps;
+      if (r >= n_tok * NT * 8) break;
+      const float amax = query_codes<HD>(w[u], s_code + r * RS, lane);
+      if (lane == 0) s_amax[r] = amax;
+    }
   }
   __syncthreads();
   int nb_max = 0;
@@ -304,7 +316,8 @@ __device__ __forceinline__ bool kth_largest(const uint32_t (&v)[N], int n, int n
 // of the maxima of groups of four keys is a lower bound for it that few more than K keys
 // reach; those are gathered and searched.  Only where that does not apply (fewer groups than
 // K, or too many keys at or above the bound, which takes ties) every key is counted.
-// `load(b)` gives the keys of blocks b .. b + 3.
+// `load(b)` gives the keys of blocks b .. b + 3.  The 3752 selections of 64 among up to 2056 blocks (938
+// rows, 4 heads) take 39 us, a chain of counting rounds each; one selection in a CTA, 3 to 5 us.
 template <int T, int KPT, typename Load>
 __device__ __forceinline__ void select_top(const TopArgs& a, int nb, int32_t* out, Load load) {
   constexpr int kGroups = T > 32 ? 1 : 8;  // (token, head) pairs per CTA
@@ -463,7 +476,9 @@ __global__ void __launch_bounds__(256)
   };
   load(rank * 8 + warp);
   for (int g = warp; g < NT * 8; g += 8) {
-    const float amax = query_codes<HD>(g < G ? q + (int64_t(tok) * Hq + hk * G + g) * HD : nullptr, s_code + g * RS, lane);
+    uint32_t w[HD / 64];
+    query_load<HD>(g < G ? q + (int64_t(tok) * Hq + hk * G + g) * HD : nullptr, lane, w);
+    const float amax = query_codes<HD>(w, s_code + g * RS, lane);
     if (lane == 0) s_amax[g] = amax;
   }
   const int nb = (token_pos(p, a.n_ctx, hk == 0 && rank == 0) + kBlk) / kBlk;
@@ -556,11 +571,11 @@ int launch_score(const uint16_t* q, const int8_t* dig, const float* dig_scale, c
   auto kern = block_score_kernel<HD, NT>;
   if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), smem)) return rc;
   const int groups = ceil_div(m, kTok);
-  // about six CTAs per SM (early tokens see fewer blocks: the spare ones even that out), no more
-  // than there are tiles
+  // about three CTAs per SM, no more than there are tiles: each makes its tokens' codes (938 rows over
+  // 32,896 tokens: selection 96 us, with twelve 117; 100 rows over 131,072: 64, with two or six 77 and 67)
   const int tiles = ceil_div(n_blocks, 16);
-  const int x = std::max(1, std::min(ceil_div(tiles, kScoreWarps), ceil_div(6 * num_sms(), int64_t(groups) * Hk)));
-  launch_pdl(kern, dim3(x, groups, Hk), dim3(kScoreWarps * 32), smem, stream, q, dig, dig_scale, positions, m, t_begin, Hq,
+  const int x = std::max(1, std::min(ceil_div(tiles, kScoreWarps), ceil_div(3 * num_sms(), int64_t(groups) * Hk)));
+  launch_pdl(kern, dim3(x, Hk, groups), dim3(kScoreWarps * 32), smem, stream, q, dig, dig_scale, positions, m, t_begin, Hq,
              Hk, n_ctx, n_blocks, keys);
   CKV_LAUNCH_CHECK("ckv_block_select(score)");
   return CKV_OK;
@@ -652,7 +667,7 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
     if (rc) return rc;
     const TopArgs a{keys, positions, blocks, n, int(t), n_kv_heads, n_ctx, nb, top, sink, recent};
     // a warp per (token, head) while its keys fit the warp's registers, then 128 threads (938 rows
-    // over 32,896 tokens: 114 us, with 256 threads 123) and more
+    // over 32,896 tokens: 39 us, with 256 threads 9 us more) and more
     if (nb <= 512) rc = launch_top<32, 16>(a, s);
     else if (nb <= 1024) rc = launch_top<32, 32>(a, s);
     else if (nb <= 4096) rc = launch_top<128, 32>(a, s);
