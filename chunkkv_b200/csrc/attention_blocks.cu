@@ -23,6 +23,11 @@
 // relative to a running power-of-two reference and rounded to fp16 (2^-12), accumulators,
 // maxima and sums are fp32.  With a bf16 cache P goes in as two bf16 parts (2^-17).
 // The online maximum is lazy: O is rescaled when a row's maximum grew by more than 2^8.
+//
+// Measured: one row over 131,069 tokens (40 heads over 8, e4m3, 269 MB) 49 us, 5.5 TB/s; over 5248
+// tokens (28 over 4) 9.2 us, most of it latency (300 tokens: 6.4); 8 rows over 32,896 tokens 36 us,
+// four row tiles of compute; 938 rows of 64 listed blocks 255 us over a bf16 cache (1.97 GB out
+// of L2, 7.7 TB/s) and 188 us over an 8-bit one (issue slots: widening and the softmax).
 #include <algorithm>
 
 #include "ckv_common.cuh"

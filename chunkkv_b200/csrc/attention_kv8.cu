@@ -23,6 +23,11 @@
 // Warps: 0..3 and 4..7 softmax / epilogue of Q tiles 0 and 1, 8..11 converters, 12 item
 // scheduler, 13 MMA issuer and TMEM owner, 14 and 15 idle.  The 512 threads start with 128
 // registers each; setmaxnreg moves them to the softmax warps (168 + 104 + 72: 65,536 in all).
+//
+// Measured (28 query heads over 4, head_dim 128): 5248 causal rows 246 us, 0.80 PFLOP/s (over a
+// bf16 cache 218 us); 938 rows spread over 5248 keys 77 us (78); 123 rows at the end of 5371 keys
+// 38 us (54).  The tensor pipe and the exponentials are each 38 % busy: what bounds a tile is the
+// chain S -> softmax -> P V of each Q tile, of which two overlap.
 #include <algorithm>
 #include <functional>
 #include <mutex>
