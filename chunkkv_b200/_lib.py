@@ -151,8 +151,12 @@ def last_error() -> str:
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise on failure."""
     rc = getattr(_lib or load(), name)(*args)
-    if rc == CKV_OK:
-        return
+    if rc != CKV_OK:
+        fail(name, rc)
+
+
+def fail(name: str, rc: int) -> None:
+    """Raise what status `rc` of entry point `name` stands for."""
     msg = f"{name}: {last_error()}"
     if rc == CKV_ERR_ARG:
         raise ValueError(msg)

@@ -68,8 +68,10 @@ _TIMER: LaunchTimer | None = None
 
 def _run(name: str, *args, flops: float = 0.0, nbytes: float = 0.0, kernels: int = 1) -> None:
     t = _TIMER
-    if t is None:
-        _lib.call(name, *args)
+    if t is None:  # as _lib.call, without a second packing of the arguments
+        rc = getattr(_lib.load(), name)(*args)
+        if rc:
+            _lib.fail(name, rc)
         return
     e0 = torch.cuda.Event(enable_timing=True)
     e1 = torch.cuda.Event(enable_timing=True)
@@ -737,7 +739,7 @@ class BlockDigest:
     `scale` [H, blocks].  Kept up to date by `block_digest`, or by `kv8_write` for the digest of
     a KV8Cache."""
 
-    __slots__ = ("codes", "scale", "n_ctx")
+    __slots__ = ("codes", "scale", "n_ctx", "n_kv_heads", "head_dim")
 
     def __init__(self, n_kv_heads: int, n_ctx: int, head_dim: int, device="cuda"):
         nb = _n_blocks(n_ctx)
@@ -761,6 +763,7 @@ class BlockDigest:
         _buf("scale", scale, 0, dtype=torch.float32)
         _same_device("codes", codes, scale=scale)
         self.codes, self.scale, self.n_ctx = codes, scale, int(n_ctx)
+        self.n_kv_heads, self.head_dim = codes.shape[0], codes.shape[3]
 
 
 class KV8Cache:
@@ -898,7 +901,7 @@ def kv8_read(cache: KV8Cache, start: int = 0, m: int | None = None) -> tuple[tor
 def block_digest(k_cache: torch.Tensor, digest: BlockDigest, start=0, m: int | None = None) -> BlockDigest:
     """Bring `digest` up to date with a bf16 K cache [H, n_ctx, D] whose tokens [start, start + m)
     are new (`start` an int or an int32 device tensor, m then 1 unless given)."""
-    H, nb, _, D = digest.codes.shape
+    H, D = digest.n_kv_heads, digest.head_dim
     rows, head, row = _rows_view("k_cache", k_cache, H, D)
     if m is None:
         m = 1 if isinstance(start, torch.Tensor) else min(digest.n_ctx, rows) - start
@@ -992,7 +995,7 @@ def block_select(q: torch.Tensor, digest: BlockDigest, positions: torch.Tensor, 
     """For every row of q [m, Hq, D] and KV head the `top` blocks of 16 keys whose score (an upper
     bound of q . k, from the digest) is highest, the first `sink` and the last `recent` visible
     blocks always among them; int32 [m, H, top], ascending, -1 past a row's last visible block."""
-    H, _, _, D = digest.codes.shape
+    H, D = digest.n_kv_heads, digest.head_dim
     m, Hq = _query(q, H, D, positions, m)
     if out is None:
         out = positions.new_empty((m, H, top))  # int32
@@ -1015,19 +1018,25 @@ def _blocks_arg(blocks: torch.Tensor, m: int, H: int) -> int:
     return blocks.shape[2]
 
 
+def _kv_caches(k_cache: torch.Tensor, v_cache: torch.Tensor) -> tuple[int, int, int]:
+    """The shape (H, n_ctx, D) of two contiguous bf16 caches."""
+    shape = k_cache.shape
+    if len(shape) != 3:
+        raise ValueError(f"k_cache: expected shape (H, n_ctx, D), got {tuple(shape)}")
+    if v_cache.shape != shape:
+        raise ValueError(f"k_cache and v_cache differ in shape: {tuple(shape)} and {tuple(v_cache.shape)}")
+    _buf("k_cache", k_cache, 0)
+    _buf("v_cache", v_cache, 0)
+    return shape
+
+
 def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor,
                      blocks: torch.Tensor, out: torch.Tensor | None = None, m: int | None = None,
                      scale: float | None = None) -> torch.Tensor:
     """`attention` restricted to the 16-key blocks listed for each row and KV head (int32
     [m, H, top], ascending, -1 past the end, as `block_select` returns them); bf16 caches
     [H, n_ctx, D].  Rows that see no key give zeros."""
-    if k_cache.dim() != 3:
-        raise ValueError(f"k_cache: expected shape (H, n_ctx, D), got {tuple(k_cache.shape)}")
-    H, n_ctx, D = k_cache.shape
-    _cache("k_cache", k_cache, H, D)
-    _cache("v_cache", v_cache, H, D)
-    if v_cache.shape[1] != n_ctx:
-        raise ValueError("k_cache and v_cache differ in length")
+    H, n_ctx, D = _kv_caches(k_cache, v_cache)
     m, Hq = _query(q, H, D, positions, m)
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
@@ -1072,15 +1081,9 @@ def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
                      scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Block-sparse attention over a bf16 cache: `block_select`, then `attention_blocks`; returns
     (out, blocks).  Without a `digest` that the caller keeps, the whole cache's is built first."""
-    if k_cache.dim() != 3:
-        raise ValueError(f"k_cache: expected shape (H, n_ctx, D), got {tuple(k_cache.shape)}")
-    H, n_ctx, D = k_cache.shape
-    _cache("k_cache", k_cache, H, D)
-    _cache("v_cache", v_cache, H, D)
-    if v_cache.shape[1] != n_ctx:
-        raise ValueError("k_cache and v_cache differ in length")
+    H, n_ctx, D = _kv_caches(k_cache, v_cache)
     m, Hq = _query(q, H, D, positions, m)
-    if digest is not None and (digest.n_ctx != n_ctx or tuple(digest.codes.shape[::3]) != (H, D)):
+    if digest is not None and (digest.n_ctx != n_ctx or digest.n_kv_heads != H or digest.head_dim != D):
         raise ValueError(f"digest of {tuple(digest.codes.shape)} for {digest.n_ctx} tokens does not match the cache "
                          f"{tuple(k_cache.shape)}")
     out, blocks = _sparse_out(q, positions, m, Hq, H, D, top, out, blocks)
