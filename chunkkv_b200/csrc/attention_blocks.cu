@@ -55,6 +55,7 @@ struct Args {
   int64_t head_rows;      // cache rows per head
   int m, Hq, Hk, n_ctx, n_blocks, top, splits, head_tiles;
   float scale_log2;
+  bool after_select;  // launched behind a kernel of the selection, which started when q and positions were complete
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -383,11 +384,25 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   }
   if (threadIdx.x == 0) *abort = 0;
   __syncthreads();
-  pdl_wait();
-  pdl_launch_next();
-
-  // as an operand owner a lane has query rows 8n + g: their positions first, then the first
-  // blocks are on their way while q is loaded
+  // Behind the selection only the lists (and, as ever, the output) wait for the kernel before: it
+  // let this one start after its own wait, so what was written before it is there.
+  if (!a.after_select) pdl_wait();
+  // as an operand owner a lane has query rows 8n + g: q and their positions first
+  uint32_t w[NT][HD / 8];  // the dims of this lane's pieces of K (16 / ES dims each)
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int pr = row0 + 8 * n + g;
+    const bool ok = pr < row_end;
+    const int tok = ok ? pr / G : 0;
+#pragma unroll
+    for (int e = 0; e < HD / 8; e += 4) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (ok)
+        x = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
+                  (B::ES == 2 ? e + c : 8 * (e / 8) + 2 * c + (e / 4) % 2));
+      w[n][e] = x.x, w[n][e + 1] = x.y, w[n][e + 2] = x.z, w[n][e + 3] = x.w;
+    }
+  }
   int pos[NT];
   int last = -1;  // last key any row of the tile sees
 #pragma unroll
@@ -405,6 +420,8 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     pos[n] = p;
     last = max(last, __reduce_max_sync(0xffffffffu, p));
   }
+  if (a.after_select) pdl_wait();
+  pdl_launch_next();
   const int nb = (last + kBlk) / kBlk;  // visible blocks
   const int n_items = LISTED ? a.top : nb;
   const int per = (n_items + a.splits - 1) / a.splits;
@@ -448,32 +465,19 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   State<HD, CT, NT> st;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    // query row 8n + g, the dims of this lane's pieces of K (16 / ES dims each)
-    const int pr = row0 + 8 * n + g;
-    const bool ok = pr < row_end;
-    const int tok = ok ? pr / G : 0;
-    uint32_t w[HD / 8];
-#pragma unroll
-    for (int e = 0; e < HD / 8; e += 4) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (ok)
-        x = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
-                  (B::ES == 2 ? e + c : 8 * (e / 8) + 2 * c + (e / 4) % 2));
-      w[e] = x.x, w[e + 1] = x.y, w[e + 2] = x.z, w[e + 3] = x.w;
-    }
     float factor = a.scale_log2;
     if constexpr (CT == kBf16) {
 #pragma unroll
       for (int t = 0; t < KSTEPS; ++t) {
-        st.qf[n][t][0] = w[2 * t];
-        st.qf[n][t][1] = w[2 * t + 1];
+        st.qf[n][t][0] = w[n][2 * t];
+        st.qf[n][t][1] = w[n][2 * t + 1];
       }
     } else {
       // to fp16 through a power of two that puts the row's largest value in [2^14, 2^15):
       // exact down to 2^-38 of it
       uint32_t mag = 0;
 #pragma unroll
-      for (int e = 0; e < HD / 8; ++e) mag = __vmaxu2(mag, w[e] & 0x7fff7fffu);
+      for (int e = 0; e < HD / 8; ++e) mag = __vmaxu2(mag, w[n][e] & 0x7fff7fffu);
       uint32_t am = max(mag & 0xffffu, mag >> 16);
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = max(am, __shfl_xor_sync(0xffffffffu, am, 2));
@@ -482,8 +486,8 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
       factor *= __uint_as_float(uint32_t(127 - sh) << 23);
 #pragma unroll
       for (int t = 0; t < KSTEPS; ++t) {
-        st.qf[n][t][0] = pack_h2(lo_bf(w[2 * t]) * up, hi_bf(w[2 * t]) * up);
-        st.qf[n][t][1] = pack_h2(lo_bf(w[2 * t + 1]) * up, hi_bf(w[2 * t + 1]) * up);
+        st.qf[n][t][0] = pack_h2(lo_bf(w[n][2 * t]) * up, hi_bf(w[n][2 * t]) * up);
+        st.qf[n][t][1] = pack_h2(lo_bf(w[n][2 * t + 1]) * up, hi_bf(w[n][2 * t + 1]) * up);
       }
     }
     // as a column owner: rows 8n + 2c and 8n + 2c + 1
@@ -866,7 +870,7 @@ int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8
                          void* workspace, cudaStream_t stream) {
   const int nb = ceil_div(n_ctx, kBlk);
   Args a{q, k8, v8, ks, vs, positions, nullptr, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, 0, 1, 1,
-         scale * 1.4426950408889634f};
+         scale * 1.4426950408889634f, false};
   const Plan p = plan(m, Hq / Hk, Hk, HD, 1, nb, false);
   if (int rc = check("ckv_attention_kv8", a, HD, p.tiles)) return rc;
   if (HD == 128)
@@ -925,26 +929,41 @@ static int attention_blocks(const char* name, Args a, int HD, int type, void* wo
   return CKV_OK;
 }
 
+static int attention_blocks_bf16(const char* name, const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                 const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD,
+                                 int n_ctx, int top, float scale, void* workspace, int64_t ws_bytes, cudaStream_t s, bool after_select) {
+  const Args a{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr,
+               positions, blocks, out, nullptr, nullptr, int64_t(n_ctx), m, Hq, Hk, n_ctx, ceil_div(n_ctx, kBlk),
+               top, 1, 1, scale * 1.4426950408889634f, after_select};
+  return attention_blocks(name, a, HD, -1, workspace, ws_bytes, s);
+}
+
+static int attention_blocks_8bit(const char* name, const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
+                                 const float* v_scale, const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq,
+                                 int Hk, int HD, int n_ctx, int top, float scale, int type, void* workspace, int64_t ws_bytes,
+                                 cudaStream_t s, bool after_select) {
+  CKV_REQUIRE(type == CKV_KV8_INT8 || type == CKV_KV8_E4M3, "%s: type %d", name, type);
+  CKV_REQUIRE(m == 0 || (k_scale && v_scale), "%s: null scales", name);
+  const int nb = ceil_div(n_ctx, kBlk);
+  const Args a{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq,
+               Hk, n_ctx, nb, top, 1, 1, scale * 1.4426950408889634f, after_select};
+  return attention_blocks(name, a, HD, type, workspace, ws_bytes, s);
+}
+
 extern "C" int ckv_attention_blocks(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
                                     const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int n_q_heads,
                                     int n_kv_heads, int head_dim, int n_ctx, int top, float scale, void* workspace,
                                     int64_t workspace_bytes, ckv_stream_t stream) {
-  const Args a{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr,
-               positions, blocks, out, nullptr, nullptr, int64_t(n_ctx), m, n_q_heads, n_kv_heads, n_ctx, ceil_div(n_ctx, kBlk),
-               top, 1, 1, scale * 1.4426950408889634f};
-  return attention_blocks("ckv_attention_blocks", a, head_dim, -1, workspace, workspace_bytes, as_stream(stream));
+  return attention_blocks_bf16("ckv_attention_blocks", q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim,
+                               n_ctx, top, scale, workspace, workspace_bytes, as_stream(stream), false);
 }
 
 extern "C" int ckv_attention_blocks_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
                                         const float* v_scale, const int32_t* positions, const int32_t* blocks, uint16_t* out,
                                         int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top, float scale,
                                         int type, void* workspace, int64_t workspace_bytes, ckv_stream_t stream) {
-  CKV_REQUIRE(type == CKV_KV8_INT8 || type == CKV_KV8_E4M3, "ckv_attention_blocks_kv8: type %d", type);
-  CKV_REQUIRE(m == 0 || (k_scale && v_scale), "ckv_attention_blocks_kv8: null scales");
-  const int nb = ceil_div(n_ctx, kBlk);
-  const Args a{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, n_q_heads,
-               n_kv_heads, n_ctx, nb, top, 1, 1, scale * 1.4426950408889634f};
-  return attention_blocks("ckv_attention_blocks_kv8", a, head_dim, type, workspace, workspace_bytes, as_stream(stream));
+  return attention_blocks_8bit("ckv_attention_blocks_kv8", q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads,
+                               head_dim, n_ctx, top, scale, type, workspace, workspace_bytes, as_stream(stream), false);
 }
 
 extern "C" int64_t ckv_attention_sparse_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top,
@@ -975,8 +994,8 @@ extern "C" int ckv_attention_sparse(const uint16_t* q, const uint16_t* k_cache, 
   if (int rc = ckv_block_select(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
                                 recent, workspace, x.step, stream))
     return rc;
-  return ckv_attention_blocks(q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, scale,
-                              workspace, x.step, stream);
+  return attention_blocks_bf16("ckv_attention_sparse", q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim,
+                               n_ctx, top, scale, workspace, x.step, as_stream(stream), true);
 }
 
 extern "C" int ckv_attention_sparse_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
@@ -991,6 +1010,6 @@ extern "C" int ckv_attention_sparse_kv8(const uint16_t* q, const uint8_t* k8, co
   if (int rc = ckv_block_select(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
                                 recent, workspace, workspace_bytes, stream))
     return rc;
-  return ckv_attention_blocks_kv8(q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx,
-                                  top, scale, type, workspace, workspace_bytes, stream);
+  return attention_blocks_8bit("ckv_attention_sparse_kv8", q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads,
+                               head_dim, n_ctx, top, scale, type, workspace, workspace_bytes, as_stream(stream), true);
 }
