@@ -862,6 +862,12 @@ int check_space(const char* name, int m, int Hq, int Hk, int HD, int es, int n_c
 int64_t kv8_stream_workspace(int m, int Hq, int Hk, int HD, int n_ctx) {
   return plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false).bytes;
 }
+// Steps (of a warp, over a pair of blocks) that the call's CTAs make one after the other.
+int64_t kv8_stream_steps(int m, int Hq, int Hk, int HD, int n_ctx) {
+  const Plan p = plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false);
+  const int64_t waves = ceil_div(int64_t(p.tiles) * Hk * p.splits, num_sms());
+  return waves * ceil_div(ceil_div(n_ctx, kBlk), int64_t(p.splits) * 8 * Block<128, kInt8>::NB);
+}
 int kv8_stream_launches(int m, int Hq, int Hk, int HD, int n_ctx) {
   return launches(plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false));
 }

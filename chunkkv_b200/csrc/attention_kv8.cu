@@ -1,7 +1,7 @@
 // Attention over the 8-bit K/V cache (one fp32 scale per KV head and block of 16 tokens).
 //
-// Few packed rows (token x head of a group) stream the cache through attention_blocks.cu;
-// past kStreamRows rows, the tcgen05 kernel below takes them in 128-row tiles.
+// Few packed rows (token x head of a group), and more over short contexts, stream the cache
+// through attention_blocks.cu; the others the tcgen05 kernel below takes in 128-row tiles.
 //
 // It is the bf16 kernel's scheme (attention_tc.cu: two Q tiles per CTA, S and P in TMEM,
 // lazy rescale, persistent items, key splits) with the operands made on the SM: a warpgroup
@@ -26,7 +26,7 @@
 //
 // Measured (28 query heads over 4, head_dim 128): 5248 causal rows 246 us, 0.80 PFLOP/s (over a
 // bf16 cache 218 us); 938 rows spread over 5248 keys 77 us (78); 123 rows at the end of 5371 keys
-// 38 us (54).  The tensor pipe and the exponentials are each 38 % busy: what bounds a tile is the
+// 32 us (54).  The tensor pipe and the exponentials are each 38 % busy: what bounds a tile is the
 // chain S -> softmax -> P V of each Q tile, of which two overlap.
 #include <algorithm>
 #include <functional>
@@ -43,6 +43,7 @@ namespace ckv {
 // attention_blocks.cu
 int64_t kv8_stream_workspace(int m, int Hq, int Hk, int HD, int n_ctx);
 int kv8_stream_launches(int m, int Hq, int Hk, int HD, int n_ctx);
+int64_t kv8_stream_steps(int m, int Hq, int Hk, int HD, int n_ctx);
 int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* ks, const float* vs,
                          const int32_t* positions, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, float scale, int type,
                          void* workspace, cudaStream_t stream);
@@ -823,18 +824,22 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kv8_kernel(const __grid
   }
 }
 
-// Packed rows per KV head up to which attention_blocks.cu takes the call, 16 rows to a tile, each
-// streaming the cache.  At 28/4 heads, 56 rows (four tiles) take 15.8 / 35.8 / 116 us over 8192 /
-// 32,896 / 131,072 keys there and 30.8 / 49.2 / 134 us here; 84 rows 18.7 / 48.8 / 169 and
-// 31.8 / 49.4 / 134 us.
-constexpr int kStreamRows = 64;
-bool use_tiles(int m, int Hq, int Hk) { return int64_t(m) * (Hq / Hk) > kStreamRows; }
+// attention_blocks.cu takes the call (16 packed rows of a KV head to a tile, each streaming the
+// cache) with up to kStreamRows packed rows, and with more while its CTAs make few steps: a step
+// takes 1.8 us, as much as 6 of them cost here what an item's start, epilogue and join do.  Streamed
+// and in tiles, 28 heads over 4: 8 rows over 32,896 keys 35 and 40 us; 10 rows over 4096 / 8192 /
+// 16,384 keys 13 / 17 / 26 (10 steps) and 19 / 22 / 26; 36 rows over 512 / 2048 / 4096 keys
+// 11 / 17 / 24 (8 steps) and 20 / 19 / 22 us.
+constexpr int kStreamRows = 64, kStreamSteps = 6;
+bool use_tiles(int m, int Hq, int Hk, int HD, int n_ctx) {
+  return int64_t(m) * (Hq / Hk) > kStreamRows && kv8_stream_steps(m, Hq, Hk, HD, n_ctx) > kStreamSteps;
+}
 
 // Costs in key-tile times (2.5 us at head_dim 128), fitted to the times of every split length at
 // eight shapes of 36 to 938 rows over 2048 to 32,896 keys (within 5 % of the best choice at
 // each): an item's start and epilogue, the same with fp32 partials, and the second launch that
 // joins them, alone, per split (a row's splits are added one after the other) and per byte.
-constexpr double kItemCost = 0.5, kSplitItemCost = 3.0, kJoinCost = 1.0, kJoinSplitCost = 0.2, kJoinBytes = 5e6;
+constexpr double kItemCost = 0.5, kSplitItemCost = 3.0, kJoinCost = 1.0, kJoinSplitCost = 0.1, kJoinBytes = 5e6;
 
 constexpr int kMaxSms = 256;
 
@@ -960,9 +965,7 @@ int launch_tiles(Args a, const SplitPlan& p, void* workspace, cudaStream_t strea
   launch_pdl(kern, dim3(int(std::min<int64_t>(n_slots, num_sms()))), dim3(kThreads), Cfg<HD>::SMEM, stream, a);
   CKV_LAUNCH_CHECK("ckv_attention_kv8");
   if (p.max_splits > 1) {
-    launch_pdl(attention_combine_kernel<HD>, dim3(p.blocks * (NQ * BM / (kCombineWarps * kCombineRows)), a.Hk),
-               dim3(kCombineWarps * 32), 0, stream, a.positions, a.out, a.M, a.Hq, a.Hk, a.n_ctx, p.tps, p.max_splits,
-               static_cast<const float*>(a.part_o), static_cast<const float2*>(a.part_ml));
+    launch_combine<HD>(p.blocks, a.positions, a.out, a.M, a.Hq, a.Hk, a.n_ctx, p.tps, p.max_splits, a.part_o, a.part_ml, stream);
     CKV_LAUNCH_CHECK("ckv_attention_kv8(combine)");
   }
   return CKV_OK;
@@ -970,7 +973,7 @@ int launch_tiles(Args a, const SplitPlan& p, void* workspace, cudaStream_t strea
 
 bool shape_ok(int m, int Hq, int Hk, int HD, int n_ctx) {
   return m > 0 && Hk > 0 && Hk <= 65535 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 128 && (HD == 64 || HD == 128) && n_ctx > 0 &&
-         n_ctx <= (1 << 30);
+         n_ctx <= (1 << 30) && int64_t(m) * Hq <= (int64_t(1) << 31) - (1 << 20);  // row numbers stay within 32 bits
 }
 
 }  // namespace
@@ -980,13 +983,13 @@ using namespace ckv;
 
 extern "C" int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
-  return use_tiles(m, n_q_heads, n_kv_heads) ? kSchedBytes + tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
+  return use_tiles(m, n_q_heads, n_kv_heads, head_dim, n_ctx) ? kSchedBytes + tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx).bytes
                                              : kv8_stream_workspace(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
 extern "C" int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
-  if (use_tiles(m, n_q_heads, n_kv_heads))
+  if (use_tiles(m, n_q_heads, n_kv_heads, head_dim, n_ctx))
     return tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx).max_splits > 1 ? 2 : 1;
   return kv8_stream_launches(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
@@ -1000,8 +1003,8 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
               "ckv_attention_kv8: bad sizes (%d rows, %d query heads, %d KV heads, context %d)", m, n_q_heads, n_kv_heads, n_ctx);
   if (m == 0) return CKV_OK;
   if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) {
-    set_error("ckv_attention_kv8: head_dim %d (64 or 128), %d query heads per KV head (at most 128), context %d", head_dim,
-              n_q_heads / n_kv_heads, n_ctx);
+    set_error("ckv_attention_kv8: head_dim %d (64 or 128), %d query heads per KV head (at most 128), context %d, %d rows", head_dim,
+              n_q_heads / n_kv_heads, n_ctx, m);
     return CKV_ERR_UNSUPPORTED;
   }
   CKV_REQUIRE(scale >= 0.f && scale <= 3.0e38f, "ckv_attention_kv8: scale %g (finite, not negative)", double(scale));
@@ -1012,7 +1015,7 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
   CKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
               "ckv_attention_kv8: workspace of %lld bytes, needs %lld (16-byte aligned)", static_cast<long long>(workspace_bytes),
               static_cast<long long>(need));
-  if (!use_tiles(m, n_q_heads, n_kv_heads))
+  if (!use_tiles(m, n_q_heads, n_kv_heads, head_dim, n_ctx))
     return kv8_stream_attention(q, k8, v8, k_scale, v_scale, positions, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, scale, type,
                                 workspace, as_stream(stream));
   const Args a{q, k8, v8, k_scale, v_scale, positions, out, nullptr, nullptr, nullptr, m, n_q_heads, n_kv_heads, n_ctx,

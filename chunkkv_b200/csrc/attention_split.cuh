@@ -49,19 +49,16 @@ constexpr uint32_t kStageBytes = NQ * 4 * 32 * kStageStride * 4;
 
 // Merge the key splits of the row blocks that were split: O = sum_s 2^(m_s - M) O_s /
 // sum_s 2^(m_s - M) l_s with M = max_s m_s (all in the log2 domain of the kernel).
-// A warp takes kCombineRows packed rows; for each, lane s reads split s's (m, l), then
-// each lane sums its four columns over the splits, the loads of all its rows in flight
-// together (one wave of CTAs at the 7B shape).  Rows of unsplit blocks were written
-// directly.
+// A warp takes R packed rows; for each, lane s reads split s's (m, l), then each lane sums its
+// four columns over the splits, the loads of all its rows in flight together.  Rows of
+// unsplit blocks were written directly.
 constexpr int kCombineWarps = 8;
-constexpr int kCombineRows = 4;
-template <int HD>
+template <int HD, int R>
 __global__ void __launch_bounds__(kCombineWarps * 32, 4) attention_combine_kernel(
     const int32_t* __restrict__ positions, uint16_t* __restrict__ out, int M, int Hq, int Hk, int n_ctx,
     int tps, int max_splits, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
   pdl_wait();  // the partials come from the attention kernel just before (dependent launch)
   pdl_launch_next();
-  constexpr int R = kCombineRows;
   const int G = Hq / Hk;
   const int T = BM / G;
   constexpr int kChunks = NQ * BM / (kCombineWarps * R);  // CTAs per (row block, KV head)
@@ -111,7 +108,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32, 4) attention_combine_kerne
   float4 acc[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+#pragma unroll(R == 1 ? 4 : 2)
   for (int sp = 0; sp < n_split; ++sp) {
     const float* ps = po + int64_t(sp) * NQ * BM * HD;
 #pragma unroll
@@ -131,6 +128,21 @@ __global__ void __launch_bounds__(kCombineWarps * 32, 4) attention_combine_kerne
     if (mine && ok[i])
       *reinterpret_cast<uint2*>(out + orow[i] + 4 * lane) =
           make_uint2(pack_bf2(acc[i].x * inv[i], acc[i].y * inv[i]), pack_bf2(acc[i].z * inv[i], acc[i].w * inv[i]));
+}
+
+// One row per warp while the warps of four rows each would not fill the SMs four CTAs deep (7 heads
+// over 4: 36 rows over 5371 keys 29.1 -> 22.5 us with the attention, 123 rows 37.9 -> 33, 300 rows
+// 51.0 -> 47), then four (938 rows over 5248 keys: 76 us, one row per warp 78).
+template <int HD>
+void launch_combine(int blocks, const int32_t* positions, uint16_t* out, int M, int Hq, int Hk, int n_ctx, int tps, int max_splits,
+                    const float* part_o, const float2* part_ml, cudaStream_t stream) {
+  const int64_t ctas = int64_t(blocks) * Hk * (NQ * BM / (kCombineWarps * 4));
+  if (ctas < 4 * num_sms())
+    launch_pdl(attention_combine_kernel<HD, 1>, dim3(blocks * (NQ * BM / kCombineWarps), Hk), dim3(kCombineWarps * 32), 0, stream,
+               positions, out, M, Hq, Hk, n_ctx, tps, max_splits, part_o, part_ml);
+  else
+    launch_pdl(attention_combine_kernel<HD, 4>, dim3(blocks * (NQ * BM / (kCombineWarps * 4)), Hk), dim3(kCombineWarps * 32), 0, stream,
+               positions, out, M, Hq, Hk, n_ctx, tps, max_splits, part_o, part_ml);
 }
 
 // Key-split plan: split only when the unsplit grid leaves SMs idle.

@@ -1020,9 +1020,7 @@ int launch(const uint16_t* q, const uint16_t* kc, const uint16_t* vc, const int3
              n_ctx, sl2, p.tps, p.max_splits, p.blocks, sched, part_o, part_ml);
   CKV_LAUNCH_CHECK("ckv_attention");
   if (p.max_splits > 1) {
-    launch_pdl(attention_combine_kernel<HD>, dim3(p.blocks * (NQ * BM / (kCombineWarps * kCombineRows)), Hk),
-               dim3(kCombineWarps * 32), 0, stream, positions, out, M, Hq, Hk, n_ctx, p.tps, p.max_splits,
-               static_cast<const float*>(part_o), static_cast<const float2*>(part_ml));
+    launch_combine<HD>(p.blocks, positions, out, M, Hq, Hk, n_ctx, p.tps, p.max_splits, part_o, part_ml, stream);
     CKV_LAUNCH_CHECK("ckv_attention(combine)");
   }
   return CKV_OK;

@@ -374,3 +374,18 @@ def test_tiles_in_two_graphs_at_once(m, n):
                 g.replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Hq,H,D,n,m", [(28, 4, 128, 900, 700), (14, 2, 64, 130, 3001), (40, 8, 128, 1300, 401), (4, 4, 128, 17, 9000),
+                                        (16, 1, 64, 5000, 37), (7, 1, 128, 2500, 63), (128, 1, 64, 700, 90)])
+def test_many_rows_in_tiles(Hq, H, D, n, m, dtype):
+    """Shapes that the tile kernel takes: long or short contexts, half-filled tiles, odd ends."""
+    c, k, v = filled(H, n, D, dtype, seed=n)
+    kd, vd = ref.values(c.k.float(), c.k_scale), ref.values(c.v.float(), c.v_scale)
+    q = queries(m, Hq, D, m)
+    g = torch.Generator().manual_seed(m)
+    p = torch.randint(-1, n, (m,), generator=g, dtype=torch.int32).to(DEV)
+    p[0], p[m - 1] = n - 1, -1
+    check_attention(ops.attention_kv8(q, c, p), q, kd, vd, p)
+    check_attention(ops.attention_kv8(q, c, p.sort().values), q, kd, vd, p.sort().values)

@@ -199,6 +199,9 @@ def test_entry_points_refuse_scales_and_row_counts():
     with pytest.raises(ValueError, match="bad sizes"):
         _lib.call("ckv_attention_sparse", *(P,) * 8, many, 4, 2, 64, 800, 4, 1, 1, 1.0, P, 1 << 40, None)
     assert _lib.load().ckv_attention_blocks_workspace_size(many, 4, 2, 64, 4, 16) == 0
+    with pytest.raises(NotImplementedError, match=f"{many} rows"):
+        _lib.call("ckv_attention_kv8", *(P,) * 7, many, 4, 2, 64, 100, 1.0, 0, P, 1 << 40, None)
+    assert _lib.load().ckv_attention_kv8_workspace_size(many, 4, 2, 64, 100) == 0
 
 
 def test_direct_calls_convert_like_ctypes():
