@@ -26,7 +26,7 @@
 //
 // Measured (28 query heads over 4, head_dim 128): 5248 causal rows 246 us, 0.80 PFLOP/s (over a
 // bf16 cache 218 us); 938 rows spread over 5248 keys 77 us (78); 123 rows at the end of 5371 keys
-// 32 us (54).  The tensor pipe and the exponentials are each 38 % busy: what bounds a tile is the
+// 32 us (39).  The tensor pipe and the exponentials are each 38 % busy: what bounds a tile is the
 // chain S -> softmax -> P V of each Q tile, of which two overlap.
 #include <algorithm>
 #include <functional>
