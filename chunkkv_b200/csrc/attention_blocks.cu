@@ -27,7 +27,7 @@
 // Measured: one row over 131,069 tokens (40 heads over 8, e4m3, 269 MB) 49 us, 5.5 TB/s; over 5248
 // tokens (28 over 4) 9.2 us, most of it latency (300 tokens: 6.4); 8 rows over 32,896 tokens 36 us,
 // four row tiles of compute; 938 rows of 64 listed blocks 255 us over a bf16 cache (1.97 GB out
-// of L2, 7.7 TB/s) and 188 us over an 8-bit one (issue slots: widening and the softmax).
+// of L2, 7.7 TB/s) and 173 us over an 8-bit one (issue slots: widening and the softmax).
 #include <algorithm>
 
 #include "ckv_common.cuh"
@@ -117,18 +117,19 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(addr) : "memory");
   return r;
 }
-// A stage holds NB blocks: their 16 rows of K each, then their 16 rows of V.  A warp works on
-// the NB blocks together: two independent chains of mma and exponentials, one wait and one
-// request (a warp's latency, not the issue rate, bounds the kernel).  Two where a pair is at
-// most 8 KiB, so that twelve warps keep two stages each.
-template <int HD, int CT>
+// A stage holds NB blocks: their 16 rows of K each, then their 16 rows of V.  Over a whole cache of
+// 8 bits a warp works on two together: two independent chains of mma and exponentials, one wait
+// and one request (131,069 tokens, 8 heads: 50 us, one by one 53; 8 rows over 32,896 tokens 35 and
+// 39).  One by one where lists give a warp few blocks (938 rows of 64 blocks: 173 us, in pairs 183; 60
+// rows 21.6 and 22.9), and where a pair of stages would not fit twelve warps (bf16).
+template <int HD, int CT, bool LISTED>
 struct Block {
   static constexpr int ES = CT == kBf16 ? 2 : 1;
   static constexpr int ROW = HD * ES;         // bytes of a row
   static constexpr int KW = HD / 4 * ES / 4;  // 32-bit words of K per key and lane (a multiple of 4)
   static constexpr int VW = HD / 8 * ES / 4;  // of V (2 or a multiple of 4)
   static constexpr int HALF = kBlk * ROW;     // bytes of one block's K
-  static constexpr int NB = 4 * HALF <= 8192 ? 2 : 1;
+  static constexpr int NB = !LISTED && 4 * HALF <= 8192 ? 2 : 1;
   static constexpr int STAGE = 2 * NB * HALF;
 
   // The warp: the rows that exist of blocks ids (a bf16 cache may end inside a block; -1: none).
@@ -187,7 +188,7 @@ struct Block {
 };
 
 // Running state of a warp: for each of its 8 NT query rows a maximum and a sum, and O.
-template <int HD, int CT, int NT>
+template <int HD, int CT, int NT, bool LISTED>
 struct State {
   static constexpr int KSTEPS = HD / 16;
   uint32_t qf[NT][KSTEPS][2];
@@ -198,10 +199,10 @@ struct State {
   float o[NT][KSTEPS][4];  // the lane's V dims 2t, 2t + 1 x rows 2c, 2c + 1
 
   // The blocks ids of a stage (-1: none) with their scales; `last`: the last key any row sees.
-  __device__ __forceinline__ void step(const uint8_t* stage, const int (&ids)[Block<HD, CT>::NB],
-                                       const float (&ks)[Block<HD, CT>::NB], const float (&vs)[Block<HD, CT>::NB], int last,
+  __device__ __forceinline__ void step(const uint8_t* stage, const int (&ids)[Block<HD, CT, LISTED>::NB],
+                                       const float (&ks)[Block<HD, CT, LISTED>::NB], const float (&vs)[Block<HD, CT, LISTED>::NB], int last,
                                        int lane) {
-    using B = Block<HD, CT>;
+    using B = Block<HD, CT, LISTED>;
     constexpr int NB = B::NB;
     const int g = lane >> 2;
     float s[NB][NT][4], s2[NB][NT][4];  // even and odd steps of the contraction: half the length of the chain
@@ -342,13 +343,13 @@ struct State {
 
 // Shared memory: W rings of stages; after the loop the same space takes the warps' states, and
 // behind it the CTA's joined state (read by the cluster's other CTAs) and the barriers.
-template <int HD, int CT, int NT, int W>
+template <int HD, int CT, int NT, int W, bool LISTED>
 struct Layout {
   static constexpr int ROWS = 8 * NT;
   // two stages where more CTAs (W = 4) or warps share the SM: at 938 rows of 64 listed blocks three
-  // CTAs of two stages take 255 us (bf16) and 183 us (8 bits), two of three 303 and 241 us
+  // CTAs of two stages take 255 us (bf16) and 173 us (8 bits), of three 303 (two CTAs) and 176 us
   static constexpr int STAGES = W == 8 ? 3 : 2;
-  static constexpr int RING = STAGES * Block<HD, CT>::STAGE;
+  static constexpr int RING = STAGES * Block<HD, CT, LISTED>::STAGE;
   static constexpr int STRIDE = HD + 4;  // floats of a state row
   static constexpr int STATES = W * ROWS * (STRIDE + 2) * 4;
   static constexpr int JOINED = (W * RING > STATES ? W * RING : STATES + 15) / 16 * 16;
@@ -364,8 +365,8 @@ struct Layout {
 template <int HD, int CT, int NT, bool LISTED, int W, bool JOIN>
 __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     attention_blocks_kernel(const __grid_constant__ Args a) {
-  using L = Layout<HD, CT, NT, W>;
-  using B = Block<HD, CT>;
+  using L = Layout<HD, CT, NT, W, LISTED>;
+  using B = Block<HD, CT, LISTED>;
   constexpr int KSTEPS = HD / 16, ROWS = L::ROWS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
 #pragma unroll
   for (int s = 0; s < L::STAGES; ++s) fill(s, i + s * W * NB);
 
-  State<HD, CT, NT> st;
+  State<HD, CT, NT, LISTED> st;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     float factor = a.scale_log2;
@@ -716,7 +717,8 @@ struct Plan {
 };
 
 // Bytes of cache that one CTA of a cluster streams at most: beyond, the few SMs of the clusters
-// would be slower than all SMs with a second kernel for the join.
+// are slower than all SMs with a second kernel for the join (one row of 4 KV heads, in clusters and split:
+// 1024 tokens 6.4 and 6.9 us, 5248 9.1 and 8.5 and the host's 3 us for a second launch, 8192 10.8 and 8.7).
 constexpr int64_t kClusterBytes = 192 * 1024;
 
 // CTAs of clusters that surely run at once: eight to a GPC's SMs, one each (its shared memory is
@@ -753,7 +755,7 @@ int launch(Args a, const Plan& p, void* workspace, cudaStream_t stream) {
     // 12 warps where pairs of blocks halve the steps (5248 tokens: 9.2 us, with eight 9.6; 64 to 128 listed
     // blocks: 6.9 and 7.3); eight with three stages over a bf16 cache (32 blocks: 5.7 us, with twelve 5.9)
     constexpr int WJ = NT == 1 && CT != kBf16 ? 12 : 8;
-    using L = Layout<HD, CT, NT, WJ>;
+    using L = Layout<HD, CT, NT, WJ, LISTED>;
     auto kern = attention_blocks_kernel<HD, CT, NT, LISTED, WJ, true>;
     if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), L::BYTES)) return rc;
     cudaLaunchConfig_t cfg = {};
@@ -779,7 +781,7 @@ int launch(Args a, const Plan& p, void* workspace, cudaStream_t stream) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + int64_t(p.splits) * p.tiles * a.Hk * 8 * NT * HD);
   }
   constexpr int W = LISTED ? 4 : NT == 2 ? 8 : 12;
-  using L = Layout<HD, CT, NT, W>;
+  using L = Layout<HD, CT, NT, W, LISTED>;
   auto kern = attention_blocks_kernel<HD, CT, NT, LISTED, W, false>;
   if (int rc = set_smem_limit(reinterpret_cast<const void*>(kern), L::BYTES)) return rc;
   launch_pdl(kern, dim3(p.splits, p.tiles, a.Hk), dim3(W * 32), L::BYTES, stream, a);
@@ -866,7 +868,7 @@ int64_t kv8_stream_workspace(int m, int Hq, int Hk, int HD, int n_ctx) {
 int64_t kv8_stream_steps(int m, int Hq, int Hk, int HD, int n_ctx) {
   const Plan p = plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false);
   const int64_t waves = ceil_div(int64_t(p.tiles) * Hk * p.splits, num_sms());
-  return waves * ceil_div(ceil_div(n_ctx, kBlk), int64_t(p.splits) * 8 * Block<128, kInt8>::NB);
+  return waves * ceil_div(ceil_div(n_ctx, kBlk), int64_t(p.splits) * 8 * Block<128, kInt8, false>::NB);
 }
 int kv8_stream_launches(int m, int Hq, int Hk, int HD, int n_ctx) {
   return launches(plan(m, Hq / Hk, Hk, HD, 1, ceil_div(n_ctx, kBlk), false));

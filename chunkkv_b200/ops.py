@@ -863,7 +863,9 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start, m: int |
     scale per KV head and block of 16 tokens.  Token t's row is row t - start of `k` and `v`, or
     row t with `by_position` (a cache-shaped source).  `start` is an int, or an int32 device
     tensor (then `m` rows are read from wherever it points at launch: a captured call serves
-    every later position).  `m` defaults to all rows (1 for a device `start`)."""
+    every later position).  `m` defaults to all rows (1 for a device `start`).  The written tokens
+    are the block's last: rows behind them in the same block become zeros (they share its scale),
+    later blocks stay as they were."""
     H, D = cache.n_kv_heads, cache.head_dim
     rows, k_head, k_row = _rows_view("k", k, H, D)
     v_rows, v_head, v_row = _rows_view("v", v, H, D)
