@@ -412,7 +412,7 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
  * meet the codes in fp16, relative to the largest value scale of the keys worked on together:
  * an output is exact to 2^-31 of the largest value there, so a row that sees only values smaller
  * than 2^-20 of it loses bits.  `scale` is finite and not negative (a negative one is refused).
- * At most 128 query heads per KV head, head_dim 64 or 128.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
+ * At most 128 query heads per KV head, head_dim 64 or 128, m * n_q_heads at most 2^31 - 2^20.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
  * 0) needs no initialisation; calls that share one must not overlap on the GPU. */
 CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 /* Kernels one ckv_attention_kv8 call launches at this shape (0 for a shape it refuses). */
@@ -440,7 +440,7 @@ CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const f
 /* Attention of row i over the keys j <= positions[i] of the blocks listed for it (ascending, -1
  * past the end; an entry out of range or not above the one before it is skipped and recorded as
  * CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache (cache_bits 16 or 8).
- * Rows that see no key give zeros.  `scale` as in ckv_attention_kv8; m * n_q_heads below 2^31 - 2^20. */
+ * Rows that see no key give zeros.  `scale` as in ckv_attention_kv8; m * n_q_heads at most 2^31 - 2^20. */
 CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top,
                                                     int cache_bits);
 CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int cache_bits);
