@@ -117,6 +117,12 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(addr) : "memory");
   return r;
 }
+// What a row's partial maxima are taken relative to when they are joined: their maximum m, or 0
+// when there is none.  Scores of NaN never become a maximum, but they make the partial sum
+// and O NaN, which a weight of 0 does not silence: the row comes out as NaN.  One that saw no
+// key has sums of 0 everywhere and comes out as zeros.
+__device__ __forceinline__ float join_base(float m) { return m == -INFINITY ? 0.f : m; }
+
 // A stage holds NB blocks: their 16 rows of K each, then their 16 rows of V.  Over a whole cache of
 // 8 bits a warp works on two together: two independent chains of mma and exponentials, one wait
 // and one request (131,069 tokens, 8 heads: 50 us, one by one 53; 8 rows over 32,896 tokens 35 and
@@ -582,19 +588,18 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     float m = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; ++w) m = fmaxf(m, s_m[w * ROWS + row]);
+    const float base = join_base(m);
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (m > -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float wt = ex2_approx(s_m[w * ROWS + row] - m);
-        const float4 x = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * L::STRIDE + col);
-        l = fmaf(wt, s_l[w * ROWS + row], l);
-        o.x = fmaf(wt, x.x, o.x);
-        o.y = fmaf(wt, x.y, o.y);
-        o.z = fmaf(wt, x.z, o.z);
-        o.w = fmaf(wt, x.w, o.w);
-      }
+    for (int w = 0; w < W; ++w) {
+      const float wt = ex2_approx(s_m[w * ROWS + row] - base);
+      const float4 x = *reinterpret_cast<const float4*>(s_o + (w * ROWS + row) * L::STRIDE + col);
+      l = fmaf(wt, s_l[w * ROWS + row], l);
+      o.x = fmaf(wt, x.x, o.x);
+      o.y = fmaf(wt, x.y, o.y);
+      o.z = fmaf(wt, x.z, o.z);
+      o.w = fmaf(wt, x.w, o.w);
     }
     if constexpr (JOIN) {
       *reinterpret_cast<float4*>(j_o + row * L::STRIDE + col) = o;
@@ -622,19 +627,18 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
         mr[r] = ld_cluster(cluster_smem_addr(j_o + ROWS * L::STRIDE + row, r));
         m = fmaxf(m, mr[r]);
       }
+      const float base = join_base(m);
       float l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (m > -INFINITY) {
 #pragma unroll
-        for (int r = 0; r < kCluster; ++r) {
-          const float wt = ex2_approx(mr[r] - m);
-          const float4 x = ld_cluster4(cluster_smem_addr(j_o + row * L::STRIDE + col, r));
-          l = fmaf(wt, ld_cluster(cluster_smem_addr(j_o + ROWS * (L::STRIDE + 1) + row, r)), l);
-          o.x = fmaf(wt, x.x, o.x);
-          o.y = fmaf(wt, x.y, o.y);
-          o.z = fmaf(wt, x.z, o.z);
-          o.w = fmaf(wt, x.w, o.w);
-        }
+      for (int r = 0; r < kCluster; ++r) {
+        const float wt = ex2_approx(mr[r] - base);
+        const float4 x = ld_cluster4(cluster_smem_addr(j_o + row * L::STRIDE + col, r));
+        l = fmaf(wt, ld_cluster(cluster_smem_addr(j_o + ROWS * (L::STRIDE + 1) + row, r)), l);
+        o.x = fmaf(wt, x.x, o.x);
+        o.y = fmaf(wt, x.y, o.y);
+        o.z = fmaf(wt, x.z, o.z);
+        o.w = fmaf(wt, x.w, o.w);
       }
       store_row(row0 + row, col, o, l);
     }
@@ -679,20 +683,19 @@ __global__ void __launch_bounds__(256) attention_blocks_join_kernel(const __grid
   m = s_red[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) m = fmaxf(m, s_red[i]);
+  const float base = join_base(m);
   float l = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (m > -INFINITY) {
 #pragma unroll 4
-    for (int s = grp; s < a.splits; s += GROUPS) {
-      const float2 ml = __ldcg(&a.part_ml[s * stride + at]);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + (s * stride + at) * HD + col));
-      const float wt = ex2_approx(ml.x - m);
-      l = fmaf(wt, ml.y, l);
-      o.x = fmaf(wt, x.x, o.x);
-      o.y = fmaf(wt, x.y, o.y);
-      o.z = fmaf(wt, x.z, o.z);
-      o.w = fmaf(wt, x.w, o.w);
-    }
+  for (int s = grp; s < a.splits; s += GROUPS) {
+    const float2 ml = __ldcg(&a.part_ml[s * stride + at]);
+    const float4 x = __ldcg(reinterpret_cast<const float4*>(a.part_o + (s * stride + at) * HD + col));
+    const float wt = ex2_approx(ml.x - base);
+    l = fmaf(wt, ml.y, l);
+    o.x = fmaf(wt, x.x, o.x);
+    o.y = fmaf(wt, x.y, o.y);
+    o.z = fmaf(wt, x.z, o.z);
+    o.w = fmaf(wt, x.w, o.w);
   }
   s_acc[grp][threadIdx.x % QV] = o;
   if (threadIdx.x % QV == 0) s_l[grp] = l;

@@ -406,7 +406,7 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
 
 /* ckv_attention over the 8-bit cache: q/out [m][Hq][D] bf16, key j visible to row i iff
  * j <= positions[i]; a row whose position is negative sees no key and gives zeros, one at or
- * past n_ctx sees every key (recorded).  Codes and scales past every row's position may hold
+ * past n_ctx sees every key (recorded).  NaN in a row of q makes that row of out NaN.  Codes and scales past every row's position may hold
  * anything; codes some row sees must be finite and scales 0 or in [2^-110, 2^120] (ckv_kv8_write
  * leaves no other), for a weight of 0 does not silence a NaN in a row that shares a tile.  Weights
  * meet the codes in fp16, relative to the largest value scale of the keys worked on together:
@@ -440,7 +440,7 @@ CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const f
 /* Attention of row i over the keys j <= positions[i] of the blocks listed for it (ascending, -1
  * past the end; an entry out of range or not above the one before it is skipped and recorded as
  * CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache (cache_bits 16 or 8).
- * Rows that see no key give zeros.  `scale` as in ckv_attention_kv8; m * n_q_heads at most 2^31 - 2^20. */
+ * Rows that see no key give zeros, a row of q with a NaN gives NaN.  `scale` as in ckv_attention_kv8; m * n_q_heads at most 2^31 - 2^20. */
 CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top,
                                                     int cache_bits);
 CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int cache_bits);
