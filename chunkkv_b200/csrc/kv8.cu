@@ -7,7 +7,8 @@
 // and code * scale is the value held.  Each of the three is one correctly rounded fp32
 // operation, so the codes are the same whatever computes them.  A block whose a is below
 // 2^-100 (where qmax / a leaves fp32) holds zeros with scale 0.  Non-finite inputs are
-// stored saturated (NaN as 0), left out of a, and reported in the device error word.
+// stored saturated (NaN as 0), left out of a, and reported in the device error word by the
+// write that brings them.
 //
 // A block that is still being filled is requantised from its bf16 rows at every write:
 // the rows written so far are kept in the cache's `tail`, so the codes never depend on how
@@ -143,6 +144,25 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
       }
     }
   }
+  if (CT != kNone && bi == 0) {
+    // the rows of the block in progress stay in the tail, as they came: what stands for an infinity
+    // goes by the block's largest value, which later rows may raise.  The warp that read the
+    // tail writes it, so no other warp can see it half replaced.
+    const int keep = end % kRows, bl = end / kRows;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int r = p * RPP + r0;
+      if (r < keep) {
+        uint4 y = x[p];
+        if (bl != b) {
+          const int64_t t = int64_t(bl) * kRows + r - (a.by_position ? 0 : start);
+          y = __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
+        }
+        *reinterpret_cast<uint4*>(tail + r * HD + col) = y;
+      }
+    }
+    if (lane == 0) a.tail_end[side * a.H + h] = keep > 0 ? end : 0;
+  }
   uint32_t mag = 0;  // largest |x| as bf16 bits, two at a time
 #pragma unroll
   for (int p = 0; p < PASSES; ++p)
@@ -151,8 +171,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
   uint32_t amag = max(mag & 0xffffu, mag >> 16);
   amag = __reduce_max_sync(0xffffffffu, amag);
   if (amag >= 0x7f80u) {  // rare: a non-finite row
-    if (lane == 0) atomicOr(&g_err_word, CKV_DEV_ERR_NONFINITE);
     amag = 0;
+    bool fresh = false;  // reported by the write that brings it, not by those after it
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
       uint16_t* e = reinterpret_cast<uint16_t*>(&x[p]);
@@ -160,10 +180,12 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
       for (int i = 0; i < 8; ++i) {
         const uint32_t mg = e[i] & 0x7fffu;
         if (mg < 0x7f80u) amag = max(amag, mg);
-        else if (mg > 0x7f80u) e[i] = 0;
+        else fresh |= p * RPP + r0 >= old;
+        if (mg > 0x7f80u) e[i] = 0;
       }
     }
     amag = __reduce_max_sync(0xffffffffu, amag);
+    if (__any_sync(0xffffffffu, fresh) && lane == 0) atomicOr(&g_err_word, CKV_DEV_ERR_NONFINITE);
     // an infinity becomes the block's largest value (the largest code)
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
@@ -225,24 +247,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
       c.y = code4_int8(lo_bf(w[2]), hi_bf(w[2]), lo_bf(w[3]), hi_bf(w[3]), inv);
       *reinterpret_cast<uint2*>(a.dig_codes + (blk * 2 + r0) * HD + col) = c;
     }
-  }
-  if (CT != kNone && bi == 0) {
-    // the rows of the block in progress stay in the tail.  The warp that read the tail
-    // writes it, so no other warp can see it half replaced.
-    const int keep = end % kRows, bl = end / kRows;
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int r = p * RPP + r0;
-      if (r < keep) {
-        uint4 y = x[p];
-        if (bl != b) {
-          const int64_t t = int64_t(bl) * kRows + r - (a.by_position ? 0 : start);
-          y = __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
-        }
-        *reinterpret_cast<uint4*>(tail + r * HD + col) = y;
-      }
-    }
-    if (lane == 0) a.tail_end[side * a.H + h] = keep > 0 ? end : 0;
   }
 }
 

@@ -375,8 +375,8 @@ CKV_API int ckv_attention(const uint16_t* q, const uint16_t* k_cache, const uint
  * All of them start as zeros.  For a block's written rows with a = max |x|:
  * scale = fp32(a / qmax), code = rn(fp32(x * fp32(qmax / a))), qmax 127 (int8) or 448 (e4m3);
  * a < 2^-100 stores zeros with scale 0.  Digest codes likewise with 127.  A NaN is stored as 0
- * and an infinity as the block's largest value, and CKV_DEV_ERR_NONFINITE is recorded.  The
- * codes past a block's last written row are 0.  The reference keeps its cache in the model's
+ * and an infinity as the block's largest value (the tail keeps the row as it came), and the
+ * write that brings it records CKV_DEV_ERR_NONFINITE.  The codes past a block's last written row are 0.  The reference keeps its cache in the model's
  * dtype (torch_engine.py:187-195); this form has no counterpart there. */
 typedef enum { CKV_KV8_INT8 = 0, CKV_KV8_E4M3 = 1 } ckv_kv8_type;
 

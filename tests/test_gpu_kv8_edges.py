@@ -54,3 +54,33 @@ def test_a_nan_query_row_gives_nan_over_blocks(Hq, H, D, n, m, top, kind):
     p = torch.arange(n - m, n, dtype=torch.int32, device=DEV)
     blocks = torch.arange(top, dtype=torch.int32, device=DEV).expand(m, H, top).contiguous()
     check_nan_rows(lambda x: attend(x, p, blocks), q, kd, vd, p, [(m - 1, 1), (0, Hq - 1)], blocks)
+
+
+# ------------------------------------------------------------------- non-finite rows
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cuts", [(4, 5, 9), (1, 2, 3, 4, 5, 6, 7, 8), (16, 20, 24), (17, 18)])
+def test_non_finite_rows_do_not_depend_on_the_pieces(cuts, dtype):
+    """An infinity is the block's largest value, also of rows that come after it; it is reported once."""
+    H, D, n = 2, 64, 26
+    k, v = (torch.randn((H, n, D), generator=torch.Generator(device=DEV).manual_seed(s), device=DEV) for s in (1, 2))
+    size = torch.arange(1, n + 1, device=DEV)[None, :, None].float()  # later rows are larger
+    k, v = (k * size).to(BF), (v * size).to(BF)
+    for t in (3, 18):
+        k[0, t, 5], k[1, t, 6], v[0, t, 7], v[1, t, 8] = float("inf"), float("nan"), float("-inf"), float("inf")
+    once = ops.KV8Cache(H, n, D, dtype, DEV, digest=True)
+    ops.kv8_write(once, k, v, 0)
+    assert _lib.device_error() & 0x10
+    for side, x in ((once.k, k), (once.v, v)):  # the largest code of its sign
+        want = torch.where(x.isposinf(), ref.QMAX[dtype], torch.where(x.isneginf(), -ref.QMAX[dtype], 0.0))
+        assert torch.equal(side.float()[:, :n][~x.isfinite()], want[~x.isfinite()])
+    c = ops.KV8Cache(H, n, D, dtype, DEV, digest=True)
+    at = 0
+    for end in (*cuts, n):
+        ops.kv8_write(c, k[:, at:end], v[:, at:end], at)
+        brought = not (k[:, at:end].isfinite().all() and v[:, at:end].isfinite().all())
+        assert bool(_lib.device_error() & 0x10) == brought
+        at = end
+    for a, b in ((c.k, once.k), (c.v, once.v)):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(c.k_scale, once.k_scale) and torch.equal(c.v_scale, once.v_scale)
+    assert torch.equal(c.digest.codes, once.digest.codes) and torch.equal(c.digest.scale, once.digest.scale)
