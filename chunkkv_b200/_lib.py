@@ -70,8 +70,8 @@ SIGNATURES: dict[str, list] = {
     "ckv_attention_workspace_size": [_i32, _i32, _i32, _i32, _i32],
     "ckv_attention_launches": [_i32, _i32, _i32, _i32, _i32, _i64],
     "ckv_attention": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _p],
-    "ckv_kv8_write": [_p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _p,
-                      _i32, _i32, _i32, _i32, _p],
+    "ckv_kv8_write": [_p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                      _p, _i32, _i32, _i32, _i32, _p],
     "ckv_kv8_read": [_p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _p],
     "ckv_block_digest": [_p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _i32, _i32, _i32, _p],
     "ckv_attention_kv8_workspace_size": [_i32, _i32, _i32, _i32, _i32],

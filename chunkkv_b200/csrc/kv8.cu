@@ -11,8 +11,12 @@
 // write that brings them.
 //
 // A block that is still being filled is requantised from its bf16 rows at every write:
-// the rows written so far are kept in the cache's `tail`, so the codes never depend on how
-// the rows were split over the writes, and no row is rounded twice.
+// the rows written so far are kept in the cache's `tail`, and the rows of the block before it in
+// `prev`.  So the codes do not depend on how the rows were split over appending writes, nor
+// on rows that were written and taken back, as far as the start of the block before the
+// one in progress (16 tokens at least).  A write that goes back further (or once more into an
+// earlier block, before the next one is full) finds its block's earlier rows only as codes,
+// and those are rounded a second time.
 #include "ckv_common.cuh"
 
 CKV_DEFINE_ERR_WORD(kv8)
@@ -35,6 +39,8 @@ struct WriteArgs {
   float* scale[2];    // [H][n_blocks]
   uint16_t* tail;     // [2][H][16][D]
   int32_t* tail_end;  // [2][H]: one past the last token whose row the tail holds
+  uint16_t* prev;     // [2][H][16][D]: the whole block before the tail's (may be null)
+  int32_t* prev_end;  // [2][H]: one past its last token (0: none)
   int8_t* dig_codes;  // [H][n_blocks][2][D]
   float* dig_scale;   // [H][n_blocks]
   int H, n_ctx, n_blocks, grid_blocks, sides;
@@ -115,14 +121,14 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
   const int r0 = lane / LPR, col = (lane % LPR) * 8;
   const uint16_t* src = a.src[side] + h * a.head_stride[side];
   const int64_t blk = int64_t(h) * a.n_blocks + b;
-  uint16_t* tail = nullptr;
-  int n_tail = 0;  // rows of this block that the tail holds
-  if (CT != kNone) {
-    tail = a.tail + (int64_t(side) * a.H + h) * kRows * HD;
-    if (old > 0) {
-      const int te = a.tail_end[side * a.H + h];
-      n_tail = te > 0 && te / kRows == b ? te % kRows : 0;
-    }
+  const uint16_t* held = nullptr;  // this block's rows, where the tail or the block before it is this one
+  int n_held = 0, prev_end = 0;
+  if (CT != kNone && bi == 0) {
+    const int64_t at = int64_t(side) * a.H + h;
+    const int te = a.tail_end[at];
+    if (a.prev != nullptr) prev_end = a.prev_end[at];
+    if (te > 0 && te / kRows == b) held = a.tail + at * kRows * HD, n_held = te % kRows;
+    else if (prev_end == (b + 1) * kRows) held = a.prev + at * kRows * HD, n_held = kRows;
   }
   uint4 x[PASSES];
 #pragma unroll
@@ -133,8 +139,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
       if (r >= old || CT == kNone) {
         const int64_t t = int64_t(b) * kRows + r - (a.by_position ? 0 : start);
         x[p] = __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
-      } else if (r < n_tail) {
-        x[p] = *reinterpret_cast<const uint4*>(tail + r * HD + col);
+      } else if (r < n_held) {
+        x[p] = *reinterpret_cast<const uint4*>(held + r * HD + col);
       } else if (CT != kNone) {
         // a write that goes back into an earlier block: its rows from the codes
         const uint2 c = *reinterpret_cast<const uint2*>(a.codes[side] + (blk * kRows + r) * HD + col);
@@ -144,25 +150,46 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
       }
     }
   }
-  if (CT != kNone && bi == 0) {
-    // the rows of the block in progress stay in the tail, as they came: what stands for an infinity
-    // goes by the block's largest value, which later rows may raise.  The warp that read the
-    // tail writes it, so no other warp can see it half replaced.
+  // (called last, or before the repairs below: in front of the sums it would hold everything up,
+  // 5248 tokens 4.0 us against 4.9)
+  auto keep_rows = [&] {
+    // The rows of the block in progress stay in the tail and those of the block before it in prev,
+    // as they came: what stands for an infinity goes by the block's largest value, which later rows
+    // may raise.  A write that begins a block reads neither, so each of the two blocks' warps
+    // keeps its own rows; else the warp that reads them writes them, and no other warp can see
+    // them half replaced.
     const int keep = end % kRows, bl = end / kRows;
+    const int64_t at = int64_t(side) * a.H + h;
+    uint16_t *tail = a.tail + at * kRows * HD, *prev = a.prev + at * kRows * HD;
+    if (start % kRows == 0 || bl == b0) {
+      if (b == bl || (b == bl - 1 && a.prev != nullptr)) {
+        uint16_t* slot = b == bl ? tail : prev;
 #pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-      const int r = p * RPP + r0;
-      if (r < keep) {
-        uint4 y = x[p];
-        if (bl != b) {
-          const int64_t t = int64_t(bl) * kRows + r - (a.by_position ? 0 : start);
-          y = __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
+        for (int p = 0; p < PASSES; ++p) {
+          const int r = p * RPP + r0;
+          if (r < rows) *reinterpret_cast<uint4*>(slot + r * HD + col) = x[p];
         }
-        *reinterpret_cast<uint4*>(tail + r * HD + col) = y;
+      }
+    } else if (bi == 0) {
+      auto row_of = [&](int block, int p) {  // row p * RPP + r0 of this block or of one that is all new
+        if (block == b) return x[p];
+        const int64_t t = int64_t(block) * kRows + p * RPP + r0 - (a.by_position ? 0 : start);
+        return __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
+      };
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int r = p * RPP + r0;
+        if (r < keep) *reinterpret_cast<uint4*>(tail + r * HD + col) = row_of(bl, p);
+        if (a.prev != nullptr) *reinterpret_cast<uint4*>(prev + r * HD + col) = row_of(bl - 1, p);
       }
     }
-    if (lane == 0) a.tail_end[side * a.H + h] = keep > 0 ? end : 0;
-  }
+    if (bi == 0 && lane == 0) {
+      a.tail_end[at] = keep > 0 ? end : 0;
+      if (bl > b) prev_end = bl * kRows;             // block bl - 1 is whole now
+      else if (prev_end != b * kRows) prev_end = 0;  // b was taken up again: the block before it is not known
+      if (a.prev != nullptr) a.prev_end[at] = prev_end;
+    }
+  };
   uint32_t mag = 0;  // largest |x| as bf16 bits, two at a time
 #pragma unroll
   for (int p = 0; p < PASSES; ++p)
@@ -170,7 +197,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
                                  __vmaxu2(x[p].z & 0x7fff7fffu, x[p].w & 0x7fff7fffu)));
   uint32_t amag = max(mag & 0xffffu, mag >> 16);
   amag = __reduce_max_sync(0xffffffffu, amag);
-  if (amag >= 0x7f80u) {  // rare: a non-finite row
+  const bool odd = amag >= 0x7f80u;
+  if (odd) {  // rare: a non-finite row
+    if constexpr (CT != kNone) keep_rows();
     amag = 0;
     bool fresh = false;  // reported by the write that brings it, not by those after it
 #pragma unroll
@@ -248,6 +277,8 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
       *reinterpret_cast<uint2*>(a.dig_codes + (blk * 2 + r0) * HD + col) = c;
     }
   }
+  if constexpr (CT != kNone)
+    if (!odd) keep_rows();
 }
 
 // Values of tokens [start, start + m) as bf16 rows [H][m][D]: a thread per 16 codes, one 16-byte
@@ -314,10 +345,13 @@ using namespace ckv;
 extern "C" int ckv_kv8_write(const uint16_t* k, const uint16_t* v, int64_t k_head_stride, int64_t k_row_stride,
                              int64_t v_head_stride, int64_t v_row_stride, int64_t src_rows, int by_position, int m,
                              int start, const int32_t* start_dev, uint8_t* k8, uint8_t* v8, float* k_scale,
-                             float* v_scale, uint16_t* tail, int32_t* tail_end, int8_t* dig_codes, float* dig_scale,
-                             int n_kv_heads, int head_dim, int n_ctx, int type, ckv_stream_t stream) {
+                             float* v_scale, uint16_t* tail, int32_t* tail_end, uint16_t* prev, int32_t* prev_end,
+                             int8_t* dig_codes, float* dig_scale, int n_kv_heads, int head_dim, int n_ctx, int type,
+                             ckv_stream_t stream) {
   CKV_REQUIRE(k8 && v8 && k_scale && v_scale && tail && tail_end, "ckv_kv8_write: null pointer");
-  CKV_REQUIRE(aligned16(k8) && aligned16(v8) && aligned16(tail), "ckv_kv8_write: the cache must be 16-byte aligned");
+  CKV_REQUIRE(aligned16(k8) && aligned16(v8) && aligned16(tail) && aligned16(prev),
+              "ckv_kv8_write: the cache must be 16-byte aligned");
+  CKV_REQUIRE((prev == nullptr) == (prev_end == nullptr), "ckv_kv8_write: prev pointers");
   CKV_REQUIRE((dig_codes == nullptr) == (dig_scale == nullptr) && aligned16(dig_codes), "ckv_kv8_write: digest pointers");
   CKV_REQUIRE(type == CKV_KV8_INT8 || type == CKV_KV8_E4M3, "ckv_kv8_write: type %d", type);
   if (head_dim != 64 && head_dim != 128) {
@@ -331,7 +365,7 @@ extern "C" int ckv_kv8_write(const uint16_t* k, const uint16_t* v, int64_t k_hea
   const int n_blocks = ceil_div(n_ctx, kRows);
   const int off = start_dev != nullptr ? kRows - 1 : start % kRows;
   WriteArgs a{{k, v}, {k_head_stride, v_head_stride}, {k_row_stride, v_row_stride}, by_position, m, start, start_dev,
-              src_rows, {k8, v8}, {k_scale, v_scale}, tail, tail_end, dig_codes, dig_scale, n_kv_heads, n_ctx, n_blocks,
+              src_rows, {k8, v8}, {k_scale, v_scale}, tail, tail_end, prev, prev_end, dig_codes, dig_scale, n_kv_heads, n_ctx, n_blocks,
               ceil_div(int64_t(off) + m, kRows), 2};
   CKV_REQUIRE(int64_t(a.grid_blocks) * 2 * n_kv_heads < (int64_t(1) << 31), "ckv_kv8_write: too many blocks");
   const cudaStream_t s = as_stream(stream);
@@ -354,7 +388,7 @@ extern "C" int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t 
   const int n_blocks = ceil_div(n_ctx, kRows);
   const int off = start_dev != nullptr ? kRows - 1 : start % kRows;
   WriteArgs a{{k, nullptr}, {head_stride, 0}, {row_stride, 0}, 1, m, start, start_dev, src_rows, {nullptr, nullptr},
-              {nullptr, nullptr}, nullptr, nullptr, dig_codes, dig_scale, n_kv_heads, n_ctx, n_blocks,
+              {nullptr, nullptr}, nullptr, nullptr, nullptr, nullptr, dig_codes, dig_scale, n_kv_heads, n_ctx, n_blocks,
               ceil_div(int64_t(off) + m, kRows), 1};
   CKV_REQUIRE(int64_t(a.grid_blocks) * n_kv_heads < (int64_t(1) << 31), "ckv_block_digest: too many blocks");
   const cudaStream_t s = as_stream(stream);

@@ -769,11 +769,12 @@ class BlockDigest:
 class KV8Cache:
     """One layer's K/V cache in 8 bits: codes `k`, `v` [H, blocks * 16, D] (int8 or float8_e4m3fn),
     fp32 scales `k_scale`, `v_scale` [H, blocks] per KV head and block of 16 tokens, the bf16 rows
-    of the block in progress (`tail` [2, H, 16, D], `tail_end` [2, H]) and, with `digest=True`, the
-    block digest of K for the sparse attention.  Tokens never written read as zeros."""
+    of the block in progress (`tail` [2, H, 16, D], `tail_end` [2, H]) and of the one before it
+    (`prev`, `prev_end`) and, with `digest=True`, the block digest of K for the sparse attention.
+    Tokens never written read as zeros."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "tail", "tail_end", "digest", "n_ctx", "n_kv_heads", "head_dim",
-                 "dtype")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "tail", "tail_end", "prev", "prev_end", "digest", "n_ctx", "n_kv_heads",
+                 "head_dim", "dtype")
 
     def __init__(self, n_kv_heads: int, n_ctx: int, head_dim: int, dtype: torch.dtype = torch.int8, device="cuda",
                  digest: bool = False):
@@ -792,7 +793,8 @@ class KV8Cache:
     def wrap(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, n_ctx: int,
              tail: torch.Tensor | None = None, tail_start: int = 0, digest: BlockDigest | None = None) -> "KV8Cache":
         """A cache over buffers that the caller owns.  `tail`, where given, holds the bf16 rows
-        of the block in progress when the cache holds `tail_start` tokens."""
+        of the block in progress when the cache holds `tail_start` tokens; without it a write into
+        that block takes the earlier rows from their codes."""
         c = cls.__new__(cls)
         c._set(k, v, k_scale, v_scale, n_ctx, tail, tail_start, digest)
         return c
@@ -824,6 +826,7 @@ class KV8Cache:
         self.k, self.v, self.k_scale, self.v_scale, self.tail, self.digest = k, v, k_scale, v_scale, tail, digest
         end = int(tail_start) if tail_start % PAGE_TOKENS else 0
         self.tail_end = torch.full((2, H), end, dtype=torch.int32, device=k.device)
+        self.prev, self.prev_end = torch.zeros_like(tail), torch.zeros_like(self.tail_end)
         self.n_ctx, self.n_kv_heads, self.head_dim, self.dtype = int(n_ctx), H, D, k.dtype
 
     @property
@@ -865,7 +868,10 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start, m: int |
     tensor (then `m` rows are read from wherever it points at launch: a captured call serves
     every later position).  `m` defaults to all rows (1 for a device `start`).  The written tokens
     are the block's last: rows behind them in the same block become zeros (they share its scale),
-    later blocks stay as they were."""
+    later blocks stay as they were.  A write may go back (rejected drafts): into the block in
+    progress or the one before it as if the rows taken back had never been written; further
+    back, or once more into an earlier block before the next one is full, its block's earlier
+    rows are taken from their codes (rounded a second time)."""
     H, D = cache.n_kv_heads, cache.head_dim
     rows, k_head, k_row = _rows_view("k", k, H, D)
     v_rows, v_head, v_row = _rows_view("v", v, H, D)
@@ -879,7 +885,8 @@ def kv8_write(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, start, m: int |
     dig = cache.digest
     _run("ckv_kv8_write", k.data_ptr(), v.data_ptr(), k_head, k_row, v_head, v_row, rows,
          int(by_position), m, s, s_dev, cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-         cache.v_scale.data_ptr(), cache.tail.data_ptr(), cache.tail_end.data_ptr(),
+         cache.v_scale.data_ptr(), cache.tail.data_ptr(), cache.tail_end.data_ptr(), cache.prev.data_ptr(),
+         cache.prev_end.data_ptr(),
          None if dig is None else dig.codes.data_ptr(), None if dig is None else dig.scale.data_ptr(), H, D,
          cache.n_ctx, _KV8_TYPES[cache.dtype], stream, nbytes=6.0 * H * m * D)
     return cache

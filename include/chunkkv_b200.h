@@ -370,6 +370,7 @@ CKV_API int ckv_attention(const uint16_t* q, const uint16_t* k_cache, const uint
  *   k_scale, v_scale [H][n_blocks]; a value is code * scale
  *   tail             [2 (K, V)][H][16][D] bf16: the rows of the block in progress
  *   tail_end         [2][H] int32: one past the last token whose row the tail holds (zero at first)
+ *   prev, prev_end   (both optional) as tail and tail_end, for the whole block before the tail's
  *   dig_codes        [H][n_blocks][2][D] int8, dig_scale [H][n_blocks] (both optional): the
  *                    block digest of K, its channel maxima and minima
  * All of them start as zeros.  For a block's written rows with a = max |x|:
@@ -383,15 +384,17 @@ typedef enum { CKV_KV8_INT8 = 0, CKV_KV8_E4M3 = 1 } ckv_kv8_type;
 /* Rows of m tokens into the cache as tokens [start, start + m).  k, v: bf16 rows of D
  * contiguous elements at the given element strides (multiples of 8); token t's row is row
  * t - start, or row t when by_position is set.  The block that holds `start` is requantised from
- * its rows so far: those in the tail, or, when the write goes back into an earlier block, the
- * values of its codes.  With start_dev the first token is read from the device (one int32; a
+ * its rows so far: those in the tail or, when the write goes back into the block before it, in
+ * prev, as if the rows that are taken back had never been written; further back (without prev,
+ * or once more into an earlier block before the next one is full), the values of its codes, which
+ * are rounded a second time.  With start_dev the first token is read from the device (one int32; a
  * captured launch then serves every later position; out of range is recorded and nothing is
  * written). */
 CKV_API int ckv_kv8_write(const uint16_t* k, const uint16_t* v, int64_t k_head_stride, int64_t k_row_stride,
                           int64_t v_head_stride, int64_t v_row_stride, int64_t src_rows, int by_position, int m,
                           int start, const int32_t* start_dev, uint8_t* k8, uint8_t* v8, float* k_scale,
-                          float* v_scale, uint16_t* tail, int32_t* tail_end, int8_t* dig_codes, float* dig_scale,
-                          int n_kv_heads, int head_dim, int n_ctx, int type, ckv_stream_t stream);
+                          float* v_scale, uint16_t* tail, int32_t* tail_end, uint16_t* prev, int32_t* prev_end,
+                          int8_t* dig_codes, float* dig_scale, int n_kv_heads, int head_dim, int n_ctx, int type, ckv_stream_t stream);
 
 /* Values of tokens [start, start + m) as bf16 rows, k_out / v_out [H][m][D]. */
 CKV_API int ckv_kv8_read(const uint8_t* k8, const uint8_t* v8, const float* k_scale, const float* v_scale,

@@ -84,3 +84,74 @@ def test_non_finite_rows_do_not_depend_on_the_pieces(cuts, dtype):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
     assert torch.equal(c.k_scale, once.k_scale) and torch.equal(c.v_scale, once.v_scale)
     assert torch.equal(c.digest.codes, once.digest.codes) and torch.equal(c.digest.scale, once.digest.scale)
+
+
+# -------------------------------------------------------------------- writes that go back
+def equal_caches(a, b, n):
+    """Codes, scales and digests of the blocks that hold the first n tokens."""
+    nb = -(-n // 16)
+    for x, y in ((a.k, b.k), (a.v, b.v)):
+        assert torch.equal(x.view(torch.uint8)[:, :nb * 16], y.view(torch.uint8)[:, :nb * 16])
+    for x, y in ((a.k_scale, b.k_scale), (a.v_scale, b.v_scale), (a.digest.scale, b.digest.scale),
+                 (a.digest.codes, b.digest.codes)):
+        assert torch.equal(x[:, :nb], y[:, :nb])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,D,base,drafts,keep", [(4, 128, 28, 8, 2), (2, 64, 30, 3, 0), (2, 64, 31, 1, 0), (2, 64, 27, 5, 3), (2, 128, 20, 12, 1),
+                                                  (1, 64, 40, 24, 9), (3, 64, 33, 30, 1), (2, 64, 40, 8, 0), (2, 64, 47, 16, 0)])
+@pytest.mark.parametrize("device_start", [False, True])
+def test_rejected_drafts_leave_nothing_behind(H, D, base, drafts, keep, dtype, device_start):
+    """Drafts are appended, all but `keep` of them are rejected and others take their place: the cache
+    is that of one write of the rows that stay, though a rejected row had set its block's scale."""
+    n = base + drafts + 40
+    k, v = (torch.randn((H, n, D), generator=torch.Generator(device=DEV).manual_seed(s), device=DEV).to(BF) for s in (3, 4))
+    bad_k, bad_v = k.clone(), v.clone()
+    bad_k[:, base + keep:], bad_v[:, base + keep:] = 1000 * k[:, base + keep:], 1000 * v[:, base + keep:]
+
+    def write(c, kk, vv, a, b):
+        start = torch.tensor([a], dtype=torch.int32, device=DEV) if device_start else a
+        ops.kv8_write(c, kk[:, a:b], vv[:, a:b], start, b - a)
+
+    c = ops.KV8Cache(H, n, D, dtype, DEV, digest=True)
+    write(c, k, v, 0, 19)
+    write(c, k, v, 19, base)
+    write(c, bad_k, bad_v, base, base + drafts)
+    at = base + keep
+    # as many rounds of drafts as fit, every one rejected but for one row
+    for _ in range(3):
+        write(c, k, v, at, at + 1)
+        at += 1
+        write(c, bad_k, bad_v, at, at + 5)
+    write(c, k, v, at, n)
+    once = ops.KV8Cache(H, n, D, dtype, DEV, digest=True)
+    ops.kv8_write(once, k, v, 0)
+    equal_caches(c, once, n)
+
+
+def test_a_second_step_back_takes_the_codes():
+    """Back into the block before, then into one before that: its rows are known as codes alone."""
+    H, D, n = 2, 64, 70
+    k, v = (torch.randn((H, n, D), generator=torch.Generator(device=DEV).manual_seed(s), device=DEV).to(BF) for s in (5, 6))
+    c = ops.KV8Cache(H, n, D, torch.int8, DEV, digest=True)
+    ops.kv8_write(c, k, v, 0, 66)
+    ops.kv8_write(c, k[:, 50:], v[:, 50:], 50, 3)
+    rk, rv = ops.kv8_read(c, 32, 8)
+    ops.kv8_write(c, k[:, 40:], v[:, 40:], 40, 4)
+    for codes, scale, old, new in ((c.k, c.k_scale, rk, k), (c.v, c.v_scale, rv, v)):
+        rc, rs = ref.quantize(torch.cat([old, new[:, 40:44]], 1), torch.int8)
+        assert torch.equal(codes[:, 32:48].double(), rc) and torch.equal(scale[:, 2:3].double(), rs)
+
+
+def test_a_cache_without_the_block_before():
+    """The entry point takes null for it: appending writes are as ever."""
+    H, D, n = 2, 64, 50
+    k, v = (torch.randn((H, n, D), generator=torch.Generator(device=DEV).manual_seed(s), device=DEV).to(BF) for s in (7, 8))
+    c, once = (ops.KV8Cache(H, n, D, torch.int8, DEV, digest=True) for _ in range(2))
+    ops.kv8_write(once, k, v, 0)
+    stream = torch.cuda.current_stream().cuda_stream
+    for a, b in ((0, 5), (5, 40), (40, n)):
+        _lib.call("ckv_kv8_write", k.data_ptr(), v.data_ptr(), n * D, D, n * D, D, n, 1, b - a, a, None, c.k.data_ptr(),
+                  c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.tail.data_ptr(), c.tail_end.data_ptr(), None, None,
+                  c.digest.codes.data_ptr(), c.digest.scale.data_ptr(), H, D, n, 0, stream)
+    equal_caches(c, once, n)
