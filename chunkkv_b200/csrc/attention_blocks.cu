@@ -391,8 +391,10 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   }
   if (threadIdx.x == 0) *abort = 0;
   __syncthreads();
-  // Behind the selection only the lists (and, as ever, the output) wait for the kernel before: it
-  // let this one start after its own wait, so what was written before it is there.
+  // Behind the selection only the lists (and the output) wait for the kernel before: every CTA of
+  // it lets this kernel start after its own wait, so q and the positions, written before the selection
+  // began, are in L2 by then.  They are read there (ld.cg): a line of them that L1 still held
+  // from an earlier kernel would be older.  (One row, 64 of 2056 blocks: 13.1 us, behind the wait 13.6.)
   if (!a.after_select) pdl_wait();
   // as an operand owner a lane has query rows 8n + g: q and their positions first
   uint32_t w[NT][HD / 8];  // the dims of this lane's pieces of K (16 / ES dims each)
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     for (int e = 0; e < HD / 8; e += 4) {
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
       if (ok)
-        x = __ldg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
+        x = __ldcg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
                   (B::ES == 2 ? e + c : 8 * (e / 8) + 2 * c + (e / 4) % 2));
       w[n][e] = x.x, w[n][e + 1] = x.y, w[n][e + 2] = x.z, w[n][e + 3] = x.w;
     }
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     const int pr = row0 + 8 * n + g;
     int p = -1;
     if (pr < row_end) {
-      p = a.positions[pr / G];
+      p = __ldcg(a.positions + pr / G);
       if (p >= a.n_ctx) {
         if (split == 0 && hk == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
         p = a.n_ctx - 1;
@@ -438,9 +440,9 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   auto block_of = [&](int i) -> int {
     if (i >= i1) return -1;
     if constexpr (!LISTED) return i;
-    const int b = __ldg(list + i);
+    const int b = list[i];  // not by the read-only path: the selection may write it while this kernel runs
     if (b == -1) return -1;
-    if (b < 0 || b >= a.n_blocks || (i > 0 && __ldg(list + i - 1) >= b)) {
+    if (b < 0 || b >= a.n_blocks || (i > 0 && list[i - 1] >= b)) {
       if (lane == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
       return -1;
     }

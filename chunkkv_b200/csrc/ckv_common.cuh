@@ -57,6 +57,10 @@ int set_smem_limit(const void* kernel, int bytes);  // raises the dynamic smem c
 // pdl_wait() before its first global-memory access (it returns once the previous kernel
 // has completed and its writes are visible), then pdl_launch_next() so that the kernel
 // after it may be scheduled in turn.  Launched without the attribute, both are no-ops.
+// One exception: the block attention behind its own selection reads q and the positions, which
+// the selection only reads, before its wait and past L1 (attention_blocks.cu).  It relies on
+// every CTA of the kernel before it calling pdl_launch_next() after its own pdl_wait(), as
+// all of this library's kernels do.
 template <typename... Params, typename... Args>
 cudaError_t launch_pdl(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                        Args&&... args) {

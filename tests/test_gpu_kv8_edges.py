@@ -155,3 +155,42 @@ def test_a_cache_without_the_block_before():
                   c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.tail.data_ptr(), c.tail_end.data_ptr(), None, None,
                   c.digest.codes.data_ptr(), c.digest.scale.data_ptr(), H, D, n, 0, stream)
     equal_caches(c, once, n)
+
+
+# ------------------------------------------------------------- calls behind other kernels
+@pytest.mark.parametrize("Hq,H,D,n,top", [(28, 4, 128, 3000, 20), (14, 2, 64, 70000, 40)])
+def test_sparse_call_takes_what_the_kernels_before_it_wrote(Hq, H, D, n, top):
+    """q by this library's RMSNorm (a dependent launch) and the position by a copy, directly before
+    the call, both in the same buffers at every step of one graph."""
+    c, _, _ = filled(H, n, D, torch.int8, seed=2, digest=True)
+    steps = 24
+    x = queries(steps, Hq, D, 3).view(steps, Hq * D)
+    w = torch.ones(Hq * D, dtype=BF, device=DEV)
+    at = torch.randint(200, n, (steps, 1), generator=torch.Generator().manual_seed(1), dtype=torch.int32).to(DEV)
+    q, p = torch.zeros((1, Hq * D), dtype=BF, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    outs = torch.zeros((steps, Hq, D), dtype=BF, device=DEV)
+    lists = torch.zeros((steps, 1, H, top), dtype=torch.int32, device=DEV)
+
+    def step(i):
+        p.copy_(at[i])
+        ops.rmsnorm(x[i:i + 1], w, 1e-6, out=q)
+        ops.attention_sparse_kv8(q.view(1, Hq, D), c, p, top, out=outs[i:i + 1], blocks=lists[i])
+
+    step(0)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for i in range(steps):
+            step(i)
+    for _ in range(5):
+        outs.zero_()
+        lists.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for i in range(steps):
+            qi = ops.rmsnorm(x[i:i + 1], w, 1e-6).view(1, Hq, D)
+            torch.cuda.synchronize()
+            want = ops.block_select(qi, c.digest, at[i], top)
+            torch.cuda.synchronize()
+            assert torch.equal(lists[i], want)
+            assert torch.equal(outs[i:i + 1], ops.attention_blocks_kv8(qi, c, at[i], want))
+            torch.cuda.synchronize()
