@@ -35,6 +35,10 @@
 CKV_DEFINE_ERR_WORD(attention_blocks)
 
 namespace ckv {
+// block_select.cu
+int block_select_check(const uint16_t* q, const int8_t* dig_codes, const float* dig_scale, const int32_t* positions,
+                       const int32_t* blocks, int m, int Hq, int Hk, int HD, int n_ctx, int top, int sink, int recent,
+                       const void* workspace, int64_t workspace_bytes);
 namespace {
 
 constexpr int kBlk = CKV_PAGE_TOKENS;
@@ -863,6 +867,85 @@ int check_space(const char* name, int m, int Hq, int Hk, int HD, int es, int n_c
   return CKV_OK;
 }
 
+// The arguments of a listed call; `type` -1: a bf16 cache.
+struct Call {
+  Args a;
+  int HD, type;
+  void* workspace;
+  int64_t ws_bytes;
+  Plan plan() const { return ckv::plan(a.m, a.Hq / a.Hk, a.Hk, HD, type < 0 ? 2 : 1, a.top, true); }
+};
+
+Call bf16_call(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* positions,
+                      const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top, float scale,
+                      void* workspace, int64_t ws_bytes, bool after_select) {
+  return {{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr, positions, blocks,
+           out, nullptr, nullptr, int64_t(n_ctx), m, Hq, Hk, n_ctx, ceil_div(n_ctx, kBlk), top, 1, 1, scale * 1.4426950408889634f,
+           after_select},
+          HD, -1, workspace, ws_bytes};
+}
+
+Call kv8_call(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale, const float* v_scale,
+                     const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top,
+                     float scale, int type, void* workspace, int64_t ws_bytes, bool after_select) {
+  const int nb = ceil_div(n_ctx, kBlk);
+  return {{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, top, 1, 1,
+           scale * 1.4426950408889634f, after_select},
+          HD, type, workspace, ws_bytes};
+}
+
+// Everything that a listed call refuses, without a launch.
+int check_call(const char* name, const Call& c, bool eight) {
+  const Args& a = c.a;
+  if (eight) {
+    CKV_REQUIRE(c.type == CKV_KV8_INT8 || c.type == CKV_KV8_E4M3, "%s: type %d", name, c.type);
+    CKV_REQUIRE(a.m == 0 || (a.ks && a.vs), "%s: null scales", name);
+  }
+  CKV_REQUIRE(a.top > 0, "%s: lists of %d blocks", name, a.top);
+  if (int rc = check(name, a, c.HD, 0)) return rc;
+  if (a.m == 0) return CKV_OK;
+  CKV_REQUIRE(a.blocks != nullptr, "%s: null block list", name);
+  const int64_t need = c.plan().bytes;
+  CKV_REQUIRE(c.ws_bytes >= need && (need == 0 || (c.workspace && aligned16(c.workspace))),
+              "%s: workspace of %lld bytes, needs %lld (16-byte aligned)", name, static_cast<long long>(c.ws_bytes),
+              static_cast<long long>(need));
+  return CKV_OK;
+}
+
+int launch_call(const Call& c, cudaStream_t s) {
+  const Args& a = c.a;
+  const Plan p = c.plan();
+  // a grid's second dimension is limited: tokens go in runs of at most 32768 tiles (rows are
+  // independent, and a call this long is never split along its lists)
+  const int run = std::max(1, 32768 / p.head_tiles);
+  for (int t = 0; t < a.m; t += run) {
+    Args b = a;
+    Plan pb = p;
+    b.m = std::min(run, a.m - t);
+    pb.tiles = b.m * p.head_tiles;
+    b.q += int64_t(t) * a.Hq * c.HD;
+    b.out += int64_t(t) * a.Hq * c.HD;
+    b.positions += t;
+    b.blocks += int64_t(t) * a.Hk * a.top;
+    int rc;
+    if (c.HD == 128)
+      rc = c.type < 0 ? launch_nt<128, kBf16, true>(b, pb, c.workspace, s)
+           : c.type == CKV_KV8_E4M3 ? launch_nt<128, kE4m3, true>(b, pb, c.workspace, s)
+                                    : launch_nt<128, kInt8, true>(b, pb, c.workspace, s);
+    else
+      rc = c.type < 0 ? launch_nt<64, kBf16, true>(b, pb, c.workspace, s)
+           : c.type == CKV_KV8_E4M3 ? launch_nt<64, kE4m3, true>(b, pb, c.workspace, s)
+                                    : launch_nt<64, kInt8, true>(b, pb, c.workspace, s);
+    if (rc) return rc;
+  }
+  return CKV_OK;
+}
+
+int attention_blocks(const char* name, const Call& c, bool eight, ckv_stream_t stream) {
+  if (int rc = check_call(name, c, eight)) return rc;
+  return c.a.m == 0 ? CKV_OK : launch_call(c, as_stream(stream));
+}
+
 }  // namespace
 
 // Few query rows over a whole 8-bit cache; used by ckv_attention_kv8 (attention_kv8.cu).
@@ -907,76 +990,24 @@ extern "C" int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_head
   return launches(plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, bits / 8, top, true));
 }
 
-static int attention_blocks(const char* name, Args a, int HD, int type, void* workspace, int64_t ws_bytes, cudaStream_t s) {
-  CKV_REQUIRE(a.top > 0, "%s: lists of %d blocks", name, a.top);
-  if (int rc = check(name, a, HD, 0)) return rc;
-  if (a.m == 0) return CKV_OK;
-  const Plan p = plan(a.m, a.Hq / a.Hk, a.Hk, HD, type < 0 ? 2 : 1, a.top, true);
-  CKV_REQUIRE(a.blocks != nullptr, "%s: null block list", name);
-  CKV_REQUIRE(ws_bytes >= p.bytes && (p.bytes == 0 || (workspace && aligned16(workspace))),
-              "%s: workspace of %lld bytes, needs %lld (16-byte aligned)", name, static_cast<long long>(ws_bytes),
-              static_cast<long long>(p.bytes));
-  // a grid's second dimension is limited: tokens go in runs of at most 32768 tiles (rows are
-  // independent, and a call this long is never split along its lists)
-  const int run = std::max(1, 32768 / p.head_tiles);
-  for (int t = 0; t < a.m; t += run) {
-    Args b = a;
-    Plan pb = p;
-    b.m = std::min(run, a.m - t);
-    pb.tiles = b.m * p.head_tiles;
-    b.q += int64_t(t) * a.Hq * HD;
-    b.out += int64_t(t) * a.Hq * HD;
-    b.positions += t;
-    b.blocks += int64_t(t) * a.Hk * a.top;
-    int rc;
-    if (HD == 128)
-      rc = type < 0 ? launch_nt<128, kBf16, true>(b, pb, workspace, s)
-           : type == CKV_KV8_E4M3 ? launch_nt<128, kE4m3, true>(b, pb, workspace, s)
-                                  : launch_nt<128, kInt8, true>(b, pb, workspace, s);
-    else
-      rc = type < 0 ? launch_nt<64, kBf16, true>(b, pb, workspace, s)
-           : type == CKV_KV8_E4M3 ? launch_nt<64, kE4m3, true>(b, pb, workspace, s)
-                                  : launch_nt<64, kInt8, true>(b, pb, workspace, s);
-    if (rc) return rc;
-  }
-  return CKV_OK;
-}
-
-static int attention_blocks_bf16(const char* name, const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
-                                 const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD,
-                                 int n_ctx, int top, float scale, void* workspace, int64_t ws_bytes, cudaStream_t s, bool after_select) {
-  const Args a{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr,
-               positions, blocks, out, nullptr, nullptr, int64_t(n_ctx), m, Hq, Hk, n_ctx, ceil_div(n_ctx, kBlk),
-               top, 1, 1, scale * 1.4426950408889634f, after_select};
-  return attention_blocks(name, a, HD, -1, workspace, ws_bytes, s);
-}
-
-static int attention_blocks_8bit(const char* name, const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
-                                 const float* v_scale, const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq,
-                                 int Hk, int HD, int n_ctx, int top, float scale, int type, void* workspace, int64_t ws_bytes,
-                                 cudaStream_t s, bool after_select) {
-  CKV_REQUIRE(type == CKV_KV8_INT8 || type == CKV_KV8_E4M3, "%s: type %d", name, type);
-  CKV_REQUIRE(m == 0 || (k_scale && v_scale), "%s: null scales", name);
-  const int nb = ceil_div(n_ctx, kBlk);
-  const Args a{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq,
-               Hk, n_ctx, nb, top, 1, 1, scale * 1.4426950408889634f, after_select};
-  return attention_blocks(name, a, HD, type, workspace, ws_bytes, s);
-}
-
 extern "C" int ckv_attention_blocks(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
                                     const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int n_q_heads,
                                     int n_kv_heads, int head_dim, int n_ctx, int top, float scale, void* workspace,
                                     int64_t workspace_bytes, ckv_stream_t stream) {
-  return attention_blocks_bf16("ckv_attention_blocks", q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim,
-                               n_ctx, top, scale, workspace, workspace_bytes, as_stream(stream), false);
+  return attention_blocks("ckv_attention_blocks",
+                          bf16_call(q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, scale,
+                                    workspace, workspace_bytes, false),
+                          false, stream);
 }
 
 extern "C" int ckv_attention_blocks_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
                                         const float* v_scale, const int32_t* positions, const int32_t* blocks, uint16_t* out,
                                         int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top, float scale,
                                         int type, void* workspace, int64_t workspace_bytes, ckv_stream_t stream) {
-  return attention_blocks_8bit("ckv_attention_blocks_kv8", q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads,
-                               head_dim, n_ctx, top, scale, type, workspace, workspace_bytes, as_stream(stream), false);
+  return attention_blocks("ckv_attention_blocks_kv8",
+                          kv8_call(q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top,
+                                   scale, type, workspace, workspace_bytes, false),
+                          true, stream);
 }
 
 extern "C" int64_t ckv_attention_sparse_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx, int top,
@@ -996,19 +1027,27 @@ extern "C" int ckv_attention_sparse(const uint16_t* q, const uint16_t* k_cache, 
     return rc;
   if (m == 0) return CKV_OK;
   const SparseSpace x = sparse_space(m, n_q_heads, n_kv_heads, head_dim, 2, n_ctx, top, build);
+  int8_t* built = nullptr;
+  float* built_scale = nullptr;
   if (build) {
-    int8_t* codes = reinterpret_cast<int8_t*>(static_cast<uint8_t*>(workspace) + x.step);
-    float* scales = reinterpret_cast<float*>(codes + int64_t(n_kv_heads) * ceil_div(n_ctx, kBlk) * 2 * head_dim);
-    if (int rc = ckv_block_digest(k_cache, int64_t(n_ctx) * head_dim, head_dim, n_ctx, n_ctx, 0, nullptr, codes, scales, n_kv_heads,
+    dig_codes = built = reinterpret_cast<int8_t*>(static_cast<uint8_t*>(workspace) + x.step);
+    dig_scale = built_scale = reinterpret_cast<float*>(built + int64_t(n_kv_heads) * ceil_div(n_ctx, kBlk) * 2 * head_dim);
+  }
+  // every step is checked before the first is launched
+  const Call c = bf16_call(q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, scale, workspace,
+                           x.step, true);
+  if (int rc = check_call("ckv_attention_sparse", c, false)) return rc;
+  if (int rc = block_select_check(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink, recent,
+                                  workspace, x.step))
+    return rc;
+  if (build)
+    if (int rc = ckv_block_digest(k_cache, int64_t(n_ctx) * head_dim, head_dim, n_ctx, n_ctx, 0, nullptr, built, built_scale, n_kv_heads,
                                   head_dim, n_ctx, stream))
       return rc;
-    dig_codes = codes, dig_scale = scales;
-  }
   if (int rc = ckv_block_select(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
                                 recent, workspace, x.step, stream))
     return rc;
-  return attention_blocks_bf16("ckv_attention_sparse", q, k_cache, v_cache, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim,
-                               n_ctx, top, scale, workspace, x.step, as_stream(stream), true);
+  return launch_call(c, as_stream(stream));
 }
 
 extern "C" int ckv_attention_sparse_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
@@ -1020,9 +1059,11 @@ extern "C" int ckv_attention_sparse_kv8(const uint16_t* q, const uint8_t* k8, co
                            workspace_bytes))
     return rc;
   if (m == 0) return CKV_OK;
+  const Call c = kv8_call(q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, scale, type,
+                          workspace, workspace_bytes, true);
+  if (int rc = check_call("ckv_attention_sparse_kv8", c, true)) return rc;
   if (int rc = ckv_block_select(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
                                 recent, workspace, workspace_bytes, stream))
     return rc;
-  return attention_blocks_8bit("ckv_attention_sparse_kv8", q, k8, v8, k_scale, v_scale, positions, blocks, out, m, n_q_heads, n_kv_heads,
-                               head_dim, n_ctx, top, scale, type, workspace, workspace_bytes, as_stream(stream), true);
+  return launch_call(c, as_stream(stream));
 }

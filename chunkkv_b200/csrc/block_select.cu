@@ -618,26 +618,46 @@ extern "C" int ckv_block_select_launches(int m, int n_q_heads, int n_kv_heads, i
   return 2 * ceil_div(m, chunk_tokens(m, n_kv_heads, ceil_div(n_ctx, kBlk)));
 }
 
-extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const float* dig_scale,
-                                const int32_t* positions, int32_t* blocks, int m, int n_q_heads, int n_kv_heads,
-                                int head_dim, int n_ctx, int top, int sink, int recent, void* workspace,
-                                int64_t workspace_bytes, ckv_stream_t stream) {
-  CKV_REQUIRE(m >= 0 && n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0 && n_ctx > 0,
-              "ckv_block_select: bad sizes");
+namespace ckv {
+// Everything that ckv_block_select refuses, without a launch (also asked by ckv_attention_sparse(_kv8)
+// before their first one).
+int block_select_check(const uint16_t* q, const int8_t* dig_codes, const float* dig_scale, const int32_t* positions,
+                       const int32_t* blocks, int m, int Hq, int Hk, int HD, int n_ctx, int top, int sink, int recent,
+                       const void* workspace, int64_t workspace_bytes) {
+  CKV_REQUIRE(m >= 0 && Hk > 0 && Hq > 0 && Hq % Hk == 0 && n_ctx > 0, "ckv_block_select: bad sizes");
   CKV_REQUIRE(sink >= 0 && recent >= 1 && top >= 1 && int64_t(sink) + recent <= top && top <= kMaxTop,
               "ckv_block_select: top %d (1 to %d) must hold the %d first and %d last blocks (at least one last)", top,
               kMaxTop, sink, recent);
-  if (!select_shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) {
-    set_error("ckv_block_select: head_dim %d (64 or 128), %d query heads per KV head (at most 16), context %d (at most %d)",
-              head_dim, n_q_heads / n_kv_heads, n_ctx, kMaxBlocks * kBlk);
+  if (!select_shape_ok(m, Hq, Hk, HD, n_ctx)) {
+    set_error("ckv_block_select: head_dim %d (64 or 128), %d query heads per KV head (at most 16), context %d (at most %d)", HD,
+              Hq / Hk, n_ctx, kMaxBlocks * kBlk);
     return CKV_ERR_UNSUPPORTED;
   }
   if (m == 0) return CKV_OK;
   const int nb = ceil_div(n_ctx, kBlk);
-  const bool few = use_cluster(m, n_kv_heads, nb);
+  const bool few = use_cluster(m, Hk, nb);
   CKV_REQUIRE(q && dig_codes && dig_scale && positions && blocks && (few || workspace), "ckv_block_select: null pointer");
   CKV_REQUIRE(aligned16(q) && aligned16(dig_codes) && (few || aligned16(workspace)),
               "ckv_block_select: tensors must be 16-byte aligned");
+  if (few) return CKV_OK;
+  const int64_t need = chunk_tokens(m, Hk, nb) * Hk * key_stride(nb) * 4;
+  CKV_REQUIRE(workspace_bytes >= need, "ckv_block_select: workspace of %lld bytes, needs %lld",
+              static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+  CKV_REQUIRE(m <= 1000000 && int64_t(m) * Hk < (int64_t(1) << 31) - 8, "ckv_block_select: too many rows");
+  return CKV_OK;
+}
+}  // namespace ckv
+
+extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const float* dig_scale,
+                                const int32_t* positions, int32_t* blocks, int m, int n_q_heads, int n_kv_heads,
+                                int head_dim, int n_ctx, int top, int sink, int recent, void* workspace,
+                                int64_t workspace_bytes, ckv_stream_t stream) {
+  if (int rc = block_select_check(q, dig_codes, dig_scale, positions, blocks, m, n_q_heads, n_kv_heads, head_dim, n_ctx, top, sink,
+                                  recent, workspace, workspace_bytes))
+    return rc;
+  if (m == 0) return CKV_OK;
+  const int nb = ceil_div(n_ctx, kBlk);
+  const bool few = use_cluster(m, n_kv_heads, nb);
   if (few) {
     const TopArgs a{nullptr, positions, blocks, m, 0, n_kv_heads, n_ctx, nb, top, sink, recent};
     const cudaStream_t s = as_stream(stream);
@@ -648,10 +668,6 @@ extern "C" int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, cons
                                       : launch_few<64, 1>(q, dig_codes, dig_scale, n_q_heads, a, s);
   }
   const int64_t step = chunk_tokens(m, n_kv_heads, nb);
-  const int64_t need = step * n_kv_heads * key_stride(nb) * 4;
-  CKV_REQUIRE(workspace_bytes >= need, "ckv_block_select: workspace of %lld bytes, needs %lld",
-              static_cast<long long>(workspace_bytes), static_cast<long long>(need));
-  CKV_REQUIRE(m <= 1000000 && int64_t(m) * n_kv_heads < (int64_t(1) << 31) - 8, "ckv_block_select: too many rows");
   const cudaStream_t s = as_stream(stream);
   uint32_t* keys = static_cast<uint32_t*>(workspace);
   for (int64_t t = 0; t < m; t += step) {

@@ -1,0 +1,62 @@
+"""Plans and refusals of the 8-bit cache's attention and of the attention over selected blocks, on the
+host: nothing here launches.  No GPU needed."""
+
+from __future__ import annotations
+
+import pytest
+
+from chunkkv_b200 import _lib
+
+P = 16  # a pointer that is never followed
+BIG = 1 << 40
+
+
+def sparse(m=1, Hq=4, H=2, D=64, n=800, top=4, sink=1, recent=1, scale=1.0, ws=P, nbytes=BIG, build=False, **ptr):
+    p = {k: ptr.get(k, P) for k in ("q", "k", "v", "codes", "dscale", "positions", "blocks", "out")}
+    if build:
+        p["codes"] = p["dscale"] = None
+    return ("ckv_attention_sparse", *p.values(), m, Hq, H, D, n, top, sink, recent, scale, ws, nbytes, None)
+
+
+def sparse8(m=1, Hq=4, H=2, D=64, n=800, top=4, sink=1, recent=1, scale=1.0, kind=0, ws=P, nbytes=BIG, **ptr):
+    names = ("q", "k", "v", "ks", "vs", "codes", "dscale", "positions", "blocks", "out")
+    return ("ckv_attention_sparse_kv8", *(ptr.get(k, P) for k in names), m, Hq, H, D, n, top, sink, recent, scale, kind, ws,
+            nbytes, None)
+
+
+BAD = [(dict(scale=float("nan")), ValueError, "scale"), (dict(scale=-1.0), ValueError, "scale"),
+       (dict(scale=float("inf")), ValueError, "scale"), (dict(out=None), ValueError, "null"), (dict(v=8), ValueError, "aligned"),
+       (dict(out=24), ValueError, "aligned"), (dict(q=8), ValueError, "aligned"), (dict(blocks=None), ValueError, "null"),
+       (dict(positions=None), ValueError, "null"), (dict(Hq=34), NotImplementedError, "17 query heads"),
+       (dict(n=600000), NotImplementedError, "at most 524288"), (dict(top=5000), ValueError, "top 5000"),
+       (dict(top=2, sink=2), ValueError, "top 2"), (dict(recent=0), ValueError, "at least one last"),
+       (dict(D=96), NotImplementedError, "head_dim 96"), (dict(m=100, nbytes=8), ValueError, "workspace of 8"),
+       (dict(m=100, ws=None), ValueError, "null|workspace")]
+
+
+@pytest.mark.parametrize("bad,exc,msg", BAD)
+def test_sparse_calls_check_every_step_before_the_first(bad, exc, msg):
+    """A call that is refused has neither built the digest nor rewritten the lists: on this host the
+    first launch would fail as a CUDA error instead."""
+    calls = [sparse(**bad), sparse8(**bad)]
+    calls.append(sparse(**bad, build=True))
+    for name, *args in calls:
+        with pytest.raises(exc, match=msg):
+            _lib.call(name, *args)
+
+
+@pytest.mark.parametrize("bad,msg", [(dict(kind=7), "type 7"), (dict(ks=None), "null scales"), (dict(vs=None), "null scales"),
+                                     (dict(codes=None), "null"), (dict(dscale=None), "null"), (dict(codes=8), "aligned")])
+def test_sparse_calls_over_8_bits_check_their_own(bad, msg):
+    name, *args = sparse8(**bad)
+    with pytest.raises(ValueError, match=msg):
+        _lib.call(name, *args)
+
+
+def test_sparse_call_refuses_half_a_digest():
+    name, *args = sparse(codes=None)
+    with pytest.raises(ValueError, match="digest pointers"):
+        _lib.call(name, *args)
+    name, *args = sparse(build=True, k=8)
+    with pytest.raises(ValueError, match="aligned"):
+        _lib.call(name, *args)
