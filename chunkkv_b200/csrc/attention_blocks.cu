@@ -440,13 +440,15 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   const int per = (n_items + a.splits - 1) / a.splits;
   const int i1 = min(n_items, (split + 1) * per);
   const int32_t* list = LISTED ? a.blocks + (int64_t(tok0) * a.Hk + hk) * a.top : nullptr;
-  // item i's block, or -1 when there is none (past the list's end, out of range, not ascending)
+  // item i's block, or -1 when there is none (past the list's end, out of range, not ascending).  Every
+  // entry is held against the one before it, so a list that lets a block through twice is recorded.
   auto block_of = [&](int i) -> int {
     if (i >= i1) return -1;
     if constexpr (!LISTED) return i;
     const int b = list[i];  // not by the read-only path: the selection may write it while this kernel runs
     if (b == -1) return -1;
-    if (b < 0 || b >= a.n_blocks || (i > 0 && list[i - 1] >= b)) {
+    const int before = i > 0 ? list[i - 1] : -2;  // -2: nothing before it
+    if (b < 0 || b >= a.n_blocks || before >= b || before == -1) {
       if (lane == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
       return -1;
     }

@@ -194,3 +194,20 @@ def test_sparse_call_takes_what_the_kernels_before_it_wrote(Hq, H, D, n, top):
             assert torch.equal(lists[i], want)
             assert torch.equal(outs[i:i + 1], ops.attention_blocks_kv8(qi, c, at[i], want))
             torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------------------ lists
+@pytest.mark.parametrize("kind", [BF, *TYPES])
+@pytest.mark.parametrize("bad", [[5, -1, 5, -1], [-1, 3, -1, -1], [2, 4, -1, 6], [-1, -1, -1, 0]])
+def test_entries_behind_the_end_of_a_list_are_reported(bad, kind):
+    Hq, H, D, n = 4, 2, 64, 400
+    attend, kd, vd, _, _ = caches(kind, H, n, D)
+    q = queries(1, Hq, D, 1)
+    p = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    lists = torch.tensor([[[1, 2, 3, -1], bad]], dtype=torch.int32, device=DEV)
+    out = attend(q, p, lists)
+    assert _lib.device_error() & 0x8
+    kept = [b if i == 0 or bad[i - 1] != -1 else -1 for i, b in enumerate(bad)]
+    check = torch.tensor([[[1, 2, 3, -1], kept]], dtype=torch.int32, device=DEV)
+    want, mass = ref.attend(q, kd, vd, p, check)
+    assert float(((out.double() - want).abs() - want.abs() * 2.0 ** -8 - mass * 2.0 ** -9).max()) <= 0
