@@ -57,7 +57,7 @@ struct Args {
   float* part_o;          // [splits][tiles][H][8 NT][D]
   float2* part_ml;        // [splits][tiles][H][8 NT]
   int64_t head_rows;      // cache rows per head
-  int m, Hq, Hk, n_ctx, n_blocks, top, splits, head_tiles;
+  int m, Hq, Hk, n_ctx, n_blocks, top, items, splits, head_tiles;  // items: entries that a list can hold, min(top, n_blocks)
   float scale_log2;
   bool after_select;  // launched behind a kernel of the selection, which started when q and positions were complete
 };
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   if (a.after_select) pdl_wait();
   pdl_launch_next();
   const int nb = (last + kBlk) / kBlk;  // visible blocks
-  const int n_items = LISTED ? a.top : nb;
+  const int n_items = LISTED ? a.items : nb;
   const int per = (n_items + a.splits - 1) / a.splits;
   const int i1 = min(n_items, (split + 1) * per);
   const int32_t* list = LISTED ? a.blocks + (int64_t(tok0) * a.Hk + hk) * a.top : nullptr;
@@ -454,6 +454,12 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     }
     return b < nb ? b : -1;  // wholly past the row's position: nothing visible
   };
+  if constexpr (LISTED) {
+    // an ascending list ends before its entry `items`, and no split takes those from there on
+    if (a.top > a.items && split == 0)
+      for (int i = a.items + threadIdx.x; i < a.top; i += W * 32)
+        if (list[i] != -1) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
+  }
   uint8_t* ring = smem + warp * L::RING;
   constexpr int NB = B::NB;
   int ids[L::STAGES][NB];                           // blocks in the ring, -1: none
@@ -810,6 +816,10 @@ int launch_nt(const Args& a, const Plan& p, void* workspace, cudaStream_t stream
   return p.nt == 1 ? launch<HD, CT, 1, LISTED>(a, p, workspace, stream) : launch<HD, CT, 2, LISTED>(a, p, workspace, stream);
 }
 
+// The entries of a list of `top` that can name a block of the context: work and partials are planned
+// for these (128 entries over 300 tokens would leave six of a cluster's eight CTAs without any).
+int list_items(int top, int n_ctx) { return std::min(top, ceil_div(n_ctx, kBlk)); }
+
 int launches(const Plan& p) { return p.splits > 1 && !p.join ? 2 : 1; }
 
 // query rows (token, head) of a call: tile and row numbers stay within 32 bits
@@ -849,7 +859,7 @@ struct SparseSpace {
 };
 SparseSpace sparse_space(int m, int Hq, int Hk, int HD, int es, int n_ctx, int top, bool build) {
   const int64_t sel = ckv_block_select_workspace_size(m, Hq, Hk, HD, n_ctx);
-  const int64_t att = plan(m, Hq / Hk, Hk, HD, es, top, true).bytes;
+  const int64_t att = plan(m, Hq / Hk, Hk, HD, es, list_items(top, n_ctx), true).bytes;
   const int64_t nb = ceil_div(n_ctx, kBlk);
   SparseSpace x;
   x.step = (std::max(sel, att) + 15) / 16 * 16;
@@ -875,15 +885,15 @@ struct Call {
   int HD, type;
   void* workspace;
   int64_t ws_bytes;
-  Plan plan() const { return ckv::plan(a.m, a.Hq / a.Hk, a.Hk, HD, type < 0 ? 2 : 1, a.top, true); }
+  Plan plan() const { return ckv::plan(a.m, a.Hq / a.Hk, a.Hk, HD, type < 0 ? 2 : 1, a.items, true); }
 };
 
 Call bf16_call(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* positions,
                       const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top, float scale,
                       void* workspace, int64_t ws_bytes, bool after_select) {
   return {{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr, positions, blocks,
-           out, nullptr, nullptr, int64_t(n_ctx), m, Hq, Hk, n_ctx, ceil_div(n_ctx, kBlk), top, 1, 1, scale * 1.4426950408889634f,
-           after_select},
+           out, nullptr, nullptr, int64_t(n_ctx), m, Hq, Hk, n_ctx, ceil_div(n_ctx, kBlk), top, list_items(top, n_ctx), 1, 1,
+           scale * 1.4426950408889634f, after_select},
           HD, -1, workspace, ws_bytes};
 }
 
@@ -891,8 +901,8 @@ Call kv8_call(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const flo
                      const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top,
                      float scale, int type, void* workspace, int64_t ws_bytes, bool after_select) {
   const int nb = ceil_div(n_ctx, kBlk);
-  return {{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, top, 1, 1,
-           scale * 1.4426950408889634f, after_select},
+  return {{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, top,
+           list_items(top, n_ctx), 1, 1, scale * 1.4426950408889634f, after_select},
           HD, type, workspace, ws_bytes};
 }
 
@@ -967,7 +977,7 @@ int kv8_stream_attention(const uint16_t* q, const uint8_t* k8, const uint8_t* v8
                          const int32_t* positions, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, float scale, int type,
                          void* workspace, cudaStream_t stream) {
   const int nb = ceil_div(n_ctx, kBlk);
-  Args a{q, k8, v8, ks, vs, positions, nullptr, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, 0, 1, 1,
+  Args a{q, k8, v8, ks, vs, positions, nullptr, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, 0, 0, 1, 1,
          scale * 1.4426950408889634f, false};
   const Plan p = plan(m, Hq / Hk, Hk, HD, 1, nb, false);
   if (int rc = check("ckv_attention_kv8", a, HD, p.tiles)) return rc;

@@ -1050,9 +1050,9 @@ def attention_blocks(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
     stream = _on_device(q, k_cache, v_cache, positions, blocks, out)
-    need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, top, 16)
+    need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, min(top, _n_blocks(n_ctx)), 16)
     ws, nbytes = _workspace_arg(None, need, q.device)
-    kernels = 1 if _TIMER is None else _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, top, 16)
+    kernels = 1 if _TIMER is None else _blocks_kernels(m, Hq, H, D, n_ctx, top, 16)
     _run("ckv_attention_blocks", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), positions.data_ptr(),
          blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, n_ctx, top, 1.0 / math.sqrt(D) if scale is None else float(scale),
          _ptr(ws), nbytes, stream, kernels=kernels)
@@ -1068,9 +1068,9 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     top = _blocks_arg(blocks, m, H)
     out = _rows_out(q, m, Hq * D, out)
     stream = _on_device(q, positions, blocks, out, cache.k)
-    need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, top, 8)
+    need = _size("ckv_attention_blocks_workspace_size", q.get_device(), m, Hq, H, D, min(top, _n_blocks(cache.n_ctx)), 8)
     ws, nbytes = _workspace_arg(None, need, q.device)
-    kernels = 1 if _TIMER is None else _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, top, 8)
+    kernels = 1 if _TIMER is None else _blocks_kernels(m, Hq, H, D, cache.n_ctx, top, 8)
     _run("ckv_attention_blocks_kv8", q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), positions.data_ptr(), blocks.data_ptr(), out.data_ptr(), m, Hq, H, D, cache.n_ctx,
          top, 1.0 / math.sqrt(D) if scale is None else float(scale), _KV8_TYPES[cache.dtype], _ptr(ws), nbytes,
@@ -1078,10 +1078,13 @@ def attention_blocks_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tens
     return out
 
 
+def _blocks_kernels(m: int, Hq: int, H: int, D: int, n_ctx: int, top: int, bits: int) -> int:
+    return _lib.load().ckv_attention_blocks_launches(m, Hq, H, D, min(top, _n_blocks(n_ctx)), bits)
+
+
 def _sparse_kernels(m: int, Hq: int, H: int, D: int, n_ctx: int, top: int, bits: int) -> int:
-    lib = _lib.load()
-    return (lib.ckv_block_select_launches(m, Hq, H, D, n_ctx)
-            + lib.ckv_attention_blocks_launches(m, Hq, H, D, top, bits))
+    return (_lib.load().ckv_block_select_launches(m, Hq, H, D, n_ctx)
+            + _blocks_kernels(m, Hq, H, D, n_ctx, top, bits))
 
 
 def attention_sparse(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, top: int,

@@ -443,7 +443,9 @@ CKV_API int ckv_block_select(const uint16_t* q, const int8_t* dig_codes, const f
 /* Attention of row i over the keys j <= positions[i] of the blocks listed for it (ascending, -1
  * past the end; an entry out of range, not above the one before it or behind a -1 is skipped and
  * recorded as CKV_DEV_ERR_POSITION_RANGE).  bf16 caches [H][n_ctx][D], or the 8-bit cache (cache_bits 16 or 8).
- * Rows that see no key give zeros, a row of q with a NaN gives NaN.  `scale` as in ckv_attention_kv8; m * n_q_heads at most 2^31 - 2^20. */
+ * Rows that see no key give zeros, a row of q with a NaN gives NaN.  `scale` as in ckv_attention_kv8; m * n_q_heads at most 2^31 - 2^20.
+ * The workspace and the launches go by the entries that can name a block: pass min(top, blocks of the
+ * context) for `top` there (more is safe, and only a larger workspace). */
 CKV_API int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int top,
                                                     int cache_bits);
 CKV_API int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int cache_bits);

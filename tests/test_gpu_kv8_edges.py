@@ -211,3 +211,30 @@ def test_entries_behind_the_end_of_a_list_are_reported(bad, kind):
     check = torch.tensor([[[1, 2, 3, -1], kept]], dtype=torch.int32, device=DEV)
     want, mass = ref.attend(q, kd, vd, p, check)
     assert float(((out.double() - want).abs() - want.abs() * 2.0 ** -8 - mass * 2.0 ** -9).max()) <= 0
+
+
+@pytest.mark.parametrize("kind", [BF, *TYPES])
+@pytest.mark.parametrize("Hq,H,D,n,m,top", [(32, 8, 128, 4096, 1, 4096), (28, 4, 128, 300, 1, 128), (14, 2, 64, 700, 30, 300),
+                                            (4, 2, 64, 9, 3, 4096)])
+def test_lists_longer_than_the_context(Hq, H, D, n, m, top, kind):
+    attend, kd, vd, sparse, _ = caches(kind, H, n, D, seed=1)
+    q = queries(m, Hq, D, 4)
+    p = torch.arange(n - m, n, dtype=torch.int32, device=DEV)
+    out, blocks = sparse(q, p, top)
+    nb = (p // 16 + 1).tolist()
+    assert all(row[h].tolist() == [*range(b), *[-1] * (top - b)] for row, b in zip(blocks, nb) for h in range(H))
+    check_attention(out, q, kd, vd, p)
+    assert torch.equal(attend(q, p, blocks), out)
+    # an entry behind as many as the context has blocks cannot be right
+    blocks[m - 1, 0, top - 1] = 0
+    assert torch.equal(attend(q, p, blocks), out) and _lib.device_error() & 0x8
+
+
+@pytest.mark.parametrize("Hq,H,D,n,m,top", [(8, 2, 64, 131072, 2, 4096), (28, 4, 128, 20000, 1, 1000), (7, 1, 128, 100000, 40, 2049)])
+def test_long_lists(Hq, H, D, n, m, top):
+    _, kd, vd, sparse, d = caches(torch.int8, H, n, D, seed=3)
+    q = queries(m, Hq, D, 5)
+    p = torch.linspace(n - 1, n // 2, m, device=DEV).to(torch.int32)
+    out, blocks = sparse(q, p, top)
+    assert torch.equal(blocks.cpu().long(), ref.select(q, d.codes, d.scale, p, top))
+    check_attention(out[:4], q[:4], kd, vd, p[:4], blocks[:4])

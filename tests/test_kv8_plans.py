@@ -60,3 +60,19 @@ def test_sparse_call_refuses_half_a_digest():
     name, *args = sparse(build=True, k=8)
     with pytest.raises(ValueError, match="aligned"):
         _lib.call(name, *args)
+
+
+def test_lists_longer_than_the_context_are_planned_by_its_blocks():
+    """`top` may exceed the blocks that exist; no list can, so work and partials go by the latter."""
+    lib = _lib.load()
+    # 4096 entries over 4096 tokens: 256 blocks, which eight CTAs of a cluster share without partials
+    for top in (256, 257, 1000, 4096):
+        assert lib.ckv_attention_sparse_workspace_size(1, 32, 8, 128, 4096, top, 8, 0) == \
+            lib.ckv_attention_sparse_workspace_size(1, 32, 8, 128, 4096, 256, 8, 0)
+    for m, Hq, H, D, n in ((1, 28, 4, 128, 300), (9, 14, 2, 64, 40000), (3, 40, 8, 128, 700), (2, 7, 1, 128, 100000)):
+        nb = -(-n // 16)
+        for top in (1, 4, 5, 64, nb, 4096):
+            for bits in (8, 16):
+                size = lib.ckv_attention_blocks_workspace_size
+                # what the call asks for is never more than the size for the whole list
+                assert size(m, Hq, H, D, min(top, nb), bits) <= size(m, Hq, H, D, top, bits)
