@@ -820,6 +820,10 @@ int launch_nt(const Args& a, const Plan& p, void* workspace, cudaStream_t stream
 // for these (128 entries over 300 tokens would leave six of a cluster's eight CTAs without any).
 int list_items(int top, int n_ctx) { return std::min(top, ceil_div(n_ctx, kBlk)); }
 
+// Tokens of a listed call per launch: a grid's second dimension is limited, so tokens go in runs of at
+// most 32768 tiles (rows are independent, and a call this long is never split along its lists).
+int run_tokens(const Plan& p) { return std::max(1, 32768 / p.head_tiles); }
+
 int launches(const Plan& p) { return p.splits > 1 && !p.join ? 2 : 1; }
 
 // query rows (token, head) of a call: tile and row numbers stay within 32 bits
@@ -927,9 +931,7 @@ int check_call(const char* name, const Call& c, bool eight) {
 int launch_call(const Call& c, cudaStream_t s) {
   const Args& a = c.a;
   const Plan p = c.plan();
-  // a grid's second dimension is limited: tokens go in runs of at most 32768 tiles (rows are
-  // independent, and a call this long is never split along its lists)
-  const int run = std::max(1, 32768 / p.head_tiles);
+  const int run = run_tokens(p);
   for (int t = 0; t < a.m; t += run) {
     Args b = a;
     Plan pb = p;
@@ -999,7 +1001,8 @@ extern "C" int64_t ckv_attention_blocks_workspace_size(int m, int n_q_heads, int
 
 extern "C" int ckv_attention_blocks_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int top, int bits) {
   if (m <= 0 || top <= 0 || !shape_ok(m, n_q_heads, n_kv_heads, head_dim, 1)) return 0;
-  return launches(plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, bits / 8, top, true));
+  const Plan p = plan(m, n_q_heads / n_kv_heads, n_kv_heads, head_dim, bits / 8, top, true);
+  return launches(p) * ceil_div(m, run_tokens(p));
 }
 
 extern "C" int ckv_attention_blocks(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,

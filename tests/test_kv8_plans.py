@@ -76,3 +76,22 @@ def test_lists_longer_than_the_context_are_planned_by_its_blocks():
                 size = lib.ckv_attention_blocks_workspace_size
                 # what the call asks for is never more than the size for the whole list
                 assert size(m, Hq, H, D, min(top, nb), bits) <= size(m, Hq, H, D, top, bits)
+
+
+def test_launches_count_every_run():
+    """Calls of more rows than one grid or one workspace holds go in several runs."""
+    lib = _lib.load()
+    blocks = lib.ckv_attention_blocks_launches
+    for bits in (8, 16):
+        assert blocks(32768, 2, 2, 64, 3, bits) == 1 and blocks(32769, 2, 2, 64, 3, bits) == 2
+        assert blocks(100_000, 2, 2, 64, 3, bits) == 4
+        assert blocks(16_384, 20, 1, 64, 3, bits) == 1 and blocks(17_000, 20, 1, 64, 3, bits) == 2  # two tiles a token
+    for m, Hq, H, D, n in ((1, 28, 4, 128, 5248), (17, 28, 4, 128, 5248), (300, 28, 4, 128, 131072), (5000, 28, 4, 128, 131072),
+                           (1300, 8, 8, 64, 131072)):
+        nb = -(-n // 16)
+        size = lib.ckv_block_select_workspace_size(m, Hq, H, D, n)
+        few = m * H <= 32 and nb <= 4096
+        per_token = H * ((nb + 3) // 4 * 4) * 4  # 4-byte keys, rows padded to 16 bytes
+        runs = 1 if few else -(-m // (size // per_token))
+        assert lib.ckv_block_select_launches(m, Hq, H, D, n) == (1 if few else 2 * runs)
+    assert lib.ckv_block_select_launches(5000, 28, 4, 128, 131072) == 6
