@@ -76,6 +76,7 @@ SIGNATURES: dict[str, list] = {
     "ckv_block_digest": [_p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _i32, _i32, _i32, _p],
     "ckv_attention_kv8_workspace_size": [_i32, _i32, _i32, _i32, _i32],
     "ckv_attention_kv8_launches": [_i32, _i32, _i32, _i32, _i32],
+    "ckv_attention_kv8_splits": [_i32, _i32, _i32, _i32, _i32],
     "ckv_attention_kv8": [_p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p, _i64, _p],
     "ckv_block_select_workspace_size": [_i32, _i32, _i32, _i32, _i32],
     "ckv_block_select_launches": [_i32, _i32, _i32, _i32, _i32],

@@ -994,6 +994,11 @@ extern "C" int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, 
   return kv8_stream_launches(m, n_q_heads, n_kv_heads, head_dim, n_ctx);
 }
 
+extern "C" int ckv_attention_kv8_splits(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx) {
+  if (!shape_ok(m, n_q_heads, n_kv_heads, head_dim, n_ctx) || !use_tiles(m, n_q_heads, n_kv_heads, head_dim, n_ctx)) return 0;
+  return tile_plan(m, n_q_heads, n_kv_heads, head_dim, n_ctx).max_splits;
+}
+
 extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
                                  const float* v_scale, const int32_t* positions, uint16_t* out, int m, int n_q_heads,
                                  int n_kv_heads, int head_dim, int n_ctx, float scale, int type, void* workspace,

@@ -420,6 +420,9 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
 CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 /* Kernels one ckv_attention_kv8 call launches at this shape (0 for a shape it refuses). */
 CKV_API int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
+/* How one call works at this shape: 0, it streams the cache past a few rows at a time (or refuses the
+ * shape); n >= 1, in 128-row tiles on tcgen05, the keys of the longest rows in n splits. */
+CKV_API int ckv_attention_kv8_splits(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 CKV_API int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale,
                               const float* v_scale, const int32_t* positions, uint16_t* out, int m, int n_q_heads,
                               int n_kv_heads, int head_dim, int n_ctx, float scale, int type, void* workspace,
