@@ -838,7 +838,7 @@ int check(const char* name, const Args& a, int HD, int64_t tiles) {
   CKV_REQUIRE(a.m >= 0 && a.Hk > 0 && a.Hk <= 65535 && a.Hq > 0 && a.Hq % a.Hk == 0, "%s: %d query heads over %d KV heads", name,
               a.Hq, a.Hk);
   CKV_REQUIRE(a.n_ctx > 0 && a.n_ctx <= (1 << 30), "%s: context of %d", name, a.n_ctx);
-  CKV_REQUIRE(a.scale_log2 >= 0.f && a.scale_log2 <= 3.0e38f, "%s: scale %g (finite, not negative)", name,
+  CKV_REQUIRE(a.scale_log2 >= 0.f && a.scale_log2 <= 3.0e38f, "%s: scale %g (0 to 2e38)", name,
               double(a.scale_log2 / 1.4426950408889634f));
   CKV_REQUIRE(int64_t(a.m) * a.Hq <= kMaxRows, "%s: %d rows of %d heads in one call", name, a.m, a.Hq);
   if (HD != 64 && HD != 128) {

@@ -1012,7 +1012,7 @@ extern "C" int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uin
               n_q_heads / n_kv_heads, n_ctx, m);
     return CKV_ERR_UNSUPPORTED;
   }
-  CKV_REQUIRE(scale >= 0.f && scale <= 3.0e38f, "ckv_attention_kv8: scale %g (finite, not negative)", double(scale));
+  CKV_REQUIRE(scale >= 0.f && scale * 1.4426950408889634f <= 3.0e38f, "ckv_attention_kv8: scale %g (0 to 2e38)", double(scale));
   CKV_REQUIRE(q && k8 && v8 && k_scale && v_scale && positions && out, "ckv_attention_kv8: null pointer");
   CKV_REQUIRE(aligned16(q) && aligned16(k8) && aligned16(v8) && aligned16(out),
               "ckv_attention_kv8: tensors must be 16-byte aligned");

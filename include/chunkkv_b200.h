@@ -414,7 +414,7 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
  * leaves no other), for a weight of 0 does not silence a NaN in a row that shares a tile.  Weights
  * meet the codes in fp16, relative to the largest value scale of the keys worked on together:
  * an output is exact to 2^-31 of the largest value there, so a row that sees only values smaller
- * than 2^-20 of it loses bits.  `scale` is finite and not negative (a negative one is refused).
+ * than 2^-20 of it loses bits.  `scale` is 0 to 2e38 (any other is refused).
  * At most 128 query heads per KV head, head_dim 64 or 128, m * n_q_heads at most 2^31 - 2^20.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
  * 0) needs no initialisation; calls that share one must not overlap on the GPU. */
 CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);

@@ -95,3 +95,17 @@ def test_launches_count_every_run():
         runs = 1 if few else -(-m // (size // per_token))
         assert lib.ckv_block_select_launches(m, Hq, H, D, n) == (1 if few else 2 * runs)
     assert lib.ckv_block_select_launches(5000, 28, 4, 128, 131072) == 6
+
+
+@pytest.mark.parametrize("scale", [2.5e38, 3.4e38, float("inf"), -1e-30, float("nan")])
+@pytest.mark.parametrize("m,n", [(1, 100), (100, 6000)])  # streamed, in tiles
+def test_softmax_scales_out_of_range(scale, m, n):
+    """Past 2e38 the scale leaves fp32 in the log2 domain: refused by every form."""
+    lib = _lib.load()
+    assert (lib.ckv_attention_kv8_splits(m, 28, 4, 128, n) > 0) == (m > 1)
+    with pytest.raises(ValueError, match="scale"):
+        _lib.call("ckv_attention_kv8", *(P,) * 7, m, 28, 4, 128, n, scale, 0, P, BIG, None)
+    with pytest.raises(ValueError, match="scale"):
+        _lib.call("ckv_attention_blocks_kv8", *(P,) * 8, m, 28, 4, 128, n, 4, scale, 0, P, BIG, None)
+    with pytest.raises(ValueError, match="scale"):
+        _lib.call("ckv_attention_blocks", *(P,) * 6, m, 28, 4, 128, n, 4, scale, P, BIG, None)
