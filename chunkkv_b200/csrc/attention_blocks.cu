@@ -398,7 +398,9 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
   // Behind the selection only the lists (and the output) wait for the kernel before: every CTA of
   // it lets this kernel start after its own wait, so q and the positions, written before the selection
   // began, are in L2 by then.  They are read there (ld.cg): a line of them that L1 still held
-  // from an earlier kernel would be older.  (One row, 64 of 2056 blocks: 13.1 us, behind the wait 13.6.)
+  // from an earlier kernel would be older.  (Over a whole cache they come through L1: up to twelve warps
+  // read the same rows, and past it one row over 5248 tokens took 9.5 us instead of 9.3.)  One row and
+  // 64 of 2056 blocks take 13.1 us, with q and the positions behind the wait 13.6.
   if (!a.after_select) pdl_wait();
   // as an operand owner a lane has query rows 8n + g: q and their positions first
   uint32_t w[NT][HD / 8];  // the dims of this lane's pieces of K (16 / ES dims each)
@@ -410,9 +412,12 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
 #pragma unroll
     for (int e = 0; e < HD / 8; e += 4) {
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (ok)
-        x = __ldcg(reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
-                  (B::ES == 2 ? e + c : 8 * (e / 8) + 2 * c + (e / 4) % 2));
+      if (ok) {
+        const uint4* at = reinterpret_cast<const uint4*>(a.q + (int64_t(tok) * a.Hq + hk * G + (pr - tok * G)) * HD) +
+                          (B::ES == 2 ? e + c : 8 * (e / 8) + 2 * c + (e / 4) % 2);
+        if constexpr (LISTED) x = __ldcg(at);
+        else x = __ldg(at);
+      }
       w[n][e] = x.x, w[n][e + 1] = x.y, w[n][e + 2] = x.z, w[n][e + 3] = x.w;
     }
   }
@@ -423,7 +428,8 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     const int pr = row0 + 8 * n + g;
     int p = -1;
     if (pr < row_end) {
-      p = __ldcg(a.positions + pr / G);
+      if constexpr (LISTED) p = __ldcg(a.positions + pr / G);
+      else p = a.positions[pr / G];
       if (p >= a.n_ctx) {
         if (split == 0 && hk == 0) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
         p = a.n_ctx - 1;
