@@ -238,3 +238,24 @@ def test_long_lists(Hq, H, D, n, m, top):
     out, blocks = sparse(q, p, top)
     assert torch.equal(blocks.cpu().long(), ref.select(q, d.codes, d.scale, p, top))
     check_attention(out[:4], q[:4], kd, vd, p[:4], blocks[:4])
+
+
+# --------------------------------------------------------------------- very large and small
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Hq,H,D,n,m", [(28, 4, 128, 1500, 1), (28, 4, 128, 9000, 1), (28, 4, 128, 700, 4), (28, 4, 128, 640, 200),
+                                        (14, 2, 64, 2500, 100)])
+@pytest.mark.parametrize("size", [-95, 96])
+def test_very_large_and_small_values(Hq, H, D, n, m, size, dtype):
+    """V near the ends of what a call takes (the largest value times the keys below 2^113), and keys and
+    queries whose products are ordinary though neither is."""
+    k, v, q = filled(H, n, D, dtype, seed=3)[1:] + (queries(m, Hq, D, 1),)
+    c = ops.KV8Cache(H, n, D, dtype, DEV, digest=True)
+    ops.kv8_write(c, (k.float() * 2.0 ** -size).to(BF), (v.float() * 2.0 ** size).to(BF), 0)
+    assert float(ref.values(c.v.float(), c.v_scale).abs().max()) * n < 2.0 ** 113
+    q = (q.float() * 2.0 ** size).to(BF)
+    p = torch.linspace(n - 1, n // 2, m, device=DEV).to(torch.int32)
+    kd, vd = ref.values(c.k.float(), c.k_scale), ref.values(c.v.float(), c.v_scale)
+    check_attention(ops.attention_kv8(q, c, p), q, kd, vd, p)
+    out, blocks = ops.attention_sparse_kv8(q, c, p, 12)
+    assert torch.equal(blocks.cpu().long(), ref.select(q, c.digest.codes, c.digest.scale, p, 12))
+    check_attention(out, q, kd, vd, p, blocks)
