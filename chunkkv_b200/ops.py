@@ -1001,8 +1001,8 @@ def attention_kv8(q: torch.Tensor, cache: KV8Cache, positions: torch.Tensor, out
 # ------------------------------------------------ attention over selected blocks
 def block_select(q: torch.Tensor, digest: BlockDigest, positions: torch.Tensor, top: int, sink: int = 1,
                  recent: int = 1, out: torch.Tensor | None = None, m: int | None = None) -> torch.Tensor:
-    """For every row of q [m, Hq, D] and KV head the `top` blocks of 16 keys whose score (an upper
-    bound of q . k, from the digest) is highest, the first `sink` and the last `recent` visible
+    """For every row of q [m, Hq, D] and KV head the `top` blocks of 16 keys whose score (a bound
+    of q . k from the digest, from above but for the rounding to 8 bits) is highest, the first `sink` and the last `recent` visible
     blocks always among them; int32 [m, H, top], ascending, -1 past a row's last visible block."""
     H, D = digest.n_kv_heads, digest.head_dim
     m, Hq = _query(q, H, D, positions, m)

@@ -409,14 +409,17 @@ CKV_API int ckv_block_digest(const uint16_t* k, int64_t head_stride, int64_t row
 
 /* ckv_attention over the 8-bit cache: q/out [m][Hq][D] bf16, key j visible to row i iff
  * j <= positions[i]; a row whose position is negative sees no key and gives zeros, one at or
- * past n_ctx sees every key (recorded).  NaN in a row of q makes that row of out NaN.  Codes and scales past every row's position may hold
- * anything; codes some row sees must be finite and scales 0 or in [2^-110, 2^120] (ckv_kv8_write
- * leaves no other), for a weight of 0 does not silence a NaN in a row that shares a tile.  Weights
- * meet the codes in fp16, relative to the largest value scale of the keys worked on together:
- * an output is exact to 2^-31 of the largest value there, so a row that sees only values smaller
- * than 2^-20 of it loses bits.  `scale` is 0 to 2e38 (any other is refused).
- * At most 128 query heads per KV head, head_dim 64 or 128, m * n_q_heads at most 2^31 - 2^20.  `workspace` (16-byte aligned, of ckv_attention_kv8_workspace_size() bytes, which may be
- * 0) needs no initialisation; calls that share one must not overlap on the GPU. */
+ * past n_ctx sees every key (recorded).  NaN in a row of q makes that row of out NaN.  Codes and
+ * scales past every row's position may hold anything; codes some row sees must be finite and
+ * scales 0 or in [2^-110, 2^122] (ckv_kv8_write leaves no other), for a weight of 0 does not
+ * silence a NaN in a row that shares a tile.  Sums are taken before the division by the weights' sum:
+ * the largest |value| of V times the keys of a row must stay below 2^113.  Weights meet the codes
+ * in fp16, relative to the largest value scale of the keys worked on together: besides its rounding
+ * (2^-12) a key's part in an output is off by up to 2^-30 of the largest value there, so a row that
+ * sees only values smaller than 2^-20 of it loses bits.  `scale` is 0 to 2e38 (any other is refused).  At most 128 query heads per KV head,
+ * head_dim 64 or 128, m * n_q_heads at most 2^31 - 2^20.  `workspace` (16-byte aligned, of
+ * ckv_attention_kv8_workspace_size() bytes, which may be 0) needs no initialisation; calls that
+ * share one must not overlap on the GPU. */
 CKV_API int64_t ckv_attention_kv8_workspace_size(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
 /* Kernels one ckv_attention_kv8 call launches at this shape (0 for a shape it refuses). */
 CKV_API int ckv_attention_kv8_launches(int m, int n_q_heads, int n_kv_heads, int head_dim, int n_ctx);
@@ -430,9 +433,9 @@ CKV_API int ckv_attention_kv8(const uint16_t* q, const uint8_t* k8, const uint8_
 
 /* ---- attention over selected blocks -----------------------------------------
  * For every query token and KV head the `top` blocks of 16 keys that a cheap score ranks
- * best: the first `sink` and the last `recent` visible blocks always, the others by score (an
- * upper bound of q . k over the block from its digest and the query's 8-bit codes, the best
- * head of the group), equal scores to the lower block.  blocks [m][H][top] int32, ascending, -1
+ * best: the first `sink` and the last `recent` visible blocks always, the others by score (a
+ * bound of q . k over the block from its digest and the query's 8-bit codes, from above but for
+ * the rounding of both to 8 bits; the best head of the group), equal scores to the lower block.  blocks [m][H][top] int32, ascending, -1
  * past a row's last visible block.  At most 16 query heads per KV head, contexts up to 524,288
  * tokens, sink + recent <= top <= 4096, recent >= 1.  The workspace (16-byte aligned, 0
  * bytes for few rows) needs no initialisation. */
