@@ -370,10 +370,12 @@ struct Layout {
 // grid: (splits, row tiles, KV heads).  Dense (LISTED = false): tile y holds the packed rows
 // (token, head of the group) [8 NT y, 8 NT (y + 1)) of its KV head.  Listed: tile y is head
 // tile y % head_tiles of token y / head_tiles, and the split takes its share of the list.
+// Four CTAs of listed 8-bit blocks share an SM (128 registers: 938 rows of 64 blocks 174 us; three CTAs
+// of 136 registers 199); over a bf16 cache three do, by shared memory.
 // JOIN: the kCluster splits of a tile are one cluster and leave finished rows; otherwise more
 // than one split leaves partials for attention_blocks_join_kernel.
 template <int HD, int CT, int NT, bool LISTED, int W, bool JOIN>
-__global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
+__global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : CT == kBf16 ? 3 : 4)
     attention_blocks_kernel(const __grid_constant__ Args a) {
   using L = Layout<HD, CT, NT, W, LISTED>;
   using B = Block<HD, CT, LISTED>;
@@ -460,12 +462,6 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
     }
     return b < nb ? b : -1;  // wholly past the row's position: nothing visible
   };
-  if constexpr (LISTED) {
-    // an ascending list ends before its entry `items`, and no split takes those from there on
-    if (a.top > a.items && split == 0)
-      for (int i = a.items + threadIdx.x; i < a.top; i += W * 32)
-        if (list[i] != -1) atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
-  }
   uint8_t* ring = smem + warp * L::RING;
   constexpr int NB = B::NB;
   int ids[L::STAGES][NB];                           // blocks in the ring, -1: none
@@ -663,6 +659,15 @@ __global__ void __launch_bounds__(W * 32, W > 4 ? 1 : NT == 2 ? 2 : 3)
       store_row(row0 + row, col, o, l);
     }
     cluster_sync();  // no CTA leaves while its shared memory is read
+  }
+  if constexpr (LISTED) {
+    // An ascending list ends before its entry `items`, and no split takes those from there on: one that
+    // is not -1 is recorded.  (Last, where it holds no registers: in front of the loop it cost a CTA
+    // per SM at head_dim 64, 863 rows of 23 blocks 26.3 us against 24.4.)
+    if (a.top > a.items && blockIdx.x == 0)
+      for (int i = a.items + threadIdx.x; i < a.top; i += W * 32)
+        if (a.blocks[(int64_t(blockIdx.y / a.head_tiles) * a.Hk + blockIdx.z) * a.top + i] != -1)
+          atomicOr(&g_err_word, CKV_DEV_ERR_POSITION_RANGE);
   }
 }
 
@@ -898,9 +903,9 @@ struct Call {
   Plan plan() const { return ckv::plan(a.m, a.Hq / a.Hk, a.Hk, HD, type < 0 ? 2 : 1, a.items, true); }
 };
 
-Call bf16_call(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* positions,
-                      const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top, float scale,
-                      void* workspace, int64_t ws_bytes, bool after_select) {
+Call bf16_call(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache, const int32_t* positions, const int32_t* blocks,
+               uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top, float scale, void* workspace, int64_t ws_bytes,
+               bool after_select) {
   return {{q, reinterpret_cast<const uint8_t*>(k_cache), reinterpret_cast<const uint8_t*>(v_cache), nullptr, nullptr, positions, blocks,
            out, nullptr, nullptr, int64_t(n_ctx), m, Hq, Hk, n_ctx, ceil_div(n_ctx, kBlk), top, list_items(top, n_ctx), 1, 1,
            scale * 1.4426950408889634f, after_select},
@@ -908,8 +913,8 @@ Call bf16_call(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cac
 }
 
 Call kv8_call(const uint16_t* q, const uint8_t* k8, const uint8_t* v8, const float* k_scale, const float* v_scale,
-                     const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top,
-                     float scale, int type, void* workspace, int64_t ws_bytes, bool after_select) {
+              const int32_t* positions, const int32_t* blocks, uint16_t* out, int m, int Hq, int Hk, int HD, int n_ctx, int top,
+              float scale, int type, void* workspace, int64_t ws_bytes, bool after_select) {
   const int nb = ceil_div(n_ctx, kBlk);
   return {{q, k8, v8, k_scale, v_scale, positions, blocks, out, nullptr, nullptr, int64_t(nb) * kBlk, m, Hq, Hk, n_ctx, nb, top,
            list_items(top, n_ctx), 1, 1, scale * 1.4426950408889634f, after_select},

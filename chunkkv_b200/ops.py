@@ -794,7 +794,8 @@ class KV8Cache:
              tail: torch.Tensor | None = None, tail_start: int = 0, digest: BlockDigest | None = None) -> "KV8Cache":
         """A cache over buffers that the caller owns.  `tail`, where given, holds the bf16 rows
         of the block in progress when the cache holds `tail_start` tokens; without it a write into
-        that block takes the earlier rows from their codes."""
+        that block takes the earlier rows from their codes, as does one that goes back into the
+        block before it until another has been filled."""
         c = cls.__new__(cls)
         c._set(k, v, k_scale, v_scale, n_ctx, tail, tail_start, digest)
         return c
@@ -826,7 +827,7 @@ class KV8Cache:
         self.k, self.v, self.k_scale, self.v_scale, self.tail, self.digest = k, v, k_scale, v_scale, tail, digest
         end = int(tail_start) if tail_start % PAGE_TOKENS else 0
         self.tail_end = torch.full((2, H), end, dtype=torch.int32, device=k.device)
-        self.prev, self.prev_end = torch.zeros_like(tail), torch.zeros_like(self.tail_end)
+        self.prev, self.prev_end = torch.empty_like(tail), torch.zeros_like(self.tail_end)  # read only where prev_end says
         self.n_ctx, self.n_kv_heads, self.head_dim, self.dtype = int(n_ctx), H, D, k.dtype
 
     @property
