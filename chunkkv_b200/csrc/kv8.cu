@@ -83,6 +83,11 @@ __device__ __forceinline__ uint32_t value2(uint32_t two, float scale) {
   }
   return pack_bf2(__fmul_rn(a, scale), __fmul_rn(b, scale));
 }
+// 16 bytes from global to shared memory, past L1 and the registers; complete after cp_async_wait
+__device__ __forceinline__ void cp_async16(uint4* dst, const uint16_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ uint32_t bmax2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -96,10 +101,12 @@ __device__ __forceinline__ uint32_t bmin2(uint32_t a, uint32_t b) {
 // One warp per (block, K | V, head): the whole block sits in the warp's registers (16 bytes
 // per lane and pass, 4 KiB at head_dim 128, all loads in flight together), so the rows are
 // read once, and nothing goes through shared memory.  CT == kNone keeps only the digest.
-// Bound by HBM: 131,069 tokens of 8 heads (805 MB) 133 us, 6.1 TB/s; a prompt of 5248 tokens, whose
-// rows are in L2, 4.0 us, and one token 2.7 us in a graph, the latency of a launch and of the tail's rows.
+// Bound by HBM: 131,069 tokens of 8 heads with K's digest (825 MB) 137 us, 6.0 TB/s; a prompt of 5248
+// tokens, whose rows are in L2, 3.9 us, and one token 2.4 us in a graph, the latency of a launch and of
+// the tail's rows.  Five CTAs per SM (96 registers): left to the compiler, or with six, 147 and 4.2 us.  (The digest
+// alone and head_dim 64 fit more of them.)
 template <int HD, int CT>
-__global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_constant__ WriteArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, HD == 128 && CT != kNone ? 5 : 1) kv8_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int LPR = HD / 8;            // lanes per row
   constexpr int RPP = 32 / LPR;          // rows per pass
   constexpr int PASSES = kRows / RPP;    // 8 at HD = 128, 4 at HD = 64
@@ -121,66 +128,89 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_write_kernel(const __grid_con
   const int r0 = lane / LPR, col = (lane % LPR) * 8;
   const uint16_t* src = a.src[side] + h * a.head_stride[side];
   const int64_t blk = int64_t(h) * a.n_blocks + b;
-  const uint16_t* held = nullptr;  // this block's rows, where the tail or the block before it is this one
-  int n_held = 0, prev_end = 0;
+  int te = 0, prev_end = 0;  // what the tail and the block before it hold
   if (CT != kNone && bi == 0) {
     const int64_t at = int64_t(side) * a.H + h;
-    const int te = a.tail_end[at];
+    te = a.tail_end[at];
     if (a.prev != nullptr) prev_end = a.prev_end[at];
-    if (te > 0 && te / kRows == b) held = a.tail + at * kRows * HD, n_held = te % kRows;
-    else if (prev_end == (b + 1) * kRows) held = a.prev + at * kRows * HD, n_held = kRows;
   }
   uint4 x[PASSES];
+  const uint16_t* row0 = src + (int64_t(b) * kRows + r0 - (a.by_position ? 0 : start)) * a.row_stride[side] + col;
+  if (CT == kNone || old == 0) {
 #pragma unroll
-  for (int p = 0; p < PASSES; ++p) {
-    const int r = p * RPP + r0;
-    x[p] = make_uint4(0u, 0u, 0u, 0u);
-    if (r < rows) {
-      if (r >= old || CT == kNone) {
-        const int64_t t = int64_t(b) * kRows + r - (a.by_position ? 0 : start);
-        x[p] = __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
-      } else if (r < n_held) {
-        x[p] = *reinterpret_cast<const uint4*>(held + r * HD + col);
-      } else if (CT != kNone) {
-        // a write that goes back into an earlier block: its rows from the codes
-        const uint2 c = *reinterpret_cast<const uint2*>(a.codes[side] + (blk * kRows + r) * HD + col);
-        const float sc = a.scale[side][blk];
-        x[p] = make_uint4(value2<CT>(c.x, sc), value2<CT>(c.x >> 16, sc), value2<CT>(c.y, sc),
-                          value2<CT>(c.y >> 16, sc));
-      }
+    for (int p = 0; p < PASSES; ++p)
+      x[p] = p * RPP + r0 < rows ? __ldg(reinterpret_cast<const uint4*>(row0 + p * RPP * a.row_stride[side])) : make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    // earlier rows from the tail, whether or not it holds this block: all loads are in flight together
+    const uint16_t* tail0 = a.tail + ((int64_t(side) * a.H + h) * kRows + r0) * HD + col;
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int r = p * RPP + r0;
+      const uint16_t* from = r < old ? tail0 + p * RPP * HD : row0 + p * RPP * a.row_stride[side];
+      x[p] = r < rows ? *reinterpret_cast<const uint4*>(from) : make_uint4(0u, 0u, 0u, 0u);
     }
   }
-  // (called last, or before the repairs below: in front of the sums it would hold everything up,
-  // 5248 tokens 4.0 us against 4.9)
-  auto keep_rows = [&] {
-    // The rows of the block in progress stay in the tail and those of the block before it in prev,
-    // as they came: what stands for an infinity goes by the block's largest value, which later rows
-    // may raise.  A write that begins a block reads neither, so each of the two blocks' warps
-    // keeps its own rows; else the warp that reads them writes them, and no other warp can see
-    // them half replaced.
-    const int keep = end % kRows, bl = end / kRows;
-    const int64_t at = int64_t(side) * a.H + h;
-    uint16_t *tail = a.tail + at * kRows * HD, *prev = a.prev + at * kRows * HD;
-    if (start % kRows == 0 || bl == b0) {
-      if (b == bl || (b == bl - 1 && a.prev != nullptr)) {
-        uint16_t* slot = b == bl ? tail : prev;
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-          const int r = p * RPP + r0;
-          if (r < rows) *reinterpret_cast<uint4*>(slot + r * HD + col) = x[p];
-        }
-      }
-    } else if (bi == 0) {
-      auto row_of = [&](int block, int p) {  // row p * RPP + r0 of this block or of one that is all new
-        if (block == b) return x[p];
-        const int64_t t = int64_t(block) * kRows + p * RPP + r0 - (a.by_position ? 0 : start);
-        return __ldg(reinterpret_cast<const uint4*>(src + t * a.row_stride[side] + col));
-      };
+  if constexpr (CT != kNone) {
+    const int held = te > 0 && te / kRows == b ? te % kRows : 0;
+    if (held < old) {
+      // a write that goes back: from the block before the tail's, or the values of the codes
+      const bool whole = prev_end == (b + 1) * kRows && held == 0;
 #pragma unroll
       for (int p = 0; p < PASSES; ++p) {
         const int r = p * RPP + r0;
-        if (r < keep) *reinterpret_cast<uint4*>(tail + r * HD + col) = row_of(bl, p);
-        if (a.prev != nullptr) *reinterpret_cast<uint4*>(prev + r * HD + col) = row_of(bl - 1, p);
+        if (r < old && r >= held) {
+          if (whole) {
+            x[p] = *reinterpret_cast<const uint4*>(a.prev + ((int64_t(side) * a.H + h) * kRows + r) * HD + col);
+          } else {
+            const uint2 c = *reinterpret_cast<const uint2*>(a.codes[side] + (blk * kRows + r) * HD + col);
+            const float sc = a.scale[side][blk];
+            x[p] = make_uint4(value2<CT>(c.x, sc), value2<CT>(c.x >> 16, sc), value2<CT>(c.y, sc), value2<CT>(c.y >> 16, sc));
+          }
+        }
+      }
+    }
+  }
+  // The rows of the block in progress stay in the tail and those of the block before it in prev, as
+  // they came: what stands for an infinity goes by the block's largest value, which later rows may
+  // raise.  A write that begins a block reads neither, so each of the two blocks' warps keeps its
+  // own rows; else the warp that reads them writes them, so that no other warp can see them half
+  // replaced, and rows of later blocks come to it through shared memory under the rest of its work
+  // (248 tokens from the middle of a block 4.4 us, loaded at the end 6.1).
+  const int keep = end % kRows, bl = end / kRows;
+  const bool passed_on = CT != kNone && bi == 0 && start % kRows != 0 && bl != b;
+  [[maybe_unused]] uint4* stage = nullptr;
+  if constexpr (CT != kNone) {
+    __shared__ uint4 s_rows[kWarps][2][PASSES * 32];
+    stage = s_rows[threadIdx.x >> 5][0];
+    if (passed_on) {
+#pragma unroll 1  // few instructions and registers, for a path that long writes take once per head
+      for (int p = 0; p < PASSES; ++p) {
+        const int r = p * RPP + r0;
+        const uint16_t* row = src + (int64_t(bl) * kRows + r - (a.by_position ? 0 : start)) * a.row_stride[side] + col;
+        if (r < keep) cp_async16(&stage[p * 32 + lane], row);
+        if (a.prev != nullptr && bl - 1 != b) cp_async16(&stage[(PASSES + p) * 32 + lane], row - kRows * a.row_stride[side]);
+      }
+    }
+  }
+  // (called last, or before the repairs below: in front of the sums it would hold everything up)
+  auto keep_rows = [&] {
+    const int64_t at = int64_t(side) * a.H + h;
+    uint16_t *tail = a.tail + at * kRows * HD, *prev = a.prev + at * kRows * HD;
+    if ((b == bl || (b == bl - 1 && a.prev != nullptr)) && (start % kRows == 0 || bi == 0)) {
+      uint16_t* slot = b == bl ? tail : prev;
+#pragma unroll
+      for (int p = 0; p < PASSES; ++p) {
+        const int r = p * RPP + r0;
+        if (r < rows) *reinterpret_cast<uint4*>(slot + r * HD + col) = x[p];
+      }
+    }
+    if (passed_on) {
+      cp_async_wait();  // a lane reads back what it copied itself
+#pragma unroll 1
+      for (int p = 0; p < PASSES; ++p) {
+        const int r = p * RPP + r0;
+        if (r < keep) *reinterpret_cast<uint4*>(tail + r * HD + col) = stage[p * 32 + lane];
+        if (a.prev != nullptr && bl - 1 != b) *reinterpret_cast<uint4*>(prev + r * HD + col) = stage[(PASSES + p) * 32 + lane];
       }
     }
     if (bi == 0 && lane == 0) {
