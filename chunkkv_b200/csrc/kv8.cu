@@ -25,7 +25,7 @@ namespace ckv {
 namespace {
 
 constexpr int kRows = CKV_PAGE_TOKENS;  // tokens per block
-constexpr int kWarps = 4;  // 131,069 tokens, 8 heads: 133 us (6.1 TB/s); 2, 8, 16 warps per CTA 147, 156, 173
+constexpr int kWarps = 4;  // 131,069 tokens, 8 heads: 126 us (6.4 TB/s); when chosen 133, with 2, 8, 16 warps per CTA 147, 156, 173
 constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
 enum { kNone = 0, kInt8 = 1, kE4m3 = 2 };
 
